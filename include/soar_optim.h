@@ -153,6 +153,108 @@ SOAR_API void soar_sgd_default_opts(soar_sgd_opts* out);
 SOAR_API int soar_sgd_create(const soar_tensor_desc* tensors, int n_tensors,
                              const soar_sgd_opts* opts, void** out_handle);
 
+/* ---- Matrices: orthogonalisation and Muon ---------------------------------
+   No counterpart in the reference. For a matrix G with shorter side m:
+     X = G / (|G|_F + eps); `steps` times: A = X X^T, X <- a X + (b A + c A A) X
+   (on the shorter side; the transpose of a matrix gives the transpose of its
+   result), which drives every singular value that is not tiny to about 1. A
+   matrix of zeros gives zeros; one with an inf or NaN gives NaN throughout.
+   The products run with fp16 operands (11 bits, scaled by powers of two) and
+   fp32 sums, X being carried in 22 bits: 0.03 % to 0.2 % off in norm. Where
+   the result is fp32 (fp32 destinations, SOAR_LAYOUT_FP32) every product is
+   taken in three parts, about as exact as fp32 products. Sides are at most
+   1048576. The same inputs give the same bits. */
+#define SOAR_NS_MAX_STEPS 16
+
+enum soar_dtype {
+    SOAR_DTYPE_FP32 = 0,
+    SOAR_DTYPE_BF16 = 1
+};
+
+/* A stack of `count` rows x cols matrices. Elements of a row are adjacent;
+   strides are in elements: `*_row` between rows, `*_mat` between matrices. */
+typedef struct soar_matrix_desc {
+    const void* src;    /* device; read only */
+    void* dst;          /* device; may be src itself (same type and strides) */
+    uint64_t count, rows, cols;
+    uint64_t src_row, src_mat;
+    uint64_t dst_row, dst_mat;
+} soar_matrix_desc;
+
+/* Fill with soar_ortho_default_opts() first. */
+typedef struct soar_ortho_opts {
+    int32_t steps;      /* 5; 1 .. SOAR_NS_MAX_STEPS */
+    float coef[SOAR_NS_MAX_STEPS][3]; /* a, b, c of each step: 3.4445, -4.7750, 2.0315 */
+    float eps;          /* 1e-7 */
+    int32_t src_type;   /* enum soar_dtype: of every source, default FP32 */
+    int32_t dst_type;   /* of every destination, default BF16 */
+    int32_t device;     /* CUDA device ordinal of every buffer; default 0 */
+} soar_ortho_opts;
+
+SOAR_API void soar_ortho_default_opts(soar_ortho_opts* out);
+/* Plans the orthogonalisation of a list of stacks (a stack without elements is
+   left alone) and allocates its workspace: 8 bytes per element and 4 per
+   element of the m x m products (8 with fp32 destinations). Buffers are bound
+   as the optimizer's are. */
+SOAR_API int soar_ortho_create(const soar_matrix_desc* mats, int n_mats,
+                               const soar_ortho_opts* opts, void** out_handle);
+/* Enqueues one orthogonalisation of every matrix on `stream`; never
+   synchronises the host; may be captured into a CUDA graph. Runs of one handle
+   share its workspace: order them on one stream (or by events), its captured
+   graphs included. */
+SOAR_API int soar_ortho_run(void* handle, void* stream);
+/* Nonzero in *out_error if a device-side wait of some run timed out: that
+   run's results must not be used (synchronises the device). */
+SOAR_API int soar_ortho_error(void* handle, int* out_error);
+SOAR_API int soar_ortho_destroy(void* handle);
+
+/* The shape of a parameter tensor: a contiguous stack of `count` rows x cols
+   matrices (a plain weight: count 1), each updated by itself. */
+typedef struct soar_matrix_shape {
+    uint64_t count, rows, cols;
+} soar_matrix_shape;
+
+/* The factor s of Muon's update, by a matrix's shape. */
+enum soar_muon_scale {
+    SOAR_MUON_SCALE_NONE = 0,   /* 1 */
+    SOAR_MUON_SCALE_ASPECT = 1, /* sqrt(max(1, rows / cols)) */
+    SOAR_MUON_SCALE_RMS = 2     /* 0.2 sqrt(max(rows, cols)): updates of AdamW's usual rms */
+};
+
+/* Muon on the same device step: momentum, orthogonalised by Newton-Schulz
+   products, as the direction of a decoupled-weight-decay update. Per tensor
+   with a gradient g (unscaled, clipped):
+     m <- momentum m + g;  u = g + momentum m (nesterov) or m;  O = NS(u)
+     w <- w - lr weight_decay w;  w <- w - lr s O
+   The handle works with every soar_optim_* call as an AdamW handle does (step,
+   zero_grad, clip, lr, info, state: MASTER and M, gradient sets, checkpoint,
+   EMA, grad_sumsq / apply, destroy). Not with soar_zero1_create: a shard of
+   the flat buffers does not hold whole matrices. Fill with
+   soar_muon_default_opts() first. */
+typedef struct soar_muon_opts {
+    float lr;               /* 2e-2 */
+    float momentum;         /* 0.95 */
+    float weight_decay;     /* 0: for callers; create() takes each tensor's own */
+    int32_t nesterov;       /* 1 */
+    int32_t scale;          /* enum soar_muon_scale, default ASPECT */
+    int32_t steps;          /* 5 */
+    float coef[SOAR_NS_MAX_STEPS][3];
+    float eps;              /* 1e-7 */
+    int32_t layout;
+    float max_grad_norm;
+    int32_t use_loss_scaler;
+    float init_scale;
+    float growth_factor;
+    float backoff_factor;
+    int32_t growth_interval;
+    int32_t device;
+} soar_muon_opts;
+
+SOAR_API void soar_muon_default_opts(soar_muon_opts* out);
+/* shapes[i]: tensor i's shape; its product must be tensors[i].numel. */
+SOAR_API int soar_muon_create(const soar_tensor_desc* tensors, const soar_matrix_shape* shapes,
+                              int n_tensors, const soar_muon_opts* opts, void** out_handle);
+
 SOAR_API int soar_optim_destroy(void* handle);
 
 /* Replaces AdamW::step() (adamw.cpp:60-117) -- and, with max_grad_norm > 0,
@@ -267,7 +369,8 @@ SOAR_API int soar_optim_use_grads(void* handle, int set);
 /* Which update kernel this optimizer's steps launch (*out_path): 0 = the
    bulk-copy pipeline (k_apply), 1 = the register-fed single-pass kernel for
    short lists (k_apply_direct: at most 4 tensors with a vector part and at
-   most 16M elements (16 x 2^20), no weight EMA, AdamW). Both compute the same bits. */
+   most 16M elements (16 x 2^20), no weight EMA, AdamW), both with the same bits;
+   2 = the matrix kernels (Muon). */
 SOAR_API int soar_optim_kernel_path(void* handle, int* out_path);
 
 /* Device address of the live loss scale (fp32), for scaling the loss on the

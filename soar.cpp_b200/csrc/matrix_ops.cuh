@@ -1,0 +1,182 @@
+// Orthogonalisation of lists of matrices by Newton-Schulz products, and the
+// Muon step built on it: structures shared by the kernels (matrix_kernels.cu)
+// and the host code that plans them (matrix_plan.cu).
+//
+// For a matrix G with shorter side m and longer side n (transposed where it
+// has more rows than columns, so that X is m x n):
+//   X = G / (|G|_F + eps);  per iteration:  A = X X^T,  B = b A + c A A,
+//   X <- a X + B X.
+//
+// Numbers: the products run on the tensor cores with fp16 operands and fp32
+// sums. X is kept as hi + lo, two fp16 numbers of 11 bits each, and a X is
+// taken from both; only the operands of products are rounded to hi. A rounding
+// of X's small singular directions would otherwise grow by a factor of a (3.4)
+// per iteration: with X in hi alone, a matrix of a few strong directions over
+// noise comes out 0.6 % to 7 % off (bf16 operands: 5 % to 60 %), with hi + lo
+// 0.03 % to 0.2 %. That is below the rounding of a bf16 result (0.17 % rms).
+// For fp32 results every product is taken as hi hi + hi lo + lo hi of both
+// operands (22 bits).
+//
+// fp16's range is met by powers of two: X is held times sx = 2^floor(log2 sqrt(m n))
+// (within 2^6 .. 2^12), which gives its elements an rms of about 1 at the start
+// and of at most sqrt(m) at the end; A and B are held times 2^10, where their
+// eigenvalues (at most about 1.5, and 3) stay below 2^12 and entries down to
+// 2^-34 still count.
+#pragma once
+
+#include <cstdint>
+#include <string>
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "optim_kernels.cuh"
+
+namespace soarb {
+
+constexpr int kNsMaxSteps = 16;
+constexpr float kNsScaleA = 1024.0f;  // A and B are held times this
+
+// Tile of a product: kNsTileM rows by at most kNsTileN columns, kNsTileK deep per stage.
+constexpr int kNsTileM = 128;
+constexpr int kNsTileN = 256;
+constexpr int kNsTileK = 64;
+constexpr int kNsStages = 4;
+constexpr int kNsThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
+constexpr uint32_t kNsStageBytes = (kNsTileM + kNsTileN) * kNsTileK * 2;
+constexpr size_t kNsSmemBytes = static_cast<size_t>(kNsStages) * kNsStageBytes + 1024;
+
+// Tensor maps of a stack: {X hi 0, X hi 1, A hi, B hi, X lo 0, X lo 1, A lo, B lo}.
+enum NsMap { kMapX0 = 0, kMapX1 = 1, kMapA = 2, kMapB = 3, kMapLo = 4, kMapsPerStack = 8 };
+
+// One stack of equal matrices.
+struct NsStack {
+    __half* x[2];   // X hi, double-buffered across iterations: [count][m][ldx]
+    __half* xl[2];  // X lo
+    __half* a;      // [count][m][lda]
+    __half* al;     // (three products only)
+    __half* b;
+    __half* bl;
+    uint32_t m, n;        // shorter and longer side
+    uint32_t ldx, lda;
+    uint32_t rows, cols;  // as the caller has it
+    uint32_t count;
+    uint32_t first;       // index of its first matrix in the plan
+    uint32_t transposed;  // rows > cols: X is the transpose
+    uint32_t tiles;       // preparation tiles per matrix
+    uint32_t first_tile;
+    float sx;             // power of two X is held by
+    // input and output of a plain orthogonalisation; row and matrix strides in elements
+    const void* src;
+    void* dst;
+    uint64_t src_row, src_mat, dst_row, dst_mat;
+    // Muon: contiguous rows x cols matrices
+    void* param;
+    float* master;
+    float* mom;
+    float wd;
+    float factor;         // the update's shape factor s
+    uint32_t tensor;      // index of its tensor in the list (its gradient's place)
+};
+
+// Preparation tile: 64 x 64 elements of one matrix.
+constexpr int kPrepTile = 64;
+struct PrepTile {
+    uint32_t stack;
+    uint32_t index;   // matrix of the stack
+    uint32_t tr, tc;  // tile row and column
+};
+
+// One output tile of one product of one matrix.
+enum NsKind : uint32_t { kNsXXt = 0, kNsAA = 1, kNsBX = 2, kNsLast = 3 };
+struct __align__(16) NsTask {
+    uint32_t stack;
+    uint32_t index;   // matrix of the stack
+    uint32_t need;    // tiles of this matrix that must be done before
+    uint16_t row, col;  // first row and column, in units of 128 and 16
+    uint16_t width;   // columns
+    uint8_t kind;
+    uint8_t step;
+    uint32_t pad[2];
+};
+static_assert(sizeof(NsTask) == 32, "a task is two 16-byte loads");
+
+// A Muon step's decision, from its first kernel for the others.
+struct MatrixStep {
+    int skip;    // nonzero: nothing is updated
+    float inv;   // 1 / loss scale
+    float coef;  // clip coefficient
+};
+
+// What a plan's kernels need, passed by value.
+struct MatrixArgs {
+    const NsStack* stacks;
+    const CUtensorMap* maps;
+    const NsTask* tasks;
+    uint32_t n_tasks;
+    const PrepTile* prep;
+    uint32_t n_prep;
+    uint32_t n_matrices;
+    double* partials;      // one per preparation tile
+    uint32_t* tickets;     // per matrix: preparation tiles summed (0 between launches)
+    float* inv;            // per matrix: sx / (norm + eps)
+    uint32_t* done;        // per matrix: product tiles done
+    uint32_t* next;        // tasks handed out
+    MatrixStep* step;
+    int* err;              // nonzero: a wait ran out
+    float coef[kNsMaxSteps][3];
+    double eps;
+    const void* const* grads;  // Muon: gradient per tensor
+    float momentum;
+    int nesterov;
+    int ema;
+};
+
+enum MatrixSource { kSrcF32 = 0, kSrcBf16 = 1, kSrcGradF32 = 2, kSrcGradBf16 = 3 };
+enum MatrixDest { kDstF32 = 0, kDstBf16 = 1, kDstParamF32 = 2, kDstParamMixed = 3 };
+
+cudaError_t prepare_matrix_kernels();
+// Sum of squares per matrix (and the momentum update of a Muon step, which
+// also takes and commits the step's decision), then the normalised hi + lo
+// split, then all products and the output in one persistent kernel.
+cudaError_t launch_matrix_ops(const MatrixArgs& args, int source, int dest, Ctl* ctl,
+                              const ApplyArgs* step, int sms, cudaStream_t stream);
+
+// ---- host: plans (matrix_plan.cu) ----
+// Whether a stack's shape can be planned (a stack without elements can).
+bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* why);
+// The quintic's usual coefficients, for every step.
+void matrix_default_coef(float (*coef)[3]);
+struct MatrixSpec {
+    const void* src = nullptr;
+    void* dst = nullptr;
+    uint64_t rows = 0, cols = 0, count = 0;
+    uint64_t src_row = 0, src_mat = 0, dst_row = 0, dst_mat = 0;
+    void* param = nullptr;
+    float* master = nullptr;
+    float* mom = nullptr;
+    float wd = 0.0f, factor = 1.0f;
+    uint32_t tensor = 0;
+};
+struct MatrixPlanOpts {
+    int steps = 5;
+    float coef[kNsMaxSteps][3] = {};
+    double eps = 1e-7;
+    int source = kSrcF32, dest = kDstF32;
+    int* err = nullptr;  // error word (nullptr: the plan's own)
+};
+struct MatrixPlan;
+// nullptr on failure, with the reason in *why. The current device's.
+MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n, const MatrixPlanOpts& opts,
+                               std::string* why);
+void matrix_plan_destroy(MatrixPlan* plan);
+cudaError_t matrix_plan_run(MatrixPlan* plan, cudaStream_t stream);
+// One Muon step (the decision from `step` and `ctl`).
+cudaError_t matrix_plan_step(MatrixPlan* plan, Ctl* ctl, const ApplyArgs& step,
+                             const void* const* grads, float momentum, bool nesterov, bool ema,
+                             cudaStream_t stream);
+int* matrix_plan_error_word(MatrixPlan* plan);
+
+}  // namespace soarb

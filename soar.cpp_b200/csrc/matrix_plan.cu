@@ -1,0 +1,354 @@
+// Host side of the matrix operators: plans the preparation tiles, the product
+// tiles and their order, and owns the workspace.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <memory>
+#include <vector>
+
+#include <cudaTypedefs.h>
+
+#include "matrix_ops.cuh"
+
+namespace soarb {
+
+struct MatrixPlan {
+    int sms = 0;
+    int source = 0, dest = 0;
+    MatrixArgs args{};
+    char* slab = nullptr;
+};
+
+namespace {
+
+size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// cuTensorMapEncodeTiled, from the driver through the runtime (the library
+// does not link the driver's own library).
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r{};
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) !=
+            cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+        return nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+}
+
+// A stack of `count` row-major fp16 matrices, in boxes of 64 rows of 64.
+bool encode(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
+            uint32_t cols, uint32_t ld, uint32_t count) {
+    const cuuint64_t dims[3] = {cols, rows, count};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2,
+                                   static_cast<cuuint64_t>(ld) * rows * 2};
+    const cuuint32_t box[3] = {64, 64, 1}, es[3] = {1, 1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tiles of one product of one matrix: (first row / 128, first column / 16, width).
+struct Tile {
+    uint16_t row, col, width;
+};
+std::vector<Tile> symmetric_tiles(uint32_t m, uint32_t wide) {
+    std::vector<Tile> out;
+    for (uint32_t r = 0; r * kNsTileM < m; ++r)
+        for (uint32_t c = r * kNsTileM; c < m; c += wide)
+            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 16),
+                           static_cast<uint16_t>(std::min(wide, m - c))});
+    return out;
+}
+std::vector<Tile> full_tiles(uint32_t m, uint32_t n, uint32_t wide) {
+    std::vector<Tile> out;
+    for (uint32_t c = 0; c < n; c += wide)
+        for (uint32_t r = 0; r * kNsTileM < m; ++r)
+            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 16),
+                           static_cast<uint16_t>(std::min(wide, n - c))});
+    return out;
+}
+
+}  // namespace
+
+bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* why) {
+    constexpr uint64_t kMostSide = 1ull << 20, kMost = 1ull << 38;
+    if (rows > kMostSide || cols > kMostSide) {
+        *why = "a side of more than 1048576";
+        return false;
+    }
+    if (rows && cols && count > kMost / (rows * cols)) {
+        *why = "more than 2^38 elements";
+        return false;
+    }
+    if (count > 0x7FFFFFFFull) {
+        *why = "more than 2^31 - 1 matrices";
+        return false;
+    }
+    return true;
+}
+
+void matrix_default_coef(float (*coef)[3]) {
+    for (int i = 0; i < kNsMaxSteps; ++i) {
+        coef[i][0] = 3.4445f;
+        coef[i][1] = -4.7750f;
+        coef[i][2] = 2.0315f;
+    }
+}
+
+void matrix_plan_destroy(MatrixPlan* p) {
+    if (!p) return;
+    cudaFree(p->slab);
+    delete p;
+}
+
+MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const MatrixPlanOpts& opts,
+                               std::string* why) {
+    auto plan = std::make_unique<MatrixPlan>();
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess)
+        e = cudaDeviceGetAttribute(&plan->sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = prepare_matrix_kernels();
+    if (e != cudaSuccess) {
+        *why = std::string("kernel set-up: ") + cudaGetErrorString(e);
+        return nullptr;
+    }
+    const auto encoder = encode_fn();
+    if (!encoder) {
+        *why = "the driver offers no cuTensorMapEncodeTiled";
+        return nullptr;
+    }
+    plan->source = opts.source;
+    plan->dest = opts.dest;
+    const bool three = opts.dest == kDstF32 || opts.dest == kDstParamF32;
+
+    // stacks, and their places in the workspace
+    std::vector<NsStack> stacks;
+    std::vector<PrepTile> prep;
+    struct Place {
+        size_t x[2], xl[2], a, al, b, bl;
+    };
+    std::vector<Place> places;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = up(off + bytes, 1024);
+        return at;
+    };
+    uint64_t matrices = 0;
+    for (int i = 0; i < n_specs; ++i) {
+        const MatrixSpec& q = specs[i];
+        if (!q.rows || !q.cols || !q.count) continue;
+        NsStack s{};
+        s.rows = static_cast<uint32_t>(q.rows);
+        s.cols = static_cast<uint32_t>(q.cols);
+        s.count = static_cast<uint32_t>(q.count);
+        s.transposed = s.rows > s.cols;
+        s.m = std::min(s.rows, s.cols);
+        s.n = std::max(s.rows, s.cols);
+        s.ldx = static_cast<uint32_t>(up(s.n, 8));
+        s.lda = static_cast<uint32_t>(up(s.m, 8));
+        s.first = static_cast<uint32_t>(matrices);
+        matrices += s.count;
+        const int lg = static_cast<int>(
+            std::floor(0.5 * std::log2(static_cast<double>(s.m) * static_cast<double>(s.n))));
+        s.sx = std::ldexp(1.0f, std::min(12, std::max(6, lg)));
+        s.src = q.src;
+        s.dst = q.dst;
+        s.src_row = q.src_row;
+        s.src_mat = q.src_mat;
+        s.dst_row = q.dst_row;
+        s.dst_mat = q.dst_mat;
+        s.param = q.param;
+        s.master = q.master;
+        s.mom = q.mom;
+        s.wd = q.wd;
+        s.factor = q.factor;
+        s.tensor = q.tensor;
+        const uint32_t tr = (s.rows + kPrepTile - 1) / kPrepTile, tc = (s.cols + kPrepTile - 1) / kPrepTile;
+        s.tiles = tr * tc;
+        s.first_tile = static_cast<uint32_t>(prep.size());
+        for (uint32_t c = 0; c < s.count; ++c)
+            for (uint32_t y = 0; y < tr; ++y)
+                for (uint32_t x = 0; x < tc; ++x)
+                    prep.push_back({static_cast<uint32_t>(stacks.size()), c, y, x});
+        Place p{};
+        const size_t xb = static_cast<size_t>(s.count) * s.m * s.ldx * 2;
+        const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
+        for (int k = 0; k < 2; ++k) {
+            p.x[k] = take(xb);
+            p.xl[k] = take(xb);
+        }
+        p.a = take(ab);
+        p.b = take(ab);
+        if (three) {
+            p.al = take(ab);
+            p.bl = take(ab);
+        }
+        stacks.push_back(s);
+        places.push_back(p);
+    }
+
+    // The tasks, in an order in which every tile's inputs come before it: lists
+    // of matrices whose operands fit in the L2 cache together go through their
+    // products side by side, one such list after another.
+    constexpr uint64_t kWaveBytes = 48ull << 20;
+    std::vector<NsTask> tasks;
+    struct Run {
+        uint32_t stack, from, to;
+    };
+    std::vector<Run> wave;
+    uint64_t wave_bytes = 0;
+    auto flush = [&]() {
+        std::vector<uint32_t> counted(wave.size(), 0);  // tiles of a matrix before this product
+        for (int step = 0; step < opts.steps; ++step) {
+            for (uint32_t kind = kNsXXt; kind <= kNsBX; ++kind) {
+                for (size_t w = 0; w < wave.size(); ++w) {
+                    const NsStack& s = stacks[wave[w].stack];
+                    const std::vector<Tile> tiles =
+                        kind == kNsBX ? full_tiles(s.m, s.n, kNsTileN) : symmetric_tiles(s.m, kNsTileN);
+                    for (uint32_t i = wave[w].from; i < wave[w].to; ++i)
+                        for (const Tile& t : tiles) {
+                            NsTask k{};
+                            k.stack = wave[w].stack;
+                            k.index = i;
+                            k.need = counted[w];
+                            k.row = t.row;
+                            k.col = t.col;
+                            k.width = t.width;
+                            k.kind = static_cast<uint8_t>(
+                                kind == kNsBX && step + 1 == opts.steps ? kNsLast : kind);
+                            k.step = static_cast<uint8_t>(step);
+                            tasks.push_back(k);
+                        }
+                    counted[w] += static_cast<uint32_t>(tiles.size());
+                }
+            }
+        }
+        wave.clear();
+        wave_bytes = 0;
+    };
+    for (uint32_t si = 0; si < stacks.size(); ++si) {
+        const NsStack& s = stacks[si];
+        const uint64_t each = 2ull * s.m * (4ull * s.ldx + (three ? 4ull : 2ull) * s.lda);
+        uint32_t i = 0;
+        while (i < s.count) {
+            const uint64_t room = wave_bytes < kWaveBytes ? (kWaveBytes - wave_bytes) / each : 0;
+            uint32_t k = static_cast<uint32_t>(std::min<uint64_t>(room, s.count - i));
+            if (k == 0) {
+                if (!wave.empty()) {
+                    flush();
+                    continue;
+                }
+                k = 1;
+            }
+            wave.push_back({si, i, i + k});
+            wave_bytes += each * k;
+            i += k;
+        }
+    }
+    flush();
+    if (tasks.size() > 0xFFFF0000ull || prep.size() > 0xFFFF0000ull || matrices > 0xFFFF0000ull) {
+        *why = "too many matrices in one list";
+        return nullptr;
+    }
+
+    // tables behind the operands
+    const size_t operand_bytes = off;
+    const size_t o_stacks = take(stacks.size() * sizeof(NsStack));
+    const size_t o_maps = take(stacks.size() * kMapsPerStack * sizeof(CUtensorMap));
+    const size_t o_tasks = take(tasks.size() * sizeof(NsTask));
+    const size_t o_prep = take(prep.size() * sizeof(PrepTile));
+    const size_t tables_end = off;
+    const size_t o_partials = take(prep.size() * sizeof(double));
+    const size_t o_inv = take(matrices * sizeof(float));
+    const size_t zero_from = off;
+    const size_t o_tickets = take(matrices * sizeof(uint32_t));
+    const size_t o_done = take(matrices * sizeof(uint32_t));
+    const size_t o_words = take(256);
+    if ((e = cudaMalloc(&plan->slab, off)) != cudaSuccess) {
+        plan->slab = nullptr;
+        *why = "matrix workspace (" + std::to_string(off) + " bytes): " + cudaGetErrorString(e);
+        cudaGetLastError();
+        return nullptr;
+    }
+    auto at = [&](size_t o) { return plan->slab + o; };
+    std::vector<char> host(tables_end - operand_bytes);
+    std::vector<CUtensorMap> maps(stacks.size() * kMapsPerStack);
+    bool ok = true;
+    for (size_t i = 0; i < stacks.size(); ++i) {
+        NsStack& s = stacks[i];
+        const Place& p = places[i];
+        for (int k = 0; k < 2; ++k) {
+            s.x[k] = reinterpret_cast<__half*>(at(p.x[k]));
+            s.xl[k] = reinterpret_cast<__half*>(at(p.xl[k]));
+        }
+        s.a = reinterpret_cast<__half*>(at(p.a));
+        s.b = reinterpret_cast<__half*>(at(p.b));
+        s.al = three ? reinterpret_cast<__half*>(at(p.al)) : s.a;
+        s.bl = three ? reinterpret_cast<__half*>(at(p.bl)) : s.b;
+        CUtensorMap* m = maps.data() + i * kMapsPerStack;
+        ok = ok && encode(encoder, m + kMapX0, s.x[0], s.m, s.n, s.ldx, s.count) &&
+             encode(encoder, m + kMapX1, s.x[1], s.m, s.n, s.ldx, s.count) &&
+             encode(encoder, m + kMapA, s.a, s.m, s.m, s.lda, s.count) &&
+             encode(encoder, m + kMapB, s.b, s.m, s.m, s.lda, s.count) &&
+             encode(encoder, m + kMapLo + kMapX0, s.xl[0], s.m, s.n, s.ldx, s.count) &&
+             encode(encoder, m + kMapLo + kMapX1, s.xl[1], s.m, s.n, s.ldx, s.count) &&
+             encode(encoder, m + kMapLo + kMapA, s.al, s.m, s.m, s.lda, s.count) &&
+             encode(encoder, m + kMapLo + kMapB, s.bl, s.m, s.m, s.lda, s.count);
+    }
+    auto put = [&](size_t o, const void* from, size_t bytes) {
+        if (bytes) std::memcpy(host.data() + (o - operand_bytes), from, bytes);
+    };
+    put(o_stacks, stacks.data(), stacks.size() * sizeof(NsStack));
+    put(o_maps, maps.data(), maps.size() * sizeof(CUtensorMap));
+    put(o_tasks, tasks.data(), tasks.size() * sizeof(NsTask));
+    put(o_prep, prep.data(), prep.size() * sizeof(PrepTile));
+    if (ok) {
+        e = cudaMemset(plan->slab, 0, operand_bytes);
+        if (e == cudaSuccess) e = cudaMemcpy(at(operand_bytes), host.data(), host.size(), cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaMemset(at(zero_from), 0, off - zero_from);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    }
+    if (!ok || e != cudaSuccess) {
+        *why = ok ? std::string("plan upload: ") + cudaGetErrorString(e) : "cuTensorMapEncodeTiled failed";
+        cudaFree(plan->slab);
+        return nullptr;
+    }
+    MatrixArgs& a = plan->args;
+    a.stacks = reinterpret_cast<const NsStack*>(at(o_stacks));
+    a.maps = reinterpret_cast<const CUtensorMap*>(at(o_maps));
+    a.tasks = reinterpret_cast<const NsTask*>(at(o_tasks));
+    a.n_tasks = static_cast<uint32_t>(tasks.size());
+    a.prep = reinterpret_cast<const PrepTile*>(at(o_prep));
+    a.n_prep = static_cast<uint32_t>(prep.size());
+    a.n_matrices = static_cast<uint32_t>(matrices);
+    a.partials = reinterpret_cast<double*>(at(o_partials));
+    a.inv = reinterpret_cast<float*>(at(o_inv));
+    a.tickets = reinterpret_cast<uint32_t*>(at(o_tickets));
+    a.done = reinterpret_cast<uint32_t*>(at(o_done));
+    a.next = reinterpret_cast<uint32_t*>(at(o_words));
+    a.step = reinterpret_cast<MatrixStep*>(at(o_words + 64));
+    a.err = opts.err ? opts.err : reinterpret_cast<int*>(at(o_words + 128));
+    std::memcpy(a.coef, opts.coef, sizeof a.coef);
+    a.eps = opts.eps;
+    return plan.release();
+}
+
+cudaError_t matrix_plan_run(MatrixPlan* p, cudaStream_t stream) {
+    return launch_matrix_ops(p->args, p->source, p->dest, nullptr, nullptr, p->sms, stream);
+}
+
+cudaError_t matrix_plan_step(MatrixPlan* p, Ctl* ctl, const ApplyArgs& step, const void* const* grads,
+                             float momentum, bool nesterov, bool ema, cudaStream_t stream) {
+    MatrixArgs a = p->args;
+    a.grads = grads;
+    a.momentum = momentum;
+    a.nesterov = nesterov ? 1 : 0;
+    a.ema = ema ? 1 : 0;
+    return launch_matrix_ops(a, p->source, p->dest, ctl, &step, p->sms, stream);
+}
+
+int* matrix_plan_error_word(MatrixPlan* p) { return p->args.err; }
+
+}  // namespace soarb

@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/soar_optim.h"
+#include "matrix_ops.cuh"
 #include "optim_kernels.cuh"
 
 namespace {
@@ -84,6 +85,7 @@ struct GradSet {
     soarb::Chunk* sumsq_chunks = nullptr;  // norm-pass table (device)
     soarb::DirectRuns druns{};
     void* alloc = nullptr;                 // device block of an added set's tables
+    const void** matrix_grads = nullptr;   // (Muon) the gradients on the device, by tensor
 };
 
 struct Optim {
@@ -92,6 +94,8 @@ struct Optim {
     bool sgd = false;            // SGD (momentum buffer in m) instead of AdamW
     float momentum = 0.0f, dampening = 0.0f;
     bool nesterov = false;
+    bool muon = false;           // Muon: momentum in m, the update by `matrices`
+    soarb::MatrixPlan* matrices = nullptr;
     soar_adamw_opts opts{};
     float lr = 1e-3f;
     float pending_coef = 1.0f;   // from a standalone clip_grad_norm (mixed layout)
@@ -148,6 +152,7 @@ struct Cosine {
 };
 
 size_t elem_bytes(const Optim& o) { return o.mixed ? 2 : 4; }
+bool has_v(const Optim& o) { return !o.sgd && !o.muon; }
 
 // bc[t] = (1 - beta1^t, sqrt(1 - beta2^t)) with the reference's own host
 // expressions (adamw.cpp:68-70), so the device reads the reference's bits.
@@ -401,14 +406,100 @@ struct SgdParams {
     bool nesterov;
 };
 
+struct MuonParams {
+    const soar_matrix_shape* shapes;
+    const soar_muon_opts* opts;
+};
+
+float muon_factor(int scale, uint64_t rows, uint64_t cols) {
+    const double r = static_cast<double>(rows), c = static_cast<double>(cols);
+    if (scale == SOAR_MUON_SCALE_ASPECT) return static_cast<float>(std::sqrt(std::max(1.0, r / c)));
+    if (scale == SOAR_MUON_SCALE_RMS) return static_cast<float>(0.2 * std::sqrt(std::max(r, c)));
+    return 1.0f;
+}
+
+// Checks that need no device.
+bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::string* why) {
+    const soar_muon_opts& o = *p.opts;
+    if (o.steps < 1 || o.steps > SOAR_NS_MAX_STEPS) {
+        *why = "steps must be 1 .. " + std::to_string(SOAR_NS_MAX_STEPS);
+        return false;
+    }
+    if (o.scale < SOAR_MUON_SCALE_NONE || o.scale > SOAR_MUON_SCALE_RMS) {
+        *why = "unknown scale";
+        return false;
+    }
+    if (!(o.eps >= 0.0f)) {
+        *why = "eps must be >= 0";
+        return false;
+    }
+    for (int i = 0; i < n; ++i) {
+        const soar_matrix_shape& s = p.shapes[i];
+        if (!soarb::matrix_shape_ok(s.count, s.rows, s.cols, why)) {
+            *why = "tensor " + std::to_string(i) + ": " + *why;
+            return false;
+        }
+        if (s.count * s.rows * s.cols != t[i].numel) {
+            *why = "tensor " + std::to_string(i) + ": count x rows x cols is not numel";
+            return false;
+        }
+    }
+    return true;
+}
+
+// The device copy of one gradient set's pointers (Muon).
+cudaError_t upload_matrix_grads(const std::vector<void*>& grads, const void*** out) {
+    cudaError_t e = cudaMalloc(out, std::max<size_t>(grads.size(), 1) * sizeof(void*));
+    if (e != cudaSuccess) return e;
+    e = cudaMemcpy(*out, grads.data(), grads.size() * sizeof(void*), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+        cudaFree(*out);
+        *out = nullptr;
+    }
+    return e;
+}
+
+// Plans the matrices of the tensors that have a gradient.
+bool plan_matrices(Optim& o, const MuonParams& p, std::string* why) {
+    std::vector<soarb::MatrixSpec> specs;
+    for (size_t i = 0; i < o.tensors.size(); ++i) {
+        const TensorRec& t = o.tensors[i];
+        if (!t.grad || !t.numel) continue;
+        soarb::MatrixSpec q;
+        q.count = p.shapes[i].count;
+        q.rows = p.shapes[i].rows;
+        q.cols = p.shapes[i].cols;
+        q.param = t.param;
+        q.master = o.mixed ? o.master + t.state_off : static_cast<float*>(t.param);
+        q.mom = o.m + t.state_off;
+        q.wd = t.wd;
+        q.factor = muon_factor(p.opts->scale, q.rows, q.cols);
+        q.tensor = static_cast<uint32_t>(i);
+        specs.push_back(q);
+    }
+    soarb::MatrixPlanOpts mo;
+    mo.steps = p.opts->steps;
+    std::memcpy(mo.coef, p.opts->coef, sizeof mo.coef);
+    mo.eps = p.opts->eps;
+    mo.source = o.mixed ? soarb::kSrcGradBf16 : soarb::kSrcGradF32;
+    mo.dest = o.mixed ? soarb::kDstParamMixed : soarb::kDstParamF32;
+    mo.err = &o.ctl->error;
+    o.matrices = soarb::matrix_plan_create(specs.data(), static_cast<int>(specs.size()), mo, why);
+    return o.matrices != nullptr;
+}
+
 int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* opts,
-                void** out, const SgdParams* sgd = nullptr) {
+                void** out, const SgdParams* sgd = nullptr, const MuonParams* muon = nullptr) {
     if (!opts || !out || n < 0 || (n > 0 && !tensors)) return fail("null argument");
     *out = nullptr;
     if (opts->layout != SOAR_LAYOUT_FP32 && opts->layout != SOAR_LAYOUT_BF16_MIXED)
         return fail("unknown layout");
     if (opts->use_loss_scaler && !(opts->init_scale > 0.0f)) return fail("init_scale must be > 0");
     if (opts->use_loss_scaler && opts->growth_interval <= 0) return fail("growth_interval must be > 0");
+    if (muon) {
+        std::string why;
+        if (!muon_valid(tensors, n, *muon, &why)) return fail(why);
+    }
 
     auto* o = new Optim();
     o->opts = *opts;
@@ -417,6 +508,11 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
         o->momentum = sgd->momentum;
         o->dampening = sgd->dampening;
         o->nesterov = sgd->nesterov;
+    }
+    if (muon) {
+        o->muon = true;
+        o->momentum = muon->opts->momentum;
+        o->nesterov = muon->opts->nesterov != 0;
     }
     o->device = opts->device;
     o->mixed = opts->layout == SOAR_LAYOUT_BF16_MIXED;
@@ -479,7 +575,7 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
     const size_t off_m = off;
     off = align_up(off + state_bytes, kSlabAlign);
     const size_t off_v = off;
-    if (!o->sgd) off = align_up(off + state_bytes, kSlabAlign);  // SGD has no second moment
+    if (has_v(*o)) off = align_up(off + state_bytes, kSlabAlign);  // SGD, Muon: no second moment
     const size_t off_chunks = off;
     off = align_up(off + o->host_chunks.size() * sizeof(soarb::Chunk), kSlabAlign);
     const size_t off_sumsq_chunks = off;
@@ -501,7 +597,7 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
     }
     o->master = o->mixed ? reinterpret_cast<float*>(o->slab + off_master) : nullptr;
     o->m = reinterpret_cast<float*>(o->slab + off_m);
-    o->v = o->sgd ? nullptr : reinterpret_cast<float*>(o->slab + off_v);
+    o->v = has_v(*o) ? reinterpret_cast<float*>(o->slab + off_v) : nullptr;
     o->chunks = reinterpret_cast<soarb::Chunk*>(o->slab + off_chunks);
     o->sumsq_chunks = reinterpret_cast<soarb::Chunk*>(o->slab + off_sumsq_chunks);
     o->partials = reinterpret_cast<double*>(o->slab + off_partials);
@@ -514,11 +610,13 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
             const uint64_t s = static_cast<uint64_t>(reinterpret_cast<uintptr_t>(c.master));
             c.master = o->mixed ? o->master + s : static_cast<float*>(c.param);
             c.m = o->m + s;
-            c.v = o->sgd ? nullptr : o->v + s;
+            c.v = o->v ? o->v + s : nullptr;
         }
     }
 
     auto cleanup = [&](const std::string& msg) {
+        for (GradSet& gs : o->grad_sets) cudaFree(gs.matrix_grads);
+        soarb::matrix_plan_destroy(o->matrices);
         cudaFree(o->slab);
         if (o->bc) cudaFree(o->bc);
         delete o;
@@ -569,7 +667,7 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
         uint64_t total = 0;
         for (const TensorRec& t : o->tensors)
             if (t.grad) total += t.numel;
-        o->direct = !o->sgd && total > 0 && total <= kDirectMaxElems &&
+        o->direct = has_v(*o) && total > 0 && total <= kDirectMaxElems &&
                     build_direct_runs(*o, g0.grads, &g0.druns);
         if (o->direct) {
             // as many CTAs as are resident at once, fewer when the vectors do
@@ -582,6 +680,13 @@ int create_impl(const soar_tensor_desc* tensors, int n, const soar_adamw_opts* o
         }
         o->druns = g0.druns;
         o->grad_sets.push_back(std::move(g0));
+    }
+    if (muon) {
+        std::string why;
+        if (!plan_matrices(*o, *muon, &why)) return cleanup(why);
+        GradSet& g0 = o->grad_sets.front();
+        if ((e = upload_matrix_grads(g0.grads, &g0.matrix_grads)) != cudaSuccess)
+            return cleanup(std::string("gradient list: ") + cudaGetErrorString(e));
     }
     if ((e = cudaDeviceSynchronize()) != cudaSuccess)
         return cleanup(std::string("create: ") + cudaGetErrorString(e));
@@ -638,7 +743,11 @@ int apply_impl(Optim& o, const double* parts, int n_parts, cudaStream_t s,
     soarb::ApplyArgs a =
         apply_args(o, parts, n_parts, max_norm >= 0.0f ? max_norm : o.opts.max_grad_norm);
     a.skip_if = skip_if;
-    if (o.direct && !ag && !o.ema) {
+    if (o.muon) {
+        SOAR_CUDA_TRY(soarb::matrix_plan_step(o.matrices, o.ctl, a,
+                                              o.grad_sets[o.grad_set].matrix_grads, o.momentum,
+                                              o.nesterov, o.ema != nullptr, s));
+    } else if (o.direct && !ag && !o.ema) {
         SOAR_CUDA_TRY(soarb::launch_apply_direct(o.mixed, o.druns, o.chunks, o.n_chunks, o.n_vec,
                                                  o.ctl, a, o.grid_direct, s));
     } else {
@@ -686,6 +795,9 @@ int optim_apply_allgather(void* optim, const double* parts, int n_parts, cudaStr
     DeviceGuard g(o.device);
     return apply_impl(o, parts, n_parts, stream, &ag, skip_if);
 }
+
+// Whether the optimizer updates whole matrices (Muon).
+bool optim_needs_matrices(void* optim) { return as_optim(optim)->muon; }
 
 // Tensor `index`'s param/grad/numel and the optimizer's layout, control block
 // and device (index -1: only the latter three).
@@ -786,17 +898,63 @@ SOAR_API int soar_sgd_create(const soar_tensor_desc* tensors, int n_tensors,
     }
 }
 
+SOAR_API void soar_muon_default_opts(soar_muon_opts* out) {
+    if (!out) return;
+    std::memset(out, 0, sizeof *out);
+    out->lr = 2e-2f;
+    out->momentum = 0.95f;
+    out->nesterov = 1;
+    out->scale = SOAR_MUON_SCALE_ASPECT;
+    out->steps = 5;
+    soarb::matrix_default_coef(out->coef);
+    out->eps = 1e-7f;
+    out->layout = SOAR_LAYOUT_FP32;
+    out->init_scale = 65536.0f;
+    out->growth_factor = 2.0f;
+    out->backoff_factor = 0.5f;
+    out->growth_interval = 200;
+}
+
+SOAR_API int soar_muon_create(const soar_tensor_desc* tensors, const soar_matrix_shape* shapes,
+                              int n_tensors, const soar_muon_opts* opts, void** out_handle) {
+    if (!opts || !out_handle || n_tensors < 0 || (n_tensors > 0 && (!tensors || !shapes)))
+        return fail("null argument");
+    try {
+        soar_adamw_opts a;
+        soar_adamw_default_opts(&a);
+        a.lr = opts->lr;
+        a.weight_decay = opts->weight_decay;
+        a.layout = opts->layout;
+        a.max_grad_norm = opts->max_grad_norm;
+        a.use_loss_scaler = opts->use_loss_scaler;
+        a.init_scale = opts->init_scale;
+        a.growth_factor = opts->growth_factor;
+        a.backoff_factor = opts->backoff_factor;
+        a.growth_interval = opts->growth_interval;
+        a.device = opts->device;
+        const MuonParams mp{shapes, opts};
+        return create_impl(tensors, n_tensors, &a, out_handle, nullptr, &mp);
+    } catch (const std::exception& ex) {
+        return fail(ex.what());
+    } catch (...) {
+        return fail("unknown exception");
+    }
+}
+
 SOAR_API int soar_optim_destroy(void* handle) {
     if (!handle) return fail("null handle");
     Optim* o = as_optim(handle);
     {
         DeviceGuard g(o->device);
         cudaDeviceSynchronize();
+        soarb::matrix_plan_destroy(o->matrices);
         cudaFree(o->slab);
         if (o->bc) cudaFree(o->bc);
         if (o->ema) cudaFree(o->ema);
-        for (GradSet& gs : o->grad_sets)
+        for (GradSet& gs : o->grad_sets) {
             if (gs.alloc) cudaFree(gs.alloc);
+            if (gs.matrix_grads) cudaFree(gs.matrix_grads);
+        }
     }
     delete o;
     return SOAR_OK;
@@ -968,7 +1126,7 @@ SOAR_API int soar_optim_state_ptr(void* handle, int index, int kind, void** out_
             *out_ptr = o.m + t.state_off;
             return SOAR_OK;
         case SOAR_STATE_V:
-            if (!o.v) return fail("SGD has no second-moment state");
+            if (!o.v) return fail("SGD and Muon have no second-moment state");
             *out_ptr = o.v + t.state_off;
             return SOAR_OK;
         case SOAR_STATE_EMA:
@@ -1076,6 +1234,11 @@ struct Counters {  // payload of the "optim.counters" record
     uint64_t n_tensors;
 };
 
+// The layout, and the optimizer where it is not AdamW.
+uint32_t layout_tag(const Optim& o) {
+    return static_cast<uint32_t>(o.opts.layout) | (o.sgd ? 0x100u : 0u) | (o.muon ? 0x200u : 0u);
+}
+
 bool write_record(FILE* f, const std::string& name, uint64_t numel, const void* data,
                   uint64_t bytes) {
     char nb[128]{0};
@@ -1098,13 +1261,13 @@ SOAR_API int soar_optim_save_state(void* handle, const char* path) {
     FILE* f = std::fopen(path, "wb");
     if (!f) return fail(std::string("cannot open ") + path);
     std::vector<int> kinds = {SOAR_STATE_MASTER, SOAR_STATE_M};
-    if (!o.sgd) kinds.push_back(SOAR_STATE_V);
+    if (has_v(o)) kinds.push_back(SOAR_STATE_V);
     if (o.ema) kinds.push_back(SOAR_STATE_EMA);
     const uint32_t n_records = 1 + static_cast<uint32_t>(kinds.size() * o.tensors.size());
     const uint32_t hdr[4] = {kSoarMagic, kStateVersion, 0u, n_records};
     bool ok = std::fwrite(hdr, 4, 4, f) == 4;
     Counters ct{c.t, c.skipped, o.host_calls, c.scale, c.tracker, o.lr,
-                static_cast<uint32_t>(o.opts.layout) | (o.sgd ? 0x100u : 0u), o.tensors.size()};
+                layout_tag(o), o.tensors.size()};
     ok = ok && write_record(f, "optim.counters", sizeof ct / 4, &ct, sizeof ct);
     std::vector<float> buf;
     for (size_t i = 0; ok && i < o.tensors.size(); ++i) {
@@ -1141,7 +1304,7 @@ SOAR_API int soar_optim_load_state(void* handle, const char* path, void* stream)
     }
     std::map<std::string, std::pair<int, int>> want;  // name -> (tensor, kind)
     std::vector<int> kinds = {SOAR_STATE_MASTER, SOAR_STATE_M};
-    if (!o.sgd) kinds.push_back(SOAR_STATE_V);
+    if (has_v(o)) kinds.push_back(SOAR_STATE_V);
     if (o.ema) kinds.push_back(SOAR_STATE_EMA);
     for (size_t i = 0; i < o.tensors.size(); ++i)
         for (int k : kinds)
@@ -1182,7 +1345,7 @@ SOAR_API int soar_optim_load_state(void* handle, const char* path, void* stream)
     std::fclose(f);
     if (!have_counters) return fail("no optim.counters record");
     if (ct.n_tensors != o.tensors.size() ||
-        ct.layout != (static_cast<uint32_t>(o.opts.layout) | (o.sgd ? 0x100u : 0u)))
+        ct.layout != layout_tag(o))
         return fail("checkpoint was written by an optimizer with a different tensor list or layout");
     if (loaded != kinds.size() * o.tensors.size())
         return fail("checkpoint is missing optimizer records (" + std::to_string(loaded) + " of " +
@@ -1303,6 +1466,7 @@ SOAR_API int soar_optim_add_grads(void* handle, void* const* grads, int* out_set
     if (e == cudaSuccess)
         e = cudaMemcpy(gs.sumsq_chunks, ns.data(), ns.size() * sizeof(soarb::Chunk),
                        cudaMemcpyHostToDevice);
+    if (e == cudaSuccess && o.muon) e = upload_matrix_grads(ng, &gs.matrix_grads);
     if (e != cudaSuccess) {
         cudaFree(gs.alloc);
         return fail(std::string("gradient-set tables: ") + cudaGetErrorString(e));
@@ -1328,7 +1492,7 @@ SOAR_API int soar_optim_use_grads(void* handle, int set) {
 SOAR_API int soar_optim_kernel_path(void* handle, int* out_path) {
     if (!handle || !out_path) return fail("null argument");
     const Optim& o = *as_optim(handle);
-    *out_path = (o.direct && !o.ema) ? 1 : 0;
+    *out_path = o.muon ? 2 : (o.direct && !o.ema) ? 1 : 0;
     return SOAR_OK;
 }
 

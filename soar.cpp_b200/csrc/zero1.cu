@@ -58,6 +58,7 @@ int optim_apply_allgather(void* optim, const double* parts, int n_parts, cudaStr
                           const AgArgs& ag, const int* skip_if);
 bool optim_tensor_info(void* optim, int index, void** param, void** grad, uint64_t* numel,
                        bool* mixed, Ctl** ctl, int* device);
+bool optim_needs_matrices(void* optim);
 }  // namespace soarb
 
 namespace soarb {
@@ -366,6 +367,7 @@ using soarb::kRsThreads;
 using soarb::kRsSmemBudget;
 using soarb::k_rs_sumsq;
 using soarb::optim_tensor_info;
+using soarb::optim_needs_matrices;
 using soarb::optim_apply_allgather;
 using soarb::Signals;
 using soarb::launch_step_done;
@@ -433,6 +435,8 @@ SOAR_API int soar_zero1_create(void* optim_handle, int rank, int world,
     if (world < 1 || world > kMaxRanks || rank < 0 || rank >= world)
         return fail("world size must be 1.." + std::to_string(kMaxRanks));
     *out = nullptr;
+    if (optim_needs_matrices(optim_handle))
+        return fail("Muon updates whole matrices; a shard of the flat buffers does not hold them");
     auto* z = new Zero1();
     z->optim = optim_handle;
     z->world = world;

@@ -15,8 +15,8 @@ LIB = LIBDIR / "libsoar_optim.so"
 INCLUDE = ROOT.parent / "include"
 
 SOURCES = ["optim_kernels.cu", "optim_capi.cu", "noalloc_sumsq.cu", "zero1.cu",
-           "dp_bootstrap.cu"]
-HEADERS = ["optim_kernels.cuh", "pipeline.cuh"]
+           "dp_bootstrap.cu", "matrix_kernels.cu", "matrix_plan.cu", "ortho_capi.cu"]
+HEADERS = ["optim_kernels.cuh", "pipeline.cuh", "step.cuh", "matrix_ops.cuh"]
 # the bench-only NVLink probe: a library of its own, not part of the C-ABI
 PROBE_LIB = LIBDIR / "libsoar_probe.so"
 PROBE_SOURCES = ["nvlink_probe.cu"]
@@ -29,7 +29,7 @@ NVCC_FLAGS = [
     # the compiler from contracting anything else
     "-fmad=false",
     "-Xcompiler", "-fPIC,-fvisibility=hidden,-O3",
-    "-shared",
+    "-shared", "--threads", "0",  # (sources compile side by side)
     "-ldl",   # NCCL is opened with dlopen by the data-parallel bootstrap
 ]
 

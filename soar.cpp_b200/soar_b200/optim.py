@@ -23,6 +23,9 @@ from pathlib import Path
 from . import _build
 
 LAYOUT_FP32 = 0
+DTYPE_FP32, DTYPE_BF16 = 0, 1
+NS_MAX_STEPS = 16
+MUON_SCALES = {"none": 0, "aspect": 1, "rms": 2}
 LAYOUT_BF16_MIXED = 1
 STATE_MASTER, STATE_M, STATE_V, STATE_EMA = 0, 1, 2, 3
 
@@ -52,6 +55,32 @@ class SGDOpts(C.Structure):
                 ("init_scale", C.c_float), ("growth_factor", C.c_float),
                 ("backoff_factor", C.c_float), ("growth_interval", C.c_int32),
                 ("device", C.c_int32)]
+
+
+class MatrixDesc(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("count", C.c_uint64),
+                ("rows", C.c_uint64), ("cols", C.c_uint64), ("src_row", C.c_uint64),
+                ("src_mat", C.c_uint64), ("dst_row", C.c_uint64), ("dst_mat", C.c_uint64)]
+
+
+class OrthoOpts(C.Structure):
+    _fields_ = [("steps", C.c_int32), ("coef", (C.c_float * 3) * NS_MAX_STEPS),
+                ("eps", C.c_float), ("src_type", C.c_int32), ("dst_type", C.c_int32),
+                ("device", C.c_int32)]
+
+
+class MatrixShape(C.Structure):
+    _fields_ = [("count", C.c_uint64), ("rows", C.c_uint64), ("cols", C.c_uint64)]
+
+
+class MuonOpts(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float),
+                ("nesterov", C.c_int32), ("scale", C.c_int32), ("steps", C.c_int32),
+                ("coef", (C.c_float * 3) * NS_MAX_STEPS), ("eps", C.c_float),
+                ("layout", C.c_int32), ("max_grad_norm", C.c_float),
+                ("use_loss_scaler", C.c_int32), ("init_scale", C.c_float),
+                ("growth_factor", C.c_float), ("backoff_factor", C.c_float),
+                ("growth_interval", C.c_int32), ("device", C.c_int32)]
 
 
 class StepInfo(C.Structure):
@@ -138,6 +167,15 @@ SIGNATURES: dict[str, tuple] = {
     "soar_optim_add_grads": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_int)]),
     "soar_optim_use_grads": (C.c_int, [C.c_void_p, C.c_int]),
     "soar_optim_kernel_path": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
+    "soar_ortho_default_opts": (None, [C.POINTER(OrthoOpts)]),
+    "soar_ortho_create": (C.c_int, [C.POINTER(MatrixDesc), C.c_int, C.POINTER(OrthoOpts),
+                                    C.POINTER(C.c_void_p)]),
+    "soar_ortho_run": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "soar_ortho_error": (C.c_int, [C.c_void_p, C.POINTER(C.c_int)]),
+    "soar_ortho_destroy": (C.c_int, [C.c_void_p]),
+    "soar_muon_default_opts": (None, [C.POINTER(MuonOpts)]),
+    "soar_muon_create": (C.c_int, [C.POINTER(TensorDesc), C.POINTER(MatrixShape), C.c_int,
+                                   C.POINTER(MuonOpts), C.POINTER(C.c_void_p)]),
     "soar_last_error": (C.c_char_p, []),
 }
 
@@ -481,10 +519,10 @@ class AdamW:
 
     @property
     def kernel_path(self) -> str:
-        """'pipeline' (k_apply) or 'direct' (k_apply_direct)."""
+        """'pipeline' (k_apply), 'direct' (k_apply_direct) or 'matrix' (Muon)."""
         out = C.c_int()
         _check(lib().soar_optim_kernel_path(self.handle, C.byref(out)), "soar_optim_kernel_path")
-        return "direct" if out.value == 1 else "pipeline"
+        return ("pipeline", "direct", "matrix")[out.value]
 
     def loss_scale_ptr(self) -> int:
         out = C.c_void_p()
@@ -517,6 +555,164 @@ class SGD(AdamW):
         o.weight_decay, o.nesterov = options.weight_decay, int(options.nesterov)
         self._create(params, grads, options.weight_decay, o, layout, max_grad_norm, loss_scaler,
                      device, lib().soar_sgd_create, "soar_sgd_create")
+
+
+def _fill_coef(dst, coefficients, steps: int) -> None:
+    """One (a, b, c) for every step, or one per step."""
+    rows = list(coefficients)
+    if rows and not hasattr(rows[0], "__len__"):
+        rows = [rows] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError("coefficients: (a, b, c), or one such triple per step")
+    if not 1 <= steps <= NS_MAX_STEPS:
+        raise ValueError(f"steps must be 1 .. {NS_MAX_STEPS}")
+    for i, row in enumerate(rows):
+        for j, v in enumerate(row):
+            dst[i][j] = v
+
+
+@dataclass
+class MuonOptions:
+    """Muon (no reference counterpart): momentum orthogonalised by `steps`
+    Newton-Schulz products. `scale` is the update's shape factor: "none",
+    "aspect" (sqrt(max(1, rows / cols))) or "rms" (0.2 sqrt(max(rows, cols)),
+    updates of AdamW's usual rms)."""
+
+    lr: float = 2e-2
+    momentum: float = 0.95
+    nesterov: bool = True
+    weight_decay: float = 0.0
+    scale: str = "aspect"
+    steps: int = 5
+    coefficients: tuple = (3.4445, -4.7750, 2.0315)
+    eps: float = 1e-7
+
+
+class Muon(AdamW):
+    """Muon on the same device step (soar_muon_create): momentum, its
+    orthogonalisation, decoupled weight decay, with the layouts, fused clip and
+    loss scaler of AdamW. Every parameter is a contiguous [rows, cols] weight or
+    [count, rows, cols] stack of weights that are updated one by one; other
+    parameters (biases, norms, embeddings) belong in an AdamW beside it. The
+    momentum buffer is state kind STATE_M; there is no STATE_V."""
+
+    def __init__(self, params, options: MuonOptions | None = None, *, layout: str = "fp32",
+                 max_grad_norm: float = 0.0, loss_scaler: LossScalerOptions | None = None,
+                 device: int | None = None, grads=None):
+        options = options or MuonOptions()
+        if options.scale not in MUON_SCALES:
+            raise ValueError(f"scale must be one of {', '.join(MUON_SCALES)}")
+        o = MuonOpts()
+        lib().soar_muon_default_opts(C.byref(o))
+        o.lr, o.momentum, o.weight_decay = options.lr, options.momentum, options.weight_decay
+        o.nesterov, o.scale = int(options.nesterov), MUON_SCALES[options.scale]
+        o.steps, o.eps = options.steps, options.eps
+        _fill_coef(o.coef, options.coefficients, options.steps)
+        flat = [q for p in params for q in (p.params if isinstance(p, ParamGroup) else [p])]
+        shapes = (MatrixShape * max(len(flat), 1))()
+        for i, p in enumerate(flat):
+            if p.dim() not in (2, 3):
+                raise ValueError(f"parameter {i}: Muon takes [rows, cols] or [count, rows, cols], "
+                                 f"not {tuple(p.shape)}")
+            if not p.is_contiguous():
+                raise ValueError(f"parameter {i}: not contiguous")
+            shapes[i].count = p.shape[0] if p.dim() == 3 else 1
+            shapes[i].rows, shapes[i].cols = p.shape[-2], p.shape[-1]
+
+        def create(descs, n, opts, out):
+            return lib().soar_muon_create(descs, shapes, n, opts, out)
+
+        self._create(params, grads, options.weight_decay, o, layout, max_grad_norm, loss_scaler,
+                     device, create, "soar_muon_create")
+
+
+@dataclass
+class OrthogonalizeOptions:
+    """Newton-Schulz iteration: X <- a X + (b A + c A A) X with A = X X^T,
+    from G / (|G|_F + eps)."""
+
+    steps: int = 5
+    coefficients: tuple = (3.4445, -4.7750, 2.0315)
+    eps: float = 1e-7
+
+
+class Orthogonalizer:
+    """Orthogonalises a list of matrices in place of a Muon optimizer's own
+    step: ``run()`` writes the result for ``srcs[i]`` to ``dsts[i]``. Each pair
+    is two CUDA tensors of one shape, [rows, cols] or [count, rows, cols], whose
+    rows are contiguous (other strides are free; a destination may be its source).
+    The sources have one type, the destinations another or the same: float32 or
+    bfloat16. The buffers are bound, as an optimizer's gradients are, and runs of
+    one object share its workspace: order them on one stream."""
+
+    def __init__(self, srcs, dsts, options: OrthogonalizeOptions | None = None, *,
+                 device: int | None = None):
+        import torch
+        options = options or OrthogonalizeOptions()
+        self.handle = None
+        self.srcs, self.dsts = list(srcs), list(dsts)
+        if len(self.srcs) != len(self.dsts):
+            raise ValueError("one destination per source")
+        types = {torch.float32: DTYPE_FP32, torch.bfloat16: DTYPE_BF16}
+        o = OrthoOpts()
+        lib().soar_ortho_default_opts(C.byref(o))
+        o.steps, o.eps = options.steps, options.eps
+        _fill_coef(o.coef, options.coefficients, options.steps)
+        for name, side in (("source", self.srcs), ("destination", self.dsts)):
+            if len({t.dtype for t in side}) > 1:
+                raise ValueError(f"{name}s of more than one type")
+            if side and side[0].dtype not in types:
+                raise ValueError(f"{name}s must be float32 or bfloat16, not {side[0].dtype}")
+        if self.srcs:
+            o.src_type, o.dst_type = types[self.srcs[0].dtype], types[self.dsts[0].dtype]
+        everything = self.srcs + self.dsts
+        for t in everything:
+            if t.device.type != "cuda":
+                raise ValueError("matrices must be CUDA tensors")
+        if len({t.device for t in everything}) > 1:
+            raise ValueError("matrices on more than one device")
+        if device is None:
+            device = everything[0].device.index if everything else 0
+        o.device = self.device = device
+        n = len(self.srcs)
+        descs = (MatrixDesc * max(n, 1))()
+        for i, (s, d) in enumerate(zip(self.srcs, self.dsts)):
+            if s.shape != d.shape or s.dim() not in (2, 3):
+                raise ValueError(f"matrix {i}: source {tuple(s.shape)} and destination "
+                                 f"{tuple(d.shape)} must be one [rows, cols] or [count, rows, cols]")
+            for t in (s, d):
+                if t.shape[-1] > 1 and t.stride(-1) != 1:
+                    raise ValueError(f"matrix {i}: rows must be contiguous")
+            q = descs[i]
+            q.src, q.dst = s.data_ptr(), d.data_ptr()
+            q.count = s.shape[0] if s.dim() == 3 else 1
+            q.rows, q.cols = s.shape[-2], s.shape[-1]
+            q.src_row, q.dst_row = s.stride(-2), d.stride(-2)
+            q.src_mat = s.stride(0) if s.dim() == 3 else 0
+            q.dst_mat = d.stride(0) if d.dim() == 3 else 0
+        h = C.c_void_p()
+        _check(lib().soar_ortho_create(descs, n, C.byref(o), C.byref(h)), "soar_ortho_create")
+        self.handle = h
+
+    def run(self, stream=None) -> None:
+        _check(lib().soar_ortho_run(self.handle, _stream_handle(stream)), "soar_ortho_run")
+
+    def error(self) -> int:
+        """Nonzero if a device-side wait of some run timed out (synchronises)."""
+        out = C.c_int()
+        _check(lib().soar_ortho_error(self.handle, C.byref(out)), "soar_ortho_error")
+        return out.value
+
+    def close(self):
+        if getattr(self, "handle", None):
+            lib().soar_ortho_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class CosineAnnealingLR:
