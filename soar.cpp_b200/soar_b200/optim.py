@@ -252,9 +252,12 @@ def _stream_handle(stream) -> int | None:
 
 
 class _DeviceArray:
-    """__cuda_array_interface__ view of library-owned device memory."""
+    """__cuda_array_interface__ view of library-owned device memory. `owner` is
+    what frees that memory when it is collected: tensors made from this object
+    hold the object, and so the owner, until they are gone themselves."""
 
-    def __init__(self, ptr: int, n: int, typestr: str = "<f4"):
+    def __init__(self, ptr: int, n: int, typestr: str = "<f4", owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {"shape": (n,), "typestr": typestr,
                                          "data": (ptr, False), "version": 3, "strides": None}
 
@@ -462,9 +465,10 @@ class AdamW:
         return out.value
 
     def state(self, index: int, kind: int):
-        """Zero-copy torch view of tensor `index`'s master / m / v."""
+        """Zero-copy torch view of tensor `index`'s master / m / v (it keeps the
+        optimizer alive; close() ends both)."""
         import torch
-        arr = _DeviceArray(self.state_ptr(index, kind), self.numel[index])
+        arr = _DeviceArray(self.state_ptr(index, kind), self.numel[index], owner=self)
         return torch.as_tensor(arr, device=f"cuda:{self.device}")
 
     def read_state(self, index: int, kind: int):

@@ -364,3 +364,21 @@ def test_zero1_refuses_muon(cuda):
     out = ctypes.c_void_p()
     rc = sb.lib().soar_zero1_create(opt.handle, 0, 1, base, base, None, 0, ctypes.byref(out))
     assert rc == -1 and b"matrices" in sb.lib().soar_last_error()
+
+
+@gpu
+def test_state_view_keeps_the_optimizer(cuda):
+    """The memory of a state view is the optimizer's: it stays while the view does."""
+    import gc
+    import weakref
+    w = matrices((64, 64), 1, "noise", 0.02).cuda()
+    opt = sb.Muon([w], grads=[w.clone()])
+    opt.step()
+    view, alive = opt.state(0, sb.STATE_M).view(64, 64), weakref.ref(opt)
+    del opt
+    gc.collect()
+    assert alive() is not None
+    assert bool((view == view).all())
+    del view
+    gc.collect()
+    assert alive() is None
