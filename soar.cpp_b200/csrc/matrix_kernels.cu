@@ -204,13 +204,72 @@ k_matrix_split(MatrixArgs a) {
 
 // ------------------------------------------------------ tcgen05 and TMA -----
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            uint32_t x, uint32_t y, uint32_t z) {
+// The other CTA's (or this one's) copy of a shared-memory address.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-        "[%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "barrier.cluster.arrive.release.aligned;\n"
+        "barrier.cluster.wait.acquire.aligned;" ::
+            : "memory");
+}
+// Arrives on a barrier of either CTA of the pair.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
+        "selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// mbar_wait for a barrier the other CTA arrives on.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
+    if (!mbar_wait(bar, parity, s_err)) return false;
+    mbar_try_cluster(bar, parity);  // (complete: acquires at cluster scope)
+    return true;
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint4& v) {
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
+                 "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+
+// Into this CTA's shared memory; the bytes count on `bar` of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                              uint32_t x, uint32_t y, uint32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, uint32_t x,
+                                         uint32_t y, uint32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, uint32_t x, uint32_t y,
+                                          uint32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     map),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
 }
 
 // Shared-memory operand descriptor, 128-byte swizzle (64 fp16 wide rows of 128
@@ -223,7 +282,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead) {
            (static_cast<uint64_t>(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// fp16 x fp16 -> fp32, M = 128, N = n; b_mn: the second operand is MN-major.
+// fp16 x fp16 -> fp32, M = 256 over the pair, N = n; b_mn: the second operand is MN-major.
 __device__ __forceinline__ uint32_t instr_desc(uint32_t n, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((kNsTileM >> 4) << 24);
 }
@@ -232,28 +291,32 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t da, uint64_t db, ui
                                         bool accumulate) {
     asm volatile(
         "{ .reg .pred p; setp.ne.u32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
         "l"(da), "l"(db), "r"(idesc), "r"(accumulate ? 1u : 0u)
         : "memory");
 }
+// Arrives on `bar` of both CTAs when the products issued so far are done.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                     bar)
-                 : "memory");
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
           "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
           "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
           "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        : "r"(addr)
+        : "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -290,55 +353,122 @@ __device__ __forceinline__ bool wait_done(const uint32_t* p, uint32_t need, int*
     }
 }
 
-// 32 consecutive fp16 of one row (16-byte aligned) as floats; columns from
-// `left` on are not read.
-__device__ __forceinline__ void load_row32(const __half* p, uint32_t left, float (&v)[32]) {
+// ---------------------------------------------------------------- staging ---
+// The epilogue's operands pass through shared memory in chunks of 64 columns
+// of the CTA's 128 rows: a slot holds one fp16 chunk as TMA has it (two boxes
+// of 64 rows of 128 bytes, 128-byte swizzle).
+
+// Byte offset of eight columns (group j of 8) of a row in a slot.
+__device__ __forceinline__ uint32_t slot_at(uint32_t row, uint32_t j) {
+    return (row >> 6) * kNsBoxBytes + (row & 63u) * 128u + ((j ^ (row & 7u)) << 4);
+}
+// Byte offset of (row, col) in a slot that holds the chunk's transpose: 64
+// rows (its columns) of 128 (its rows), in two boxes of 64 x 64.
+__device__ __forceinline__ uint32_t mirror_at(uint32_t row, uint32_t col) {
+    return (row >> 6) * kNsBoxBytes + col * 128u + ((((row & 63u) >> 3) ^ (col & 7u)) << 4) + (row & 7u) * 2u;
+}
+// Word offset of (row, col) of a chunk of floats in two slots: rows and
+// columns are both read and written without bank conflicts.
+__device__ __forceinline__ uint32_t float_at(uint32_t row, uint32_t col) {
+    return row * 64u + (((col >> 2) ^ (row & 15u)) << 2) + ((col + (row >> 3)) & 3u);
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
+}
+
+// x[32] += (or =) the thread's 32 columns of its row.
+template <bool kAdd>
+__device__ __forceinline__ void slot_read(uint32_t slot, uint32_t row, uint32_t half, float (&x)[32]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        uint4 q = make_uint4(0, 0, 0, 0);
-        if (static_cast<uint32_t>(j * 8) < left) q = __ldcg(reinterpret_cast<const uint4*>(p) + j);
+        const uint4 q = lds128(slot + slot_at(row, half * 4 + j));
         const __half2* h = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float2 f = __half22float2(h[e]);
-            v[j * 8 + 2 * e] = f.x;
-            v[j * 8 + 2 * e + 1] = f.y;
+            x[j * 8 + 2 * e] = kAdd ? x[j * 8 + 2 * e] + f.x : f.x;
+            x[j * 8 + 2 * e + 1] = kAdd ? x[j * 8 + 2 * e + 1] + f.y : f.y;
         }
     }
 }
 
-// The row's 32 values as fp16 (hi, and lo where given), eight to a store. A
-// store may run past `left` columns into the row's padding, never further.
-template <bool kLo>
-__device__ __forceinline__ void store_row32(__half* hp, __half* lp, uint32_t left, const float (&v)[32]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (static_cast<uint32_t>(j * 8) >= left) break;
-        __half h[8], l[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split_half(v[j * 8 + e], h[e], l[e]);
-        reinterpret_cast<uint4*>(hp)[j] = *reinterpret_cast<uint4*>(h);
-        if constexpr (kLo) reinterpret_cast<uint4*>(lp)[j] = *reinterpret_cast<uint4*>(l);
-    }
+// Two values as packed fp16 (hi), and what is left of them (lo).
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // --------------------------------------------------------------- products ---
 
+// One wave of eight elements of the result, each lane's own: the stack's
+// destination, or Muon's update of the weights there.
 template <int kDst>
-__global__ void __launch_bounds__(kNsThreads, 1)
+__device__ __forceinline__ void put_result(const MatrixArgs& a, const ApplyArgs& step, const NsStack& s,
+                                           const uint64_t (&at)[8], const float (&o)[8], uint32_t valid) {
+    if constexpr (kDst == kDstF32 || kDst == kDstBf16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (!(valid >> i & 1u)) continue;
+            if constexpr (kDst == kDstF32)
+                static_cast<float*>(s.dst)[at[i]] = o[i];
+            else
+                static_cast<uint16_t*>(s.dst)[at[i]] = f32_to_bf16_rn(o[i]);
+        }
+    } else {
+        float w[8], e[8];
+        float* sh = s.mom + step.ema_delta;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = valid >> i & 1u ? s.master[at[i]] : 0.0f;
+        if (a.ema) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = valid >> i & 1u ? sh[at[i]] : 0.0f;
+        }
+        const float lr_wd = __fmul_rn(step.lr, s.wd), lr_s = __fmul_rn(step.lr, s.factor);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (s.wd != 0.0f) w[i] = __fsub_rn(w[i], __fmul_rn(lr_wd, w[i]));
+            w[i] = __fsub_rn(w[i], __fmul_rn(lr_s, o[i]));
+            if (!(valid >> i & 1u)) continue;
+            s.master[at[i]] = w[i];
+            if constexpr (kDst == kDstParamMixed)
+                static_cast<uint16_t*>(s.param)[at[i]] = f32_to_bf16_rn(w[i]);
+        }
+        if (a.ema) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (valid >> i & 1u)
+                    sh[at[i]] = __fadd_rn(__fmul_rn(step.ema_decay, e[i]), __fmul_rn(step.ema_omd, w[i]));
+        }
+    }
+}
+
+template <int kDst>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
-    // fp32 results take three products, bf16 results one
-    constexpr bool kThree = kDst == kDstF32 || kDst == kDstParamF32;
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
-    constexpr uint32_t kPasses = kThree ? 3 : 1;
     constexpr int kRing = 4;  // tasks taken ahead
-    constexpr uint32_t kEnd = 0xFFFFFFFFu;
+    constexpr int kEpi = kNsEpilogueWarps * 32;
+    constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t drain_bar;
-    __shared__ NsTask s_task[kRing];
-    __shared__ uint32_t s_index[kRing];
+    __shared__ __align__(8) uint64_t stage_bar[2], drain_bar;
+    __shared__ __align__(16) NsTask s_task[kRing];
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_drain_err, s_cfail[2];
 
@@ -348,7 +478,9 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     if constexpr (kMuon) {
         if (a.step->skip) return;
     }
+    const uint32_t rank = cluster_rank();  // 0 leads the pair: hands out tasks, issues products
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t staging = smem + kNsStages * kNsStageBytes;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNsStages; ++i) {
             mbar_init(smem_u32(&full_bar[i]), 1);
@@ -356,24 +488,26 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 128);
+            mbar_init(smem_u32(&acc_empty[i]), 2 * kNsEpilogueWarps);  // both CTAs' warps
+            mbar_init(smem_u32(&stage_bar[i]), 1);
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            mbar_init(smem_u32(&task_empty[i]), 2);
+            mbar_init(smem_u32(&task_empty[i]), 4);  // products, two epilogues, the other CTA's loads
         }
         mbar_init(smem_u32(&drain_bar), 1);
         s_err = s_drain_err = s_cfail[0] = s_cfail[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                          smem_u32(&s_tmem))
                      : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
@@ -382,40 +516,58 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         if (lane == 0) {
             fence_async_proxy();  // (X of the kernel before)
             uint32_t it = 0;      // stages issued
-            uint32_t claim = atomicAdd(a.next, 1u);
+            uint32_t claim = rank == 0 ? atomicAdd(a.next, 1u) : 0u;
             for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q % kRing, idx = claim;
-                if (q >= kRing && !mbar_wait(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
-                    break;
-                const bool end = idx >= a.n_tasks;
+                const uint32_t slot = q % kRing;
                 NsTask t{};
-                if (!end) {
-                    t = a.tasks[idx];
+                if (rank == 0) {
+                    if (q >= kRing &&
+                        !mbar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
+                        break;
+                    if (claim < a.n_tasks) {
+                        t = a.tasks[claim];
+                        claim = atomicAdd(a.next, 1u);
+                    } else {
+                        t.stack = kEnd;
+                    }
                     s_task[slot] = t;
+                    mbar_arrive(smem_u32(&task_full[slot]));
+                    const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
+                    st_cluster_v4(there, reinterpret_cast<const uint4*>(&t)[0]);
+                    st_cluster_v4(there + 16, reinterpret_cast<const uint4*>(&t)[1]);
+                    mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
+                } else {
+                    if (!mbar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
+                    t = s_task[slot];
+                    mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
                 }
-                s_index[slot] = end ? kEnd : idx;
-                mbar_arrive(smem_u32(&task_full[slot]));
-                if (end) break;
-                claim = atomicAdd(a.next, 1u);
+                if (t.stack == kEnd) break;
                 const NsStack& s = a.stacks[t.stack];
                 const CUtensorMap* maps = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack;
                 if (t.need) {
                     if (!wait_done(a.done + s.first + t.index, t.need, &s_err, a.err)) break;
-                    fence_async_proxy();  // written by other SMs' ordinary stores
+                    fence_async_proxy();  // (other SMs' stores, by TMA)
                 }
-                const uint32_t row = t.row * kNsTileM, col = t.col * 16u;
                 const int xmap = (t.step & 1) ? kMapX1 : kMapX0;
                 const bool bx = t.kind >= kNsBX;
                 const int ma = t.kind == kNsXXt ? xmap : t.kind == kNsAA ? kMapA : kMapB;
                 const int mb = t.kind == kNsAA ? static_cast<int>(kMapA) : xmap;
                 const uint32_t depth = t.kind == kNsXXt ? s.n : s.m;
-                const uint32_t boxes_a = s.m - row > 64 ? 2 : 1, boxes_b = (t.width + 63u) / 64u;
-                const uint32_t bytes = (boxes_a + boxes_b) * kNsBoxBytes;
+                // this CTA's 128 rows of the first operand, its half of the second one's columns
+                const uint32_t row = t.row * kNsTileM + rank * kNsRows;
+                const uint32_t n_half = ((t.width + 31u) & ~31u) / 2;
+                const uint32_t col = t.col * 32u + rank * n_half;
+                const uint32_t row0 = t.row * kNsTileM;
+                auto row_boxes = [&](uint32_t r) { return r >= s.m ? 0u : s.m - r > 64 ? 2u : 1u; };
+                const uint32_t boxes_a = row_boxes(row), boxes_b = (n_half + 63u) / 64u;
+                const uint32_t bytes =
+                    (row_boxes(row0) + row_boxes(row0 + kNsRows) + 2 * boxes_b) * kNsBoxBytes;
+                const uint32_t passes = s.three ? 3 : 1;
                 bool ok = true;
-                for (uint32_t p = 0; p < kPasses && ok; ++p) {
+                for (uint32_t p = 0; p < passes && ok; ++p) {
                     // the small products first: lo hi, hi lo, hi hi
-                    const CUtensorMap* mapa = maps + ma + (kThree && p == 0 ? kMapLo : 0);
-                    const CUtensorMap* mapb = maps + mb + (kThree && p == 1 ? kMapLo : 0);
+                    const CUtensorMap* mapa = maps + ma + (s.three && p == 0 ? kMapLo : 0);
+                    const CUtensorMap* mapb = maps + mb + (s.three && p == 1 ? kMapLo : 0);
                     for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK, ++it) {
                         const uint32_t st = it % kNsStages;
                         if (it >= kNsStages &&
@@ -423,46 +575,51 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                             ok = false;
                             break;
                         }
-                        const uint32_t bar = smem_u32(&full_bar[st]);
+                        // both CTAs' bytes count on the leader's barrier
+                        const uint32_t bar = map_to(smem_u32(&full_bar[st]), 0);
                         const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
-                        mbar_expect_tx(bar, bytes);
+                        if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[st]), bytes);
                         for (uint32_t i = 0; i < boxes_a; ++i)
-                            tma_load_3d(sa + i * kNsBoxBytes, mapa, bar, k0, row + 64 * i, t.index);
+                            tma_load_pair(sa + i * kNsBoxBytes, mapa, bar, k0, row + 64 * i, t.index);
                         for (uint32_t i = 0; i < boxes_b; ++i) {
                             if (bx)
-                                tma_load_3d(sb + i * kNsBoxBytes, mapb, bar, col + 64 * i, k0, t.index);
+                                tma_load_pair(sb + i * kNsBoxBytes, mapb, bar, col + 64 * i, k0, t.index);
                             else
-                                tma_load_3d(sb + i * kNsBoxBytes, mapb, bar, k0, col + 64 * i, t.index);
+                                tma_load_pair(sb + i * kNsBoxBytes, mapb, bar, k0, col + 64 * i, t.index);
                         }
                     }
                 }
                 if (!ok) break;
             }
-            if (*reinterpret_cast<volatile int*>(&s_err)) {
+            if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0) {
                 // copies in flight land before the CTA may end
                 for (uint32_t j = it > kNsStages ? it - kNsStages : 0; j < it; ++j)
                     mbar_wait(smem_u32(&full_bar[j % kNsStages]), (j / kNsStages) & 1, &s_drain_err);
             }
         }
     } else if (warp == 1) {
-        // ---- one thread issues the products ----
-        if (lane == 0) {
+        // ---- the leader's thread issues the pair's products ----
+        if (lane == 0 && rank == 0) {
             uint32_t it = 0;
             for (uint32_t q = 0;; ++q) {
                 const uint32_t slot = q % kRing, buf = q & 1;
                 if (!mbar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
-                if (s_index[slot] == kEnd) break;
                 const NsTask t = s_task[slot];
+                if (t.stack == kEnd) break;
                 mbar_arrive(smem_u32(&task_empty[slot]));
-                if (q >= 2 && !mbar_wait(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err)) break;
-                tc_fence_after();
                 const NsStack& s = a.stacks[t.stack];
                 const bool bx = t.kind >= kNsBX;
-                const uint32_t idesc = instr_desc((t.width + 15u) & ~15u, bx);
+                const uint32_t n = (t.width + 31u) & ~31u;
+                const uint32_t idesc = instr_desc(n, bx);
                 const uint32_t depth = t.kind == kNsXXt ? s.n : s.m;
                 const uint32_t d = tmem + buf * kNsTileN;
+                const uint32_t blocks = (depth + kNsTileK - 1) / kNsTileK;
+                // three products: the last one's first half has an accumulator of its own
+                const uint32_t from = s.three ? 2 * blocks : 0, to = from + (s.three ? blocks / 2 : 0);
+                const uint32_t steps = s.three ? 3 * blocks : blocks;
+                if (q >= 2 && !mbar_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err)) break;
+                tc_fence_after();
                 bool ok = true;
-                const uint32_t steps = kPasses * ((depth + kNsTileK - 1) / kNsTileK);
                 for (uint32_t j = 0; j < steps; ++j, ++it) {
                     const uint32_t st = it % kNsStages;
                     if (!mbar_wait(smem_u32(&full_bar[st]), (it / kNsStages) & 1, &s_err)) {
@@ -471,12 +628,15 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                     }
                     tc_fence_after();
                     const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
+                    const bool second = j >= from && j < to;
+                    const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
+                    const bool fresh = j == 0 || (second && j == from);
 #pragma unroll
                     for (uint32_t k = 0; k < kNsTileK / 16; ++k)
-                        mma_f16(d, operand_desc(sa + k * 32, 16),
+                        mma_f16(dd, operand_desc(sa + k * 32, 16),
                                 bx ? operand_desc(sb + k * 2048, kNsBoxBytes)
                                    : operand_desc(sb + k * 32, 16),
-                                idesc, j + k > 0);
+                                idesc, !(fresh && k == 0));
                     mma_commit(smem_u32(&empty_bar[st]));
                 }
                 if (!ok) break;
@@ -488,130 +648,214 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             }
         }
     } else {
-        // ---- four warps turn accumulators into operands or results ----
-        const uint32_t quad = warp & 3;  // the TMEM lanes this warp may read
-        const uint32_t tlane = quad * 32 + lane;
+        // ---- eight warps turn accumulators into operands or results ----
+        const uint32_t ew = warp - 2, quad = warp & 3, half = ew >> 2;
+        const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
+        const bool first = threadIdx.x == 64;    // issues the epilogue's copies
+        uint32_t uses[2] = {0, 0};               // addends waited for, per buffer
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = mbar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
-            const bool end = ok && s_index[slot] == kEnd;
+            bool ok = mbar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            const NsTask t = s_task[slot];
+            const bool end = ok && t.stack == kEnd;
+            const NsStack& s = a.stacks[ok && !end ? t.stack : 0];
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(ok && !end ? t.stack : 0) * kMapsPerStack;
+            const bool sym = t.kind <= kNsAA, three = s.three != 0;
+            const uint32_t row0 = t.row * kNsTileM + rank * kNsRows, col0 = t.col * 32u;
+            const bool some = row0 < s.m;  // this CTA has rows in the tile
+            const bool addend = t.kind != kNsXXt && some;
+            const bool lo = !sym || three;  // addend and result have a lo part
+            // slots of one chunk: hi, lo (where it has one), then the mirror's; two chunks
+            // at a time where they fit
+            const uint32_t pair = sym && three ? 0u : 1u;
+            const uint32_t cols = sym ? s.m : s.n;
+            const uint32_t chunks = (t.width + 63u) / 64u;
+            const int in = t.step & 1;
+            const CUtensorMap* src = maps + (sym ? static_cast<int>(kMapA) : kMapX0 + in);
+            auto load_addend = [&](uint32_t c) {
+                const uint32_t b = c & pair, at = staging + b * 2 * kNsSlotBytes;
+                const uint32_t bar = smem_u32(&stage_bar[b]);
+                const uint32_t boxes = s.m - row0 > 64 ? 2 : 1;
+                mbar_expect_tx(bar, boxes * (lo ? 2 : 1) * kNsBoxBytes);
+                for (uint32_t i = 0; i < boxes; ++i) {
+                    tma_load(at + i * kNsBoxBytes, src, bar, col0 + c * 64, row0 + i * 64, t.index);
+                    if (lo)
+                        tma_load(at + kNsSlotBytes + i * kNsBoxBytes, src + kMapLo, bar, col0 + c * 64,
+                                 row0 + i * 64, t.index);
+                }
+            };
+            if (ok && !end && addend && first) {
+                ok = wait_done(a.done + s.first + t.index, t.need, &s_err, a.err);
+                if (ok) {
+                    fence_async_proxy();
+                    load_addend(0);
+                    if (pair && chunks > 1) load_addend(1);
+                }
+            }
             if (ok && !end) ok = mbar_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
             if (!ok) s_cfail[q & 1] = 1;
-            consumers_sync<128>();
+            consumers_sync<kEpi>();
             if (s_cfail[q & 1] || end) break;
-            const NsTask t = s_task[slot];
-            consumers_sync<128>();
-            if (threadIdx.x == 64) mbar_arrive(smem_u32(&task_empty[slot]));
+            if (first) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
             tc_fence_after();
-            const NsStack& s = a.stacks[t.stack];
-            const uint32_t r = t.row * kNsTileM + tlane;
-            const uint32_t col0 = t.col * 16u;
-            const bool sym = t.kind <= kNsAA;
-            const uint32_t cols = sym ? s.m : s.n;
             const float ca = a.coef[t.step][0], cb = a.coef[t.step][1], cc = a.coef[t.step][2];
-            const uint64_t abase = static_cast<uint64_t>(t.index) * s.m * s.lda;
-            const uint64_t xbase = static_cast<uint64_t>(t.index) * s.m * s.ldx;
-            for (uint32_t c = 0; c < t.width; c += 32) {
+            bool bad = false;
+            for (uint32_t c = 0; c < chunks; ++c) {
+                const uint32_t b = c & pair, at = staging + b * 2 * kNsSlotBytes;
                 float v[32];
                 __syncwarp();
-                tmem_ld32(tmem + buf * kNsTileN + ((quad * 32u) << 16) + c, v);
-                const uint32_t col = col0 + c;
-                if (r >= s.m || col >= cols) continue;
-                const uint32_t left = cols - col;
-                if (sym) {
-                    __half* hp = t.kind == kNsXXt ? s.a : s.b;
-                    __half* lp = t.kind == kNsXXt ? s.al : s.bl;
-                    const uint64_t at = abase + static_cast<uint64_t>(r) * s.lda + col;
-                    if (t.kind == kNsXXt) {
-                        const float f = kNsScaleA / (s.sx * s.sx);
+                tmem_ld32(tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32, v);
+                if (three) {
+                    float w[32];
+                    tmem_ld32(tmem + buf * kNsTileN + kNsTileN / 2 + ((quad * 32u) << 16) + c * 64 + half * 32, w);
+                    // (a depth of one stage has no second accumulator)
+                    if ((t.kind == kNsXXt ? s.n : s.m) > kNsTileK) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= f;
-                    } else {
-                        float x[32];
-                        load_row32(s.a + at, left, x);
-                        if constexpr (kThree) {
-                            float y[32];
-                            load_row32(s.al + at, left, y);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) x[j] += y[j];
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = cb * x[j] + (cc / kNsScaleA) * v[j];
+                        for (int j = 0; j < 32; ++j) v[j] += w[j];
                     }
-                    store_row32<kThree>(hp + at, lp + at, left, v);
-                    // the mirror image: right of the block on the diagonal
-                    if (col >= (t.row + 1u) * kNsTileM) {
-                        const uint64_t to = abase + static_cast<uint64_t>(col) * s.lda + r;
+                }
+                if (c + 1 == chunks) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+                }
+                if (!some) continue;
+                const uint32_t col = col0 + c * 64;
+                if (addend) {
+                    if (!mbar_wait(smem_u32(&stage_bar[b]), uses[b] & 1, &s_err)) bad = true;
+                    ++uses[b];
+                    float x[32];
+                    slot_read<false>(at, trow, half, x);
+                    if (lo) slot_read<true>(at + kNsSlotBytes, trow, half, x);
+                    const float fx = sym ? cb : ca, fv = sym ? cc / kNsScaleA : 1.0f / kNsScaleA;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (static_cast<uint32_t>(j) >= left) break;
-                            __half hi, lo;
-                            split_half(v[j], hi, lo);
-                            hp[to + static_cast<uint64_t>(j) * s.lda] = hi;
-                            if constexpr (kThree) lp[to + static_cast<uint64_t>(j) * s.lda] = lo;
-                        }
-                    }
+                    for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(fx, x[j], fv * v[j]);
                 } else {
-                    const int in = t.step & 1;
-                    const uint64_t at = xbase + static_cast<uint64_t>(r) * s.ldx + col;
-                    {
-                        float x[32], y[32];
-                        load_row32(s.x[in] + at, left, x);
-                        load_row32(s.xl[in] + at, left, y);
+                    const float f = kNsScaleA / (s.sx * s.sx);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            v[j] = ca * (x[j] + y[j]) + v[j] * (1.0f / kNsScaleA);
+                    for (int j = 0; j < 32; ++j) v[j] *= f;
+                    // the buffer's last stores have read it
+                    if (first) {
+                        if (pair && c > 0) bulk_wait_read<1>();
+                        else bulk_wait_read<0>();
                     }
-                    if (t.kind == kNsBX) {
-                        store_row32<true>(s.x[in ^ 1] + at, s.xl[in ^ 1] + at, left, v);
-                    } else {
-                        const float f = 1.0f / s.sx;
-                        const uint64_t mat = t.index;
+                    consumers_sync<kEpi>();
+                }
+                if (t.kind == kNsLast) {
+                    // through shared memory as floats, so that the result is written row by row
+                    // of the caller's matrix
+                    const float f = 1.0f / s.sx;
+                    float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
+                    consumers_sync<kEpi>();  // (all have read their addend)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            if (static_cast<uint32_t>(j) >= left) break;
-                            const float o = v[j] * f;
-                            const uint64_t orow = s.transposed ? col + j : r;
-                            const uint64_t ocol = s.transposed ? r : col + j;
-                            if constexpr (kDst == kDstF32) {
-                                static_cast<float*>(s.dst)[mat * s.dst_mat + orow * s.dst_row + ocol] = o;
-                            } else if constexpr (kDst == kDstBf16) {
-                                static_cast<uint16_t*>(
-                                    s.dst)[mat * s.dst_mat + orow * s.dst_row + ocol] = f32_to_bf16_rn(o);
-                            } else {
-                                const uint64_t e = (mat * s.rows + orow) * s.cols + ocol;
-                                float w = s.master[e];
-                                if (s.wd != 0.0f)
-                                    w = __fsub_rn(w, __fmul_rn(__fmul_rn(step.lr, s.wd), w));
-                                w = __fsub_rn(w, __fmul_rn(__fmul_rn(step.lr, s.factor), o));
-                                s.master[e] = w;
-                                if constexpr (kDst == kDstParamMixed)
-                                    static_cast<uint16_t*>(s.param)[e] = f32_to_bf16_rn(w);
-                                if (a.ema) {
-                                    float* sh = s.mom + step.ema_delta;
-                                    sh[e] = __fadd_rn(__fmul_rn(step.ema_decay, sh[e]),
-                                                      __fmul_rn(step.ema_omd, w));
-                                }
+                    for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
+                    consumers_sync<kEpi>();
+                    const uint64_t base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
+                                                : static_cast<uint64_t>(t.index) * s.dst_mat;
+                    const uint64_t pitch = kMuon ? s.cols : s.dst_row;
+#pragma unroll 1
+                    for (int g = 0; g < 4; ++g) {
+                        uint64_t to[8];
+                        float o[8];
+                        uint32_t valid = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t e = g * 8 + i;
+                            const uint32_t rr = s.transposed ? lane + 32 * (e & 3) : ew * 16 + (e >> 1);
+                            const uint32_t rc = s.transposed ? ew * 8 + (e >> 2) : lane + 32 * (e & 1);
+                            const uint32_t y = row0 + rr, x = col + rc;
+                            to[i] = base + (s.transposed ? x * pitch + y : y * pitch + x);
+                            o[i] = fs[float_at(rr, rc)];
+                            if (y < s.m && x < s.n) valid |= 1u << i;
+                        }
+                        put_result<kDst>(a, step, s, to, o, valid);
+                    }
+                    fence_async_proxy();
+                    consumers_sync<kEpi>();
+                    if (first && c + 2 < chunks) load_addend(c + 2);
+                    continue;
+                }
+                // hi and lo in place of the addend, and the mirror image beside them
+                const bool mirror = sym && col >= (t.row + 1u) * kNsTileM;
+                const uint32_t image = at + (lo ? 2 : 1) * kNsSlotBytes;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
+                    const uint32_t o = slot_at(trow, half * 4 + j);
+                    sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
+                    if (lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
+                    if (mirror) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
+                            const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
+                            sts16(image + m0, h[e] & 0xFFFFu);
+                            sts16(image + m1, h[e] >> 16);
+                            if (lo) {
+                                sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
+                                sts16(image + kNsSlotBytes + m1, l[e] >> 16);
                             }
                         }
                     }
                 }
+                fence_async_proxy();
+                consumers_sync<kEpi>();
+                if (first) {
+                    const CUtensorMap* dst =
+                        maps + (t.kind == kNsXXt ? static_cast<int>(kMapA)
+                                                 : t.kind == kNsAA ? static_cast<int>(kMapB) : kMapX0 + (in ^ 1));
+                    for (uint32_t i = 0; i < 2 && row0 + i * 64 < s.m; ++i) {
+                        tma_store(dst, at + i * kNsBoxBytes, col, row0 + i * 64, t.index);
+                        if (lo)
+                            tma_store(dst + kMapLo, at + kNsSlotBytes + i * kNsBoxBytes, col, row0 + i * 64,
+                                      t.index);
+                        if (mirror) {
+                            tma_store(dst, image + i * kNsBoxBytes, row0 + i * 64, col, t.index);
+                            if (lo)
+                                tma_store(dst + kMapLo, image + kNsSlotBytes + i * kNsBoxBytes, row0 + i * 64,
+                                          col, t.index);
+                        }
+                    }
+                    bulk_commit();
+                    if (addend) {
+                        // the next chunk but one of a pair of buffers (the next of one): its
+                        // buffer's stores have read it
+                        if (!pair) {
+                            if (c + 1 < chunks) {
+                                bulk_wait_read<0>();
+                                load_addend(c + 1);
+                            }
+                        } else if (c >= 1 && c + 1 < chunks) {
+                            bulk_wait_read<1>();
+                            load_addend(c + 1);
+                        }
+                    }
+                }
             }
-            tc_fence_before();
-            mbar_arrive(smem_u32(&acc_empty[buf]));
-            // this tile's stores, before it counts as done
-            __threadfence();
-            fence_async_proxy();
-            consumers_sync<128>();
-            if (threadIdx.x == 64) red_release_add1(a.done + s.first + t.index);
+            if (bad) s_cfail[(q + 1) & 1] = 1;  // (read after the next tile's first barrier)
+            if (first) {
+                bulk_wait_all();  // this tile's stores, before it counts as done
+                fence_async_proxy();
+                __threadfence();
+                red_release_add1(a.done + s.first + t.index);
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && (s_err | s_drain_err)) {
+        atomicOr(a.err, 1);
+        // the other CTA's copies may still be landing here, or counting on barriers here
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {}
+    }
+    __syncthreads();
+    cluster_sync();  // the other CTA may use this one's shared memory until it is done too
     tc_fence_after();
-    if (threadIdx.x == 0 && (s_err | s_drain_err)) atomicOr(a.err, 1);
     if (warp == 1)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <int kSrc>
@@ -625,8 +869,8 @@ cudaError_t launch_prep(const MatrixArgs& a, Ctl* ctl, const ApplyArgs& step, in
 
 template <int kDst>
 cudaError_t launch_ns(const MatrixArgs& a, const ApplyArgs& step, int sms, cudaStream_t stream) {
-    const int grid = static_cast<int>(std::min<uint64_t>(a.n_tasks, static_cast<uint64_t>(sms)));
-    return launch_pdl(k_ns<kDst>, dim3(grid), dim3(kNsThreads), kNsSmemBytes, stream, a, step);
+    const int pairs = static_cast<int>(std::min<uint64_t>(a.n_tasks, static_cast<uint64_t>(sms / 2)));
+    return launch_pdl(k_ns<kDst>, dim3(2 * pairs), dim3(kNsThreads), kNsSmemBytes, stream, a, step);
 }
 
 }  // namespace

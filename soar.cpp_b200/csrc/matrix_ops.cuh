@@ -38,15 +38,23 @@ namespace soarb {
 constexpr int kNsMaxSteps = 16;
 constexpr float kNsScaleA = 1024.0f;  // A and B are held times this
 
-// Tile of a product: kNsTileM rows by at most kNsTileN columns, kNsTileK deep per stage.
-constexpr int kNsTileM = 128;
+// Tile of a product: 256 rows by at most 256 columns, by a pair of CTAs (a
+// cluster of two): each holds 128 rows of the first operand, half of the second
+// one's columns and the accumulator of its 128 rows. A pair's tile needs two
+// thirds of the operand traffic of two 128 x 256 tiles.
+constexpr int kNsTileM = 256;
 constexpr int kNsTileN = 256;
-constexpr int kNsTileK = 64;
-constexpr int kNsStages = 4;
-constexpr int kNsThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+constexpr int kNsRows = 128;   // a CTA's share of the rows
+constexpr int kNsTileK = 64;   // depth of one stage
+constexpr int kNsStages = 5;
+constexpr int kNsEpilogueWarps = 8;
+constexpr int kNsThreads = (2 + kNsEpilogueWarps) * 32;  // TMA warp, MMA warp, epilogue
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
-constexpr uint32_t kNsStageBytes = (kNsTileM + kNsTileN) * kNsTileK * 2;
-constexpr size_t kNsSmemBytes = static_cast<size_t>(kNsStages) * kNsStageBytes + 1024;
+constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
+constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue staging: 128 rows of 64 fp16
+constexpr int kNsSlots = 4;
+constexpr size_t kNsSmemBytes =
+    static_cast<size_t>(kNsStages) * kNsStageBytes + kNsSlots * kNsSlotBytes + 1024;
 
 // Tensor maps of a stack: {X hi 0, X hi 1, A hi, B hi, X lo 0, X lo 1, A lo, B lo}.
 enum NsMap { kMapX0 = 0, kMapX1 = 1, kMapA = 2, kMapB = 3, kMapLo = 4, kMapsPerStack = 8 };
@@ -65,6 +73,7 @@ struct NsStack {
     uint32_t count;
     uint32_t first;       // index of its first matrix in the plan
     uint32_t transposed;  // rows > cols: X is the transpose
+    uint32_t three;       // products in three parts
     uint32_t tiles;       // preparation tiles per matrix
     uint32_t first_tile;
     float sx;             // power of two X is held by
@@ -94,8 +103,8 @@ enum NsKind : uint32_t { kNsXXt = 0, kNsAA = 1, kNsBX = 2, kNsLast = 3 };
 struct __align__(16) NsTask {
     uint32_t stack;
     uint32_t index;   // matrix of the stack
-    uint32_t need;    // tiles of this matrix that must be done before
-    uint16_t row, col;  // first row and column, in units of 128 and 16
+    uint32_t need;    // CTAs' tiles of this matrix that must be done before
+    uint16_t row, col;  // first row and column, in units of 256 and 32
     uint16_t width;   // columns
     uint8_t kind;
     uint8_t step;
@@ -122,7 +131,7 @@ struct MatrixArgs {
     double* partials;      // one per preparation tile
     uint32_t* tickets;     // per matrix: preparation tiles summed (0 between launches)
     float* inv;            // per matrix: sx / (norm + eps)
-    uint32_t* done;        // per matrix: product tiles done
+    uint32_t* done;        // per matrix: product tiles done, counted by each CTA of a pair
     uint32_t* next;        // tasks handed out
     MatrixStep* step;
     int* err;              // nonzero: a wait ran out

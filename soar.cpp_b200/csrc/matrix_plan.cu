@@ -47,15 +47,16 @@ bool encode(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, u
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tiles of one product of one matrix: (first row / 128, first column / 16, width).
+// Tiles of one product of one matrix: (first row / 256, first column / 32, width).
 struct Tile {
     uint16_t row, col, width;
 };
+// A symmetric product: the blocks on the diagonal and what is right of them.
 std::vector<Tile> symmetric_tiles(uint32_t m, uint32_t wide) {
     std::vector<Tile> out;
     for (uint32_t r = 0; r * kNsTileM < m; ++r)
         for (uint32_t c = r * kNsTileM; c < m; c += wide)
-            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 16),
+            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 32),
                            static_cast<uint16_t>(std::min(wide, m - c))});
     return out;
 }
@@ -63,9 +64,13 @@ std::vector<Tile> full_tiles(uint32_t m, uint32_t n, uint32_t wide) {
     std::vector<Tile> out;
     for (uint32_t c = 0; c < n; c += wide)
         for (uint32_t r = 0; r * kNsTileM < m; ++r)
-            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 16),
+            out.push_back({static_cast<uint16_t>(r), static_cast<uint16_t>(c / 32),
                            static_cast<uint16_t>(std::min(wide, n - c))});
     return out;
+}
+std::vector<Tile> product_tiles(const NsStack& s, uint32_t kind, uint32_t wide) {
+    if (s.three) wide = std::min(wide, static_cast<uint32_t>(kNsTileN / 2));
+    return kind == kNsBX ? full_tiles(s.m, s.n, wide) : symmetric_tiles(s.m, wide);
 }
 
 }  // namespace
@@ -144,6 +149,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.cols = static_cast<uint32_t>(q.cols);
         s.count = static_cast<uint32_t>(q.count);
         s.transposed = s.rows > s.cols;
+        s.three = three;
         s.m = std::min(s.rows, s.cols);
         s.n = std::max(s.rows, s.cols);
         s.ldx = static_cast<uint32_t>(up(s.n, 8));
@@ -203,10 +209,17 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         std::vector<uint32_t> counted(wave.size(), 0);  // tiles of a matrix before this product
         for (int step = 0; step < opts.steps; ++step) {
             for (uint32_t kind = kNsXXt; kind <= kNsBX; ++kind) {
+                // narrower tiles where whole ones would leave pairs of CTAs idle
+                uint32_t wide = kNsTileN;
+                for (; wide > 64; wide /= 2) {
+                    uint64_t all = 0;
+                    for (const Run& r : wave)
+                        all += product_tiles(stacks[r.stack], kind, wide).size() * (r.to - r.from);
+                    if (all >= static_cast<uint64_t>(plan->sms / 2)) break;
+                }
                 for (size_t w = 0; w < wave.size(); ++w) {
                     const NsStack& s = stacks[wave[w].stack];
-                    const std::vector<Tile> tiles =
-                        kind == kNsBX ? full_tiles(s.m, s.n, kNsTileN) : symmetric_tiles(s.m, kNsTileN);
+                    const std::vector<Tile> tiles = product_tiles(s, kind, wide);
                     for (uint32_t i = wave[w].from; i < wave[w].to; ++i)
                         for (const Tile& t : tiles) {
                             NsTask k{};
@@ -221,7 +234,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                             k.step = static_cast<uint8_t>(step);
                             tasks.push_back(k);
                         }
-                    counted[w] += static_cast<uint32_t>(tiles.size());
+                    counted[w] += 2 * static_cast<uint32_t>(tiles.size());
                 }
             }
         }
