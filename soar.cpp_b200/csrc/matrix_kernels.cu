@@ -210,10 +210,14 @@ __device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
+// One lane of a converged warp, the same at every call. (Copies and products are
+// issued from converged warps: their operands then stay in uniform registers.
+// From a loop of one lane, each instruction cost 130 to 330 cycles, a stage of
+// four copies more than 1000 where its products take 512.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile(
@@ -235,10 +239,33 @@ __device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) 
         : "memory");
     return ok != 0;
 }
-// mbar_wait for a barrier the other CTA arrives on.
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
-    if (!mbar_wait(bar, parity, s_err)) return false;
-    mbar_try_cluster(bar, parity);  // (complete: acquires at cluster scope)
+// Bounded waits, as pipeline.cuh's mbar_wait and wait_flags; the clock is first
+// read after a thousand failed tries (%globaltimer is slow to read).
+struct Patience {
+    uint64_t t0 = 0;
+    uint32_t tries = 0;
+    // false: give up
+    __device__ __forceinline__ bool more(int* s_err) {
+        if ((++tries & 1023u) != 0) return true;
+        if (*reinterpret_cast<volatile int*>(s_err)) return false;  // another thread gave up
+        const uint64_t now = global_timer_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 <= kWaitLimitNs) return true;
+        atomicOr(s_err, 1);
+        return false;
+    }
+};
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* s_err) {
+    Patience p;
+    while (!mbar_try(bar, parity))
+        if (!p.more(s_err)) return false;
+    return true;
+}
+// bar_wait for a barrier the other CTA arrives on.
+__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
+    Patience p;
+    while (!mbar_try_cluster(bar, parity))
+        if (!p.more(s_err)) return false;
     return true;
 }
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint4& v) {
@@ -254,6 +281,14 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* m
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
         "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                              uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
 }
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, uint32_t x,
@@ -327,6 +362,9 @@ __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_shared() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t ld_acquire(const uint32_t* p) {
     uint32_t v;
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -339,28 +377,25 @@ __device__ __forceinline__ void red_release_add1(uint32_t* p) {
 // Bounded wait until *p >= need; gives up when the kernel's error word is set.
 __device__ __forceinline__ bool wait_done(const uint32_t* p, uint32_t need, int* s_err,
                                           const int* err) {
-    if (ld_acquire(p) >= need) return true;
-    const uint64_t t0 = global_timer_ns();
-    for (uint32_t i = 1;; ++i) {
-        if (ld_acquire(p) >= need) return true;
-        if ((i & 63u) == 0) {
-            if (global_timer_ns() - t0 > kWaitLimitNs || *reinterpret_cast<const volatile int*>(err)) {
-                atomicOr(s_err, 1);
-                return false;
-            }
-            if (*reinterpret_cast<volatile int*>(s_err)) return false;
+    Patience wait;
+    while (ld_acquire(p) < need) {
+        if (!wait.more(s_err)) return false;
+        if ((wait.tries & 1023u) == 0 && *reinterpret_cast<const volatile int*>(err)) {
+            atomicOr(s_err, 1);
+            return false;
         }
     }
+    return true;
 }
 
 // ---------------------------------------------------------------- staging ---
 // The epilogue's operands pass through shared memory in chunks of 64 columns
-// of the CTA's 128 rows: a slot holds one fp16 chunk as TMA has it (two boxes
-// of 64 rows of 128 bytes, 128-byte swizzle).
+// of the CTA's 128 rows: a slot holds one fp16 chunk as TMA has it (rows of 128
+// bytes, 128-byte swizzle).
 
 // Byte offset of eight columns (group j of 8) of a row in a slot.
 __device__ __forceinline__ uint32_t slot_at(uint32_t row, uint32_t j) {
-    return (row >> 6) * kNsBoxBytes + (row & 63u) * 128u + ((j ^ (row & 7u)) << 4);
+    return row * 128u + ((j ^ (row & 7u)) << 4);
 }
 // Byte offset of (row, col) in a slot that holds the chunk's transpose: 64
 // rows (its columns) of 128 (its rows), in two boxes of 64 x 64.
@@ -417,8 +452,17 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 
 // One wave of eight elements of the result, each lane's own: the stack's
 // destination, or Muon's update of the weights there.
+// Where a stack's result goes, in registers.
+struct Target {
+    void* dst;          // the destination, or the parameters
+    float* master;
+    float* ema;
+    uint64_t base, pitch;
+    float lr_wd, lr_s;  // Muon: lr times the weight decay, and times the shape factor
+};
+
 template <int kDst>
-__device__ __forceinline__ void put_result(const MatrixArgs& a, const ApplyArgs& step, const NsStack& s,
+__device__ __forceinline__ void put_result(const ApplyArgs& step, const Target& s, bool ema,
                                            const uint64_t (&at)[8], const float (&o)[8], uint32_t valid) {
     if constexpr (kDst == kDstF32 || kDst == kDstBf16) {
 #pragma unroll
@@ -431,28 +475,26 @@ __device__ __forceinline__ void put_result(const MatrixArgs& a, const ApplyArgs&
         }
     } else {
         float w[8], e[8];
-        float* sh = s.mom + step.ema_delta;
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = valid >> i & 1u ? s.master[at[i]] : 0.0f;
-        if (a.ema) {
+        if (ema) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = valid >> i & 1u ? sh[at[i]] : 0.0f;
+            for (int i = 0; i < 8; ++i) e[i] = valid >> i & 1u ? s.ema[at[i]] : 0.0f;
         }
-        const float lr_wd = __fmul_rn(step.lr, s.wd), lr_s = __fmul_rn(step.lr, s.factor);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (s.wd != 0.0f) w[i] = __fsub_rn(w[i], __fmul_rn(lr_wd, w[i]));
-            w[i] = __fsub_rn(w[i], __fmul_rn(lr_s, o[i]));
+            if (s.lr_wd != 0.0f) w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_wd, w[i]));
+            w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_s, o[i]));
             if (!(valid >> i & 1u)) continue;
             s.master[at[i]] = w[i];
             if constexpr (kDst == kDstParamMixed)
-                static_cast<uint16_t*>(s.param)[at[i]] = f32_to_bf16_rn(w[i]);
+                static_cast<uint16_t*>(s.dst)[at[i]] = f32_to_bf16_rn(w[i]);
         }
-        if (a.ema) {
+        if (ema) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (valid >> i & 1u)
-                    sh[at[i]] = __fadd_rn(__fmul_rn(step.ema_decay, e[i]), __fmul_rn(step.ema_omd, w[i]));
+                    s.ema[at[i]] = __fadd_rn(__fmul_rn(step.ema_decay, e[i]), __fmul_rn(step.ema_omd, w[i]));
         }
     }
 }
@@ -478,7 +520,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     if constexpr (kMuon) {
         if (a.step->skip) return;
     }
-    const uint32_t rank = cluster_rank();  // 0 leads the pair: hands out tasks, issues products
+    const uint32_t rank = blockIdx.x & 1u;  // 0 leads the pair: hands out tasks, issues products
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t staging = smem + kNsStages * kNsStageBytes;
     if (threadIdx.x == 0) {
@@ -513,140 +555,151 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
 
     if (warp == 0) {
         // ---- takes tasks, waits for their inputs, loads operand tiles ----
-        if (lane == 0) {
-            fence_async_proxy();  // (X of the kernel before)
-            uint32_t it = 0;      // stages issued
-            uint32_t claim = rank == 0 ? atomicAdd(a.next, 1u) : 0u;
-            for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q % kRing;
-                NsTask t{};
-                if (rank == 0) {
-                    if (q >= kRing &&
-                        !mbar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
-                        break;
-                    if (claim < a.n_tasks) {
-                        t = a.tasks[claim];
-                        claim = atomicAdd(a.next, 1u);
-                    } else {
-                        t.stack = kEnd;
+        fence_async_proxy();  // (X of the kernel before)
+        uint32_t st = 0, phase = 1;  // the next stage; its empty barrier's phase to wait for
+        uint32_t issued = 0;
+        // a task is read one task ahead, and its number taken two ahead
+        NsTask ahead{};
+        uint32_t claim = 0;
+        auto read_ahead = [&]() {
+            if (claim < a.n_tasks) ahead = a.tasks[claim];
+            else ahead.stack = kEnd;
+            claim = atomicAdd(a.next, 1u);
+        };
+        if (rank == 0 && lane == 0) {
+            claim = atomicAdd(a.next, 1u);
+            read_ahead();
+        }
+        for (uint32_t q = 0;; ++q) {
+            const uint32_t slot = q % kRing;
+            bool ok = true;
+            if (rank == 0) {
+                if (lane == 0) {
+                    if (q >= kRing) ok = bar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err);
+                    if (ok) {
+                        s_task[slot] = ahead;
+                        mbar_arrive(smem_u32(&task_full[slot]));
+                        const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
+#pragma unroll
+                        for (int i = 0; i < 3; ++i)  // (the rest is padding)
+                            st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&ahead)[i]);
+                        mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
+                        if (ahead.stack != kEnd) read_ahead();
                     }
-                    s_task[slot] = t;
-                    mbar_arrive(smem_u32(&task_full[slot]));
-                    const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
-                    st_cluster_v4(there, reinterpret_cast<const uint4*>(&t)[0]);
-                    st_cluster_v4(there + 16, reinterpret_cast<const uint4*>(&t)[1]);
-                    mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
-                } else {
-                    if (!mbar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
-                    t = s_task[slot];
-                    mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
                 }
-                if (t.stack == kEnd) break;
-                const NsStack& s = a.stacks[t.stack];
-                const CUtensorMap* maps = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack;
-                if (t.need) {
-                    if (!wait_done(a.done + s.first + t.index, t.need, &s_err, a.err)) break;
-                    fence_async_proxy();  // (other SMs' stores, by TMA)
-                }
-                const int xmap = (t.step & 1) ? kMapX1 : kMapX0;
-                const bool bx = t.kind >= kNsBX;
-                const int ma = t.kind == kNsXXt ? xmap : t.kind == kNsAA ? kMapA : kMapB;
-                const int mb = t.kind == kNsAA ? static_cast<int>(kMapA) : xmap;
-                const uint32_t depth = t.kind == kNsXXt ? s.n : s.m;
-                // this CTA's 128 rows of the first operand, its half of the second one's columns
-                const uint32_t row = t.row * kNsTileM + rank * kNsRows;
-                const uint32_t n_half = ((t.width + 31u) & ~31u) / 2;
-                const uint32_t col = t.col * 32u + rank * n_half;
-                const uint32_t row0 = t.row * kNsTileM;
-                auto row_boxes = [&](uint32_t r) { return r >= s.m ? 0u : s.m - r > 64 ? 2u : 1u; };
-                const uint32_t boxes_a = row_boxes(row), boxes_b = (n_half + 63u) / 64u;
-                const uint32_t bytes =
-                    (row_boxes(row0) + row_boxes(row0 + kNsRows) + 2 * boxes_b) * kNsBoxBytes;
-                const uint32_t passes = s.three ? 3 : 1;
-                bool ok = true;
-                for (uint32_t p = 0; p < passes && ok; ++p) {
-                    // the small products first: lo hi, hi lo, hi hi
-                    const CUtensorMap* mapa = maps + ma + (s.three && p == 0 ? kMapLo : 0);
-                    const CUtensorMap* mapb = maps + mb + (s.three && p == 1 ? kMapLo : 0);
-                    for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK, ++it) {
-                        const uint32_t st = it % kNsStages;
-                        if (it >= kNsStages &&
-                            !mbar_wait(smem_u32(&empty_bar[st]), (it / kNsStages + 1) & 1, &s_err)) {
-                            ok = false;
-                            break;
-                        }
-                        // both CTAs' bytes count on the leader's barrier
+                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+            } else {
+                ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err));
+            }
+            if (!ok) break;
+            __syncwarp();
+            const NsTask t = s_task[slot];
+            if (t.stack == kEnd) break;
+            if (t.need) {
+                if (lane == 0) ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
+                if (!__shfl_sync(0xFFFFFFFFu, ok, 0)) break;
+                fence_async_proxy();  // (other SMs' stores, by TMA)
+            }
+            __syncwarp();
+            if (rank == 1 && lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack;
+            const bool bx = t.kind >= kNsBX;
+            const int xmap = (t.step & 1) ? kMapX1 : kMapX0;
+            // this CTA's 128 rows of the first operand, its half of the second one's columns
+            const bool narrow = t.width <= kNsTileN / 2;
+            const uint32_t n_half = narrow ? kNsTileN / 4 : kNsTileN / 2;
+            const int ma = t.kind == kNsXXt ? xmap : t.kind == kNsAA ? kMapA : kMapB;
+            const int mb = (t.kind == kNsAA ? static_cast<int>(kMapA) : xmap) + (bx ? kMapN : 0) + (narrow ? kMap64 : 0);
+            const uint32_t depth = t.kind == kNsXXt ? t.n : t.m;
+            const uint32_t row = t.row * kNsTileM + rank * kNsRows;
+            const uint32_t col = t.col * 32u + rank * n_half;
+            // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
+            const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
+            for (uint32_t p = t.three ? 0 : 2; p < 3 && ok; ++p) {
+                // the small products first: lo hi, hi lo, hi hi
+                const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
+                const CUtensorMap* mapb = maps + mb + (p == 1 ? kMapLo : 0);
+                for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK) {
+                    ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&empty_bar[st]), phase, &s_err));
+                    if (!ok) break;
+                    if (elect_one()) {
                         const uint32_t bar = map_to(smem_u32(&full_bar[st]), 0);
                         const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
                         if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[st]), bytes);
-                        for (uint32_t i = 0; i < boxes_a; ++i)
-                            tma_load_pair(sa + i * kNsBoxBytes, mapa, bar, k0, row + 64 * i, t.index);
-                        for (uint32_t i = 0; i < boxes_b; ++i) {
-                            if (bx)
-                                tma_load_pair(sb + i * kNsBoxBytes, mapb, bar, col + 64 * i, k0, t.index);
-                            else
-                                tma_load_pair(sb + i * kNsBoxBytes, mapb, bar, k0, col + 64 * i, t.index);
-                        }
+                        tma_load_pair(sa, mapa, bar, k0, row, t.index);
+                        if (bx)
+                            tma_load_pair(sb, mapb, bar, 0, k0, col / 64, t.index);
+                        else
+                            tma_load_pair(sb, mapb, bar, k0, col, t.index);
+                    }
+                    ++issued;
+                    if (++st == kNsStages) {
+                        st = 0;
+                        phase ^= 1;
                     }
                 }
-                if (!ok) break;
             }
-            if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0) {
-                // copies in flight land before the CTA may end
-                for (uint32_t j = it > kNsStages ? it - kNsStages : 0; j < it; ++j)
-                    mbar_wait(smem_u32(&full_bar[j % kNsStages]), (j / kNsStages) & 1, &s_drain_err);
-            }
+            if (!ok) break;
+        }
+        if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0 && lane == 0) {
+            // copies in flight land before the CTA may end
+            for (uint32_t j = issued > kNsStages ? issued - kNsStages : 0; j < issued; ++j)
+                bar_wait(smem_u32(&full_bar[j % kNsStages]), (j / kNsStages) & 1, &s_drain_err);
         }
     } else if (warp == 1) {
-        // ---- the leader's thread issues the pair's products ----
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0;
-            for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q % kRing, buf = q & 1;
-                if (!mbar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
-                const NsTask t = s_task[slot];
-                if (t.stack == kEnd) break;
-                mbar_arrive(smem_u32(&task_empty[slot]));
-                const NsStack& s = a.stacks[t.stack];
-                const bool bx = t.kind >= kNsBX;
-                const uint32_t n = (t.width + 31u) & ~31u;
-                const uint32_t idesc = instr_desc(n, bx);
-                const uint32_t depth = t.kind == kNsXXt ? s.n : s.m;
-                const uint32_t d = tmem + buf * kNsTileN;
-                const uint32_t blocks = (depth + kNsTileK - 1) / kNsTileK;
-                // three products: the last one's first half has an accumulator of its own
-                const uint32_t from = s.three ? 2 * blocks : 0, to = from + (s.three ? blocks / 2 : 0);
-                const uint32_t steps = s.three ? 3 * blocks : blocks;
-                if (q >= 2 && !mbar_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err)) break;
+        // ---- the leader's second warp issues the pair's products ----
+        uint32_t st = 0, phase = 0;
+        for (uint32_t q = 0; rank == 0; ++q) {
+            const uint32_t slot = q % kRing, buf = q & 1;
+            bool ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err));
+            if (!ok) break;
+            const NsTask t = s_task[slot];
+            if (t.stack == kEnd) break;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&task_empty[slot]));
+            const bool bx = t.kind >= kNsBX;
+            const uint32_t idesc = instr_desc(t.width <= kNsTileN / 2 ? kNsTileN / 2 : kNsTileN, bx);
+            const uint32_t depth = t.kind == kNsXXt ? t.n : t.m;
+            const uint32_t d = tmem + buf * kNsTileN;
+            const uint32_t blocks = (depth + kNsTileK - 1) / kNsTileK;
+            // three products: the last one's first half has an accumulator of its own
+            const uint32_t from = t.three ? 2 * blocks : 0, to = from + (t.three ? blocks / 2 : 0);
+            const uint32_t steps = t.three ? 3 * blocks : blocks;
+            // K steps of 16 lie 32 bytes apart in K-major operands, sixteen rows of 128 in the other
+            const uint64_t da0 = operand_desc(smem, 16);
+            const uint64_t db0 = operand_desc(smem + 2 * kNsBoxBytes, bx ? kNsBoxBytes : 16);
+            const uint32_t db_k = bx ? 2048 >> 4 : 32 >> 4;
+            if (q >= 2)
+                ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err));
+            if (!ok) break;
+            tc_fence_after();
+            for (uint32_t j = 0; j < steps; ++j) {
+                ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&full_bar[st]), phase, &s_err));
+                if (!ok) break;
                 tc_fence_after();
-                bool ok = true;
-                for (uint32_t j = 0; j < steps; ++j, ++it) {
-                    const uint32_t st = it % kNsStages;
-                    if (!mbar_wait(smem_u32(&full_bar[st]), (it / kNsStages) & 1, &s_err)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
-                    const bool second = j >= from && j < to;
-                    const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
-                    const bool fresh = j == 0 || (second && j == from);
+                const bool second = j >= from && j < to;
+                const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
+                const bool fresh = j == 0 || (second && j == from);
+                const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
+                if (elect_one()) {
 #pragma unroll
                     for (uint32_t k = 0; k < kNsTileK / 16; ++k)
-                        mma_f16(dd, operand_desc(sa + k * 32, 16),
-                                bx ? operand_desc(sb + k * 2048, kNsBoxBytes)
-                                   : operand_desc(sb + k * 32, 16),
-                                idesc, !(fresh && k == 0));
+                        mma_f16(dd, da + k * 2, db + k * db_k, idesc, !(fresh && k == 0));
                     mma_commit(smem_u32(&empty_bar[st]));
+                    if (j + 1 == steps) mma_commit(smem_u32(&acc_full[buf]));
                 }
-                if (!ok) break;
-                mma_commit(smem_u32(&acc_full[buf]));
+                if (++st == kNsStages) {
+                    st = 0;
+                    phase ^= 1;
+                }
             }
-            if (*reinterpret_cast<volatile int*>(&s_err)) {
-                mma_commit(smem_u32(&drain_bar));
-                mbar_wait(smem_u32(&drain_bar), 0, &s_drain_err);
-            }
+            if (!ok) break;
         }
+        if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0) {
+            if (elect_one()) mma_commit(smem_u32(&drain_bar));
+            bar_wait(smem_u32(&drain_bar), 0, &s_drain_err);
+        }
+        __syncwarp();
     } else {
         // ---- eight warps turn accumulators into operands or results ----
         const uint32_t ew = warp - 2, quad = warp & 3, half = ew >> 2;
@@ -655,44 +708,50 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t uses[2] = {0, 0};               // addends waited for, per buffer
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = mbar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = bar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             const NsTask t = s_task[slot];
             const bool end = ok && t.stack == kEnd;
-            const NsStack& s = a.stacks[ok && !end ? t.stack : 0];
-            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(ok && !end ? t.stack : 0) * kMapsPerStack;
-            const bool sym = t.kind <= kNsAA, three = s.three != 0;
+            const uint32_t stack = ok && !end ? t.stack : 0;
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
+            const bool sym = t.kind <= kNsAA, three = t.three != 0;
+            Target target{};
+            if (t.kind == kNsLast) {
+                const NsStack& s = a.stacks[stack];
+                target.dst = kMuon ? s.param : s.dst;
+                target.master = s.master;
+                target.ema = s.mom + step.ema_delta;
+                target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
+                                    : static_cast<uint64_t>(t.index) * s.dst_mat;
+                target.pitch = kMuon ? s.cols : s.dst_row;
+                target.lr_wd = __fmul_rn(step.lr, s.wd);
+                target.lr_s = __fmul_rn(step.lr, s.factor);
+            }
             const uint32_t row0 = t.row * kNsTileM + rank * kNsRows, col0 = t.col * 32u;
-            const bool some = row0 < s.m;  // this CTA has rows in the tile
+            const bool some = row0 < t.m;  // this CTA has rows in the tile
             const bool addend = t.kind != kNsXXt && some;
             const bool lo = !sym || three;  // addend and result have a lo part
             // slots of one chunk: hi, lo (where it has one), then the mirror's; two chunks
             // at a time where they fit
             const uint32_t pair = sym && three ? 0u : 1u;
-            const uint32_t cols = sym ? s.m : s.n;
             const uint32_t chunks = (t.width + 63u) / 64u;
             const int in = t.step & 1;
-            const CUtensorMap* src = maps + (sym ? static_cast<int>(kMapA) : kMapX0 + in);
+            const CUtensorMap* src = maps + (sym ? kMapA : in ? kMapX1 : kMapX0);
             auto load_addend = [&](uint32_t c) {
                 const uint32_t b = c & pair, at = staging + b * 2 * kNsSlotBytes;
                 const uint32_t bar = smem_u32(&stage_bar[b]);
-                const uint32_t boxes = s.m - row0 > 64 ? 2 : 1;
-                mbar_expect_tx(bar, boxes * (lo ? 2 : 1) * kNsBoxBytes);
-                for (uint32_t i = 0; i < boxes; ++i) {
-                    tma_load(at + i * kNsBoxBytes, src, bar, col0 + c * 64, row0 + i * 64, t.index);
-                    if (lo)
-                        tma_load(at + kNsSlotBytes + i * kNsBoxBytes, src + kMapLo, bar, col0 + c * 64,
-                                 row0 + i * 64, t.index);
-                }
+                mbar_expect_tx(bar, (lo ? 2 : 1) * kNsSlotBytes);
+                tma_load(at, src, bar, col0 + c * 64, row0, t.index);
+                if (lo) tma_load(at + kNsSlotBytes, src + kMapLo, bar, col0 + c * 64, row0, t.index);
             };
             if (ok && !end && addend && first) {
-                ok = wait_done(a.done + s.first + t.index, t.need, &s_err, a.err);
+                ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
                 if (ok) {
                     fence_async_proxy();
                     load_addend(0);
                     if (pair && chunks > 1) load_addend(1);
                 }
             }
-            if (ok && !end) ok = mbar_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
+            if (ok && !end) ok = bar_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
             if (!ok) s_cfail[q & 1] = 1;
             consumers_sync<kEpi>();
             if (s_cfail[q & 1] || end) break;
@@ -709,7 +768,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                     float w[32];
                     tmem_ld32(tmem + buf * kNsTileN + kNsTileN / 2 + ((quad * 32u) << 16) + c * 64 + half * 32, w);
                     // (a depth of one stage has no second accumulator)
-                    if ((t.kind == kNsXXt ? s.n : s.m) > kNsTileK) {
+                    if ((t.kind == kNsXXt ? t.n : t.m) > kNsTileK) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] += w[j];
                     }
@@ -722,7 +781,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (!some) continue;
                 const uint32_t col = col0 + c * 64;
                 if (addend) {
-                    if (!mbar_wait(smem_u32(&stage_bar[b]), uses[b] & 1, &s_err)) bad = true;
+                    if (!bar_wait(smem_u32(&stage_bar[b]), uses[b] & 1, &s_err)) bad = true;
                     ++uses[b];
                     float x[32];
                     slot_read<false>(at, trow, half, x);
@@ -731,7 +790,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(fx, x[j], fv * v[j]);
                 } else {
-                    const float f = kNsScaleA / (s.sx * s.sx);
+                    const float f = kNsScaleA / (t.sx * t.sx);
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] *= f;
                     // the buffer's last stores have read it
@@ -744,15 +803,12 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (t.kind == kNsLast) {
                     // through shared memory as floats, so that the result is written row by row
                     // of the caller's matrix
-                    const float f = 1.0f / s.sx;
+                    const float f = 1.0f / t.sx;
                     float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
                     consumers_sync<kEpi>();  // (all have read their addend)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
                     consumers_sync<kEpi>();
-                    const uint64_t base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
-                                                : static_cast<uint64_t>(t.index) * s.dst_mat;
-                    const uint64_t pitch = kMuon ? s.cols : s.dst_row;
 #pragma unroll 1
                     for (int g = 0; g < 4; ++g) {
                         uint64_t to[8];
@@ -761,16 +817,16 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const uint32_t e = g * 8 + i;
-                            const uint32_t rr = s.transposed ? lane + 32 * (e & 3) : ew * 16 + (e >> 1);
-                            const uint32_t rc = s.transposed ? ew * 8 + (e >> 2) : lane + 32 * (e & 1);
+                            const uint32_t rr = t.transposed ? lane + 32 * (e & 3) : ew * 16 + (e >> 1);
+                            const uint32_t rc = t.transposed ? ew * 8 + (e >> 2) : lane + 32 * (e & 1);
                             const uint32_t y = row0 + rr, x = col + rc;
-                            to[i] = base + (s.transposed ? x * pitch + y : y * pitch + x);
+                            to[i] = target.base + (t.transposed ? x * target.pitch + y : y * target.pitch + x);
                             o[i] = fs[float_at(rr, rc)];
-                            if (y < s.m && x < s.n) valid |= 1u << i;
+                            if (y < t.m && x < t.n) valid |= 1u << i;
                         }
-                        put_result<kDst>(a, step, s, to, o, valid);
+                        put_result<kDst>(step, target, a.ema != 0, to, o, valid);
                     }
-                    fence_async_proxy();
+                    fence_async_shared();
                     consumers_sync<kEpi>();
                     if (first && c + 2 < chunks) load_addend(c + 2);
                     continue;
@@ -800,23 +856,18 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         }
                     }
                 }
-                fence_async_proxy();
+                fence_async_shared();
                 consumers_sync<kEpi>();
                 if (first) {
                     const CUtensorMap* dst =
-                        maps + (t.kind == kNsXXt ? static_cast<int>(kMapA)
-                                                 : t.kind == kNsAA ? static_cast<int>(kMapB) : kMapX0 + (in ^ 1));
-                    for (uint32_t i = 0; i < 2 && row0 + i * 64 < s.m; ++i) {
-                        tma_store(dst, at + i * kNsBoxBytes, col, row0 + i * 64, t.index);
+                        maps + (t.kind == kNsXXt ? kMapA : t.kind == kNsAA ? kMapB : in ? kMapX0 : kMapX1);
+                    tma_store(dst, at, col, row0, t.index);
+                    if (lo) tma_store(dst + kMapLo, at + kNsSlotBytes, col, row0, t.index);
+                    for (uint32_t i = 0; mirror && i < 2 && row0 + i * 64 < t.m; ++i) {
+                        tma_store(dst + kMap64, image + i * kNsBoxBytes, row0 + i * 64, col, t.index);
                         if (lo)
-                            tma_store(dst + kMapLo, at + kNsSlotBytes + i * kNsBoxBytes, col, row0 + i * 64,
-                                      t.index);
-                        if (mirror) {
-                            tma_store(dst, image + i * kNsBoxBytes, row0 + i * 64, col, t.index);
-                            if (lo)
-                                tma_store(dst + kMapLo, image + kNsSlotBytes + i * kNsBoxBytes, row0 + i * 64,
-                                          col, t.index);
-                        }
+                            tma_store(dst + kMapLo + kMap64, image + kNsSlotBytes + i * kNsBoxBytes,
+                                      row0 + i * 64, col, t.index);
                     }
                     bulk_commit();
                     if (addend) {
@@ -839,7 +890,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 bulk_wait_all();  // this tile's stores, before it counts as done
                 fence_async_proxy();
                 __threadfence();
-                red_release_add1(a.done + s.first + t.index);
+                red_release_add1(a.done + t.matrix);
             }
         }
     }

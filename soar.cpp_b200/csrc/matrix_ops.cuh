@@ -38,7 +38,7 @@ namespace soarb {
 constexpr int kNsMaxSteps = 16;
 constexpr float kNsScaleA = 1024.0f;  // A and B are held times this
 
-// Tile of a product: 256 rows by at most 256 columns, by a pair of CTAs (a
+// Tile of a product: 256 rows by 256 or 128 columns (fewer at a matrix's edge), by a pair of CTAs (a
 // cluster of two): each holds 128 rows of the first operand, half of the second
 // one's columns and the accumulator of its 128 rows. A pair's tile needs two
 // thirds of the operand traffic of two 128 x 256 tiles.
@@ -56,8 +56,20 @@ constexpr int kNsSlots = 4;
 constexpr size_t kNsSmemBytes =
     static_cast<size_t>(kNsStages) * kNsStageBytes + kNsSlots * kNsSlotBytes + 1024;
 
-// Tensor maps of a stack: {X hi 0, X hi 1, A hi, B hi, X lo 0, X lo 1, A lo, B lo}.
-enum NsMap { kMapX0 = 0, kMapX1 = 1, kMapA = 2, kMapB = 3, kMapLo = 4, kMapsPerStack = 8 };
+// Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
+// of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
+// ("N": boxes of 64 rows of two or one groups of 64 columns). The lo parts'
+// maps follow the hi parts'.
+enum NsMap {
+    kMapX0 = 0,        // {K128, K64, N128, N64} of the first X buffer, then of the second
+    kMapX1 = 4,
+    kMapA = 8,         // {K128, K64}
+    kMapB = 10,
+    kMapLo = 12,
+    kMapsPerStack = 24
+};
+constexpr int kMap64 = 1;  // from a K128 (N128) map to its K64 (N64) one
+constexpr int kMapN = 2;   // from X's K maps to its N maps
 
 // One stack of equal matrices.
 struct NsStack {
@@ -68,7 +80,7 @@ struct NsStack {
     __half* b;
     __half* bl;
     uint32_t m, n;        // shorter and longer side
-    uint32_t ldx, lda;
+    uint32_t ldx, lda;    // row pitches (ldx: whole groups of 64 columns)
     uint32_t rows, cols;  // as the caller has it
     uint32_t count;
     uint32_t first;       // index of its first matrix in the plan
@@ -102,15 +114,21 @@ struct PrepTile {
 enum NsKind : uint32_t { kNsXXt = 0, kNsAA = 1, kNsBX = 2, kNsLast = 3 };
 struct __align__(16) NsTask {
     uint32_t stack;
-    uint32_t index;   // matrix of the stack
-    uint32_t need;    // CTAs' tiles of this matrix that must be done before
+    uint32_t index;     // matrix of the stack
+    uint32_t matrix;    // matrix of the plan
+    uint32_t need;      // CTAs' tiles of this matrix that must be done before
     uint16_t row, col;  // first row and column, in units of 256 and 32
-    uint16_t width;   // columns
+    uint16_t width;     // columns
     uint8_t kind;
     uint8_t step;
-    uint32_t pad[2];
+    // of the stack, so that a tile needs one read
+    uint32_t m, n;
+    float sx;
+    uint8_t three, transposed;
+    uint8_t pad[2];
+    uint32_t pad2[5];
 };
-static_assert(sizeof(NsTask) == 32, "a task is two 16-byte loads");
+static_assert(sizeof(NsTask) == 64, "a task is four 16-byte loads");
 
 // A Muon step's decision, from its first kernel for the others.
 struct MatrixStep {

@@ -35,14 +35,27 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
 }
 
-// A stack of `count` row-major fp16 matrices, in boxes of 64 rows of 64.
-bool encode(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
-            uint32_t cols, uint32_t ld, uint32_t count) {
+// A stack of `count` row-major fp16 matrices, in boxes of `height` rows of 64 columns.
+bool encode_rows(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
+                 uint32_t cols, uint32_t ld, uint32_t count, uint32_t height) {
     const cuuint64_t dims[3] = {cols, rows, count};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2,
                                    static_cast<cuuint64_t>(ld) * rows * 2};
-    const cuuint32_t box[3] = {64, 64, 1}, es[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {64, height, 1}, es[3] = {1, 1, 1};
     return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// The same as groups of 64 columns, in boxes of 64 rows of `groups` groups, a
+// group after another. (Columns of the last group that are padding come with
+// it; they are columns of a product that nobody stores.)
+bool encode_groups(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
+                   uint32_t ld, uint32_t count, uint32_t groups) {
+    const cuuint64_t dims[4] = {64, rows, ld / 64, count};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(ld) * 2, 128,
+                                   static_cast<cuuint64_t>(ld) * rows * 2};
+    const cuuint32_t box[4] = {64, 64, groups, 1}, es[4] = {1, 1, 1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, box, es,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -152,7 +165,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.three = three;
         s.m = std::min(s.rows, s.cols);
         s.n = std::max(s.rows, s.cols);
-        s.ldx = static_cast<uint32_t>(up(s.n, 8));
+        s.ldx = static_cast<uint32_t>(up(s.n, 64));
         s.lda = static_cast<uint32_t>(up(s.m, 8));
         s.first = static_cast<uint32_t>(matrices);
         matrices += s.count;
@@ -211,7 +224,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
             for (uint32_t kind = kNsXXt; kind <= kNsBX; ++kind) {
                 // narrower tiles where whole ones would leave pairs of CTAs idle
                 uint32_t wide = kNsTileN;
-                for (; wide > 64; wide /= 2) {
+                for (; wide > kNsTileN / 2; wide /= 2) {
                     uint64_t all = 0;
                     for (const Run& r : wave)
                         all += product_tiles(stacks[r.stack], kind, wide).size() * (r.to - r.from);
@@ -225,7 +238,13 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                             NsTask k{};
                             k.stack = wave[w].stack;
                             k.index = i;
+                            k.matrix = s.first + i;
                             k.need = counted[w];
+                            k.m = s.m;
+                            k.n = s.n;
+                            k.sx = s.sx;
+                            k.three = static_cast<uint8_t>(s.three);
+                            k.transposed = static_cast<uint8_t>(s.transposed);
                             k.row = t.row;
                             k.col = t.col;
                             k.width = t.width;
@@ -301,14 +320,21 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.al = three ? reinterpret_cast<__half*>(at(p.al)) : s.a;
         s.bl = three ? reinterpret_cast<__half*>(at(p.bl)) : s.b;
         CUtensorMap* m = maps.data() + i * kMapsPerStack;
-        ok = ok && encode(encoder, m + kMapX0, s.x[0], s.m, s.n, s.ldx, s.count) &&
-             encode(encoder, m + kMapX1, s.x[1], s.m, s.n, s.ldx, s.count) &&
-             encode(encoder, m + kMapA, s.a, s.m, s.m, s.lda, s.count) &&
-             encode(encoder, m + kMapB, s.b, s.m, s.m, s.lda, s.count) &&
-             encode(encoder, m + kMapLo + kMapX0, s.xl[0], s.m, s.n, s.ldx, s.count) &&
-             encode(encoder, m + kMapLo + kMapX1, s.xl[1], s.m, s.n, s.ldx, s.count) &&
-             encode(encoder, m + kMapLo + kMapA, s.al, s.m, s.m, s.lda, s.count) &&
-             encode(encoder, m + kMapLo + kMapB, s.bl, s.m, s.m, s.lda, s.count);
+        for (int lo = 0; lo < 2; ++lo) {
+            CUtensorMap* q = m + (lo ? kMapLo : 0);
+            for (int k = 0; k < 2; ++k) {
+                __half* x = lo ? s.xl[k] : s.x[k];
+                CUtensorMap* qx = q + (k ? kMapX1 : kMapX0);
+                ok = ok && encode_rows(encoder, qx, x, s.m, s.n, s.ldx, s.count, 128) &&
+                     encode_rows(encoder, qx + kMap64, x, s.m, s.n, s.ldx, s.count, 64) &&
+                     encode_groups(encoder, qx + kMapN, x, s.m, s.ldx, s.count, 2) &&
+                     encode_groups(encoder, qx + kMapN + kMap64, x, s.m, s.ldx, s.count, 1);
+                __half* ab = k ? (lo ? s.bl : s.b) : (lo ? s.al : s.a);
+                CUtensorMap* qa = q + (k ? kMapB : kMapA);
+                ok = ok && encode_rows(encoder, qa, ab, s.m, s.m, s.lda, s.count, 128) &&
+                     encode_rows(encoder, qa + kMap64, ab, s.m, s.m, s.lda, s.count, 64);
+            }
+        }
     }
     auto put = [&](size_t o, const void* from, size_t bytes) {
         if (bytes) std::memcpy(host.data() + (o - operand_bytes), from, bytes);
