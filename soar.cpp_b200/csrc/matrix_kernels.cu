@@ -255,17 +255,27 @@ struct Patience {
         return false;
     }
 };
+// A converged warp's value, known to the compiler to be the same in all lanes.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xFFFFFFFFu, x); }
+
+// A converged warp's wait.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* s_err) {
+    Patience p;
+    while (!__all_sync(0xFFFFFFFFu, mbar_try(bar, parity)))
+        if (!__all_sync(0xFFFFFFFFu, p.more(s_err))) return false;
+    return true;
+}
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* s_err) {
     Patience p;
     while (!mbar_try(bar, parity))
         if (!p.more(s_err)) return false;
     return true;
 }
-// bar_wait for a barrier the other CTA arrives on.
-__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
+// warp_wait for a barrier the other CTA arrives on.
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
     Patience p;
-    while (!mbar_try_cluster(bar, parity))
-        if (!p.more(s_err)) return false;
+    while (!__all_sync(0xFFFFFFFFu, mbar_try_cluster(bar, parity)))
+        if (!__all_sync(0xFFFFFFFFu, p.more(s_err))) return false;
     return true;
 }
 __device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint4& v) {
@@ -504,12 +514,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
     constexpr int kRing = 4;  // tasks taken ahead
-    constexpr int kEpi = kNsEpilogueWarps * 32;
+    constexpr int kMath = kNsMathWarps * 32;
+    constexpr int kFirstMath = 3 * 32;
     constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t stage_bar[2], drain_bar;
+    __shared__ __align__(8) uint64_t in_full[kNsBuffers], out_full[kNsBuffers], drain_bar;
     __shared__ __align__(16) NsTask s_task[kRing];
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_drain_err, s_cfail[2];
@@ -530,12 +541,15 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 2 * kNsEpilogueWarps);  // both CTAs' warps
-            mbar_init(smem_u32(&stage_bar[i]), 1);
+            mbar_init(smem_u32(&acc_empty[i]), 2 * kNsMathWarps);  // both CTAs' warps
+        }
+        for (int i = 0; i < kNsBuffers; ++i) {
+            mbar_init(smem_u32(&in_full[i]), 1);
+            mbar_init(smem_u32(&out_full[i]), kNsMathWarps);
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            mbar_init(smem_u32(&task_empty[i]), 4);  // products, two epilogues, the other CTA's loads
+            mbar_init(smem_u32(&task_empty[i]), 6);  // products, the other CTA's copies, two epilogues' two parts
         }
         mbar_init(smem_u32(&drain_bar), 1);
         s_err = s_drain_err = s_cfail[0] = s_cfail[1] = 0;
@@ -558,6 +572,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         fence_async_proxy();  // (X of the kernel before)
         uint32_t st = 0, phase = 1;  // the next stage; its empty barrier's phase to wait for
         uint32_t issued = 0;
+        const uint32_t lead_full = uniform(map_to(smem_u32(&full_bar[0]), 0));
         // a task is read one task ahead, and its number taken two ahead
         NsTask ahead{};
         uint32_t claim = 0;
@@ -574,63 +589,65 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint32_t slot = q % kRing;
             bool ok = true;
             if (rank == 0) {
-                if (lane == 0) {
-                    if (q >= kRing) ok = bar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err);
-                    if (ok) {
-                        s_task[slot] = ahead;
-                        mbar_arrive(smem_u32(&task_full[slot]));
-                        const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
+                if (q >= kRing) ok = warp_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err);
+                if (ok && lane == 0) {
+                    s_task[slot] = ahead;
+                    mbar_arrive(smem_u32(&task_full[slot]));
+                    const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
 #pragma unroll
-                        for (int i = 0; i < 3; ++i)  // (the rest is padding)
-                            st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&ahead)[i]);
-                        mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
-                        if (ahead.stack != kEnd) read_ahead();
-                    }
+                    for (int i = 0; i < 3; ++i)  // (the rest is padding)
+                        st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&ahead)[i]);
+                    mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
+                    if (ahead.stack != kEnd) read_ahead();
                 }
-                ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                __syncwarp();
             } else {
-                ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err));
+                ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             }
             if (!ok) break;
-            __syncwarp();
-            const NsTask t = s_task[slot];
-            if (t.stack == kEnd) break;
-            if (t.need) {
-                if (lane == 0) ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
-                if (!__shfl_sync(0xFFFFFFFFu, ok, 0)) break;
+            const NsTask& t = s_task[slot];
+            const uint32_t stack = uniform(t.stack);
+            if (stack == kEnd) break;
+            const uint32_t index = uniform(t.index), kind = uniform(t.kind), three = uniform(t.three);
+            const uint32_t tm = uniform(t.m), tn = uniform(t.n), need = uniform(t.need);
+            const uint32_t odd = uniform(t.step) & 1u, width = uniform(t.width);
+            const uint32_t row = uniform(t.row) * kNsTileM + rank * kNsRows;
+            const uint32_t col0 = uniform(t.col) * 32u;
+            const uint32_t* done = a.done + t.matrix;
+            if (rank == 1 && lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+            if (need) {
+                if (lane == 0) ok = wait_done(done, need, &s_err, a.err);
+                if (!__all_sync(0xFFFFFFFFu, ok)) break;
                 fence_async_proxy();  // (other SMs' stores, by TMA)
             }
-            __syncwarp();
-            if (rank == 1 && lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
-            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack;
-            const bool bx = t.kind >= kNsBX;
-            const int xmap = (t.step & 1) ? kMapX1 : kMapX0;
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
+            const bool bx = kind >= kNsBX;
+            const uint32_t xmap = odd ? kMapX1 : kMapX0;
             // this CTA's 128 rows of the first operand, its half of the second one's columns
-            const bool narrow = t.width <= kNsTileN / 2;
+            const bool narrow = width <= kNsTileN / 2;
             const uint32_t n_half = narrow ? kNsTileN / 4 : kNsTileN / 2;
-            const int ma = t.kind == kNsXXt ? xmap : t.kind == kNsAA ? kMapA : kMapB;
-            const int mb = (t.kind == kNsAA ? static_cast<int>(kMapA) : xmap) + (bx ? kMapN : 0) + (narrow ? kMap64 : 0);
-            const uint32_t depth = t.kind == kNsXXt ? t.n : t.m;
-            const uint32_t row = t.row * kNsTileM + rank * kNsRows;
-            const uint32_t col = t.col * 32u + rank * n_half;
+            const uint32_t col = col0 + rank * n_half;
+            const uint32_t ma = kind == kNsXXt ? xmap : kind == kNsAA ? kMapA : kMapB;
+            const uint32_t mb = (kind == kNsAA ? static_cast<uint32_t>(kMapA) : xmap) + (bx ? kMapN : 0) + (narrow ? kMap64 : 0);
+            const uint32_t depth = kind == kNsXXt ? tn : tm;
             // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
             const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
-            for (uint32_t p = t.three ? 0 : 2; p < 3 && ok; ++p) {
+            for (uint32_t p = three ? 0 : 2; p < 3 && ok; ++p) {
                 // the small products first: lo hi, hi lo, hi hi
                 const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
                 const CUtensorMap* mapb = maps + mb + (p == 1 ? kMapLo : 0);
                 for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK) {
-                    ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&empty_bar[st]), phase, &s_err));
+                    ok = warp_wait(smem_u32(&empty_bar[st]), phase, &s_err);
                     if (!ok) break;
                     if (elect_one()) {
-                        const uint32_t bar = map_to(smem_u32(&full_bar[st]), 0);
+                        const uint32_t bar = lead_full + st * 8;
                         const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
                         if (rank == 0) mbar_expect_tx(smem_u32(&full_bar[st]), bytes);
-                        tma_load_pair(sa, mapa, bar, k0, row, t.index);
+                        tma_load_pair(sa, mapa, bar, k0, row, index);
                         if (bx)
-                            tma_load_pair(sb, mapb, bar, 0, k0, col / 64, t.index);
+                            tma_load_pair(sb, mapb, bar, 0, k0, col / 64, index);
                         else
-                            tma_load_pair(sb, mapb, bar, k0, col, t.index);
+                            tma_load_pair(sb, mapb, bar, k0, col, index);
                     }
                     ++issued;
                     if (++st == kNsStages) {
@@ -651,37 +668,37 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t st = 0, phase = 0;
         for (uint32_t q = 0; rank == 0; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err));
+            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
-            const NsTask t = s_task[slot];
-            if (t.stack == kEnd) break;
+            const NsTask& t = s_task[slot];
+            if (uniform(t.stack) == kEnd) break;
+            const uint32_t kind = uniform(t.kind), three = uniform(t.three), width = uniform(t.width);
+            const uint32_t depth = uniform(kind == kNsXXt ? t.n : t.m);
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&task_empty[slot]));
-            const bool bx = t.kind >= kNsBX;
-            const uint32_t idesc = instr_desc(t.width <= kNsTileN / 2 ? kNsTileN / 2 : kNsTileN, bx);
-            const uint32_t depth = t.kind == kNsXXt ? t.n : t.m;
-            const uint32_t d = tmem + buf * kNsTileN;
+            const bool bx = kind >= kNsBX;
+            const uint32_t idesc = instr_desc(width <= kNsTileN / 2 ? kNsTileN / 2 : kNsTileN, bx);
+            const uint32_t d = uniform(tmem) + buf * kNsTileN;
             const uint32_t blocks = (depth + kNsTileK - 1) / kNsTileK;
             // three products: the last one's first half has an accumulator of its own
-            const uint32_t from = t.three ? 2 * blocks : 0, to = from + (t.three ? blocks / 2 : 0);
-            const uint32_t steps = t.three ? 3 * blocks : blocks;
+            const uint32_t from = three ? 2 * blocks : 0, to = from + (three ? blocks / 2 : 0);
+            const uint32_t steps = three ? 3 * blocks : blocks;
             // K steps of 16 lie 32 bytes apart in K-major operands, sixteen rows of 128 in the other
             const uint64_t da0 = operand_desc(smem, 16);
             const uint64_t db0 = operand_desc(smem + 2 * kNsBoxBytes, bx ? kNsBoxBytes : 16);
             const uint32_t db_k = bx ? 2048 >> 4 : 32 >> 4;
-            if (q >= 2)
-                ok = __all_sync(0xFFFFFFFFu, bar_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err));
+            if (q >= 2) ok = warp_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err);
             if (!ok) break;
             tc_fence_after();
             for (uint32_t j = 0; j < steps; ++j) {
-                ok = __all_sync(0xFFFFFFFFu, bar_wait(smem_u32(&full_bar[st]), phase, &s_err));
+                ok = warp_wait(smem_u32(&full_bar[st]), phase, &s_err);
                 if (!ok) break;
                 tc_fence_after();
-                const bool second = j >= from && j < to;
-                const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
-                const bool fresh = j == 0 || (second && j == from);
-                const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
                 if (elect_one()) {
+                    const bool second = j >= from && j < to;
+                    const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
+                    const bool fresh = j == 0 || (second && j == from);
+                    const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
 #pragma unroll
                     for (uint32_t k = 0; k < kNsTileK / 16; ++k)
                         mma_f16(dd, da + k * 2, db + k * db_k, idesc, !(fresh && k == 0));
@@ -701,196 +718,262 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         }
         __syncwarp();
     } else {
-        // ---- eight warps turn accumulators into operands or results ----
-        const uint32_t ew = warp - 2, quad = warp & 3, half = ew >> 2;
-        const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
-        const bool first = threadIdx.x == 64;    // issues the epilogue's copies
-        uint32_t uses[2] = {0, 0};               // addends waited for, per buffer
-        for (uint32_t q = 0;; ++q) {
-            const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = bar_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
-            const NsTask t = s_task[slot];
-            const bool end = ok && t.stack == kEnd;
-            const uint32_t stack = ok && !end ? t.stack : 0;
-            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
-            const bool sym = t.kind <= kNsAA, three = t.three != 0;
-            Target target{};
-            if (t.kind == kNsLast) {
-                const NsStack& s = a.stacks[stack];
-                target.dst = kMuon ? s.param : s.dst;
-                target.master = s.master;
-                target.ema = s.mom + step.ema_delta;
-                target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
-                                    : static_cast<uint64_t>(t.index) * s.dst_mat;
-                target.pitch = kMuon ? s.cols : s.dst_row;
-                target.lr_wd = __fmul_rn(step.lr, s.wd);
-                target.lr_s = __fmul_rn(step.lr, s.factor);
-            }
-            const uint32_t row0 = t.row * kNsTileM + rank * kNsRows, col0 = t.col * 32u;
-            const bool some = row0 < t.m;  // this CTA has rows in the tile
-            const bool addend = t.kind != kNsXXt && some;
-            const bool lo = !sym || three;  // addend and result have a lo part
-            // slots of one chunk: hi, lo (where it has one), then the mirror's; two chunks
-            // at a time where they fit
-            const uint32_t pair = sym && three ? 0u : 1u;
-            const uint32_t chunks = (t.width + 63u) / 64u;
-            const int in = t.step & 1;
-            const CUtensorMap* src = maps + (sym ? kMapA : in ? kMapX1 : kMapX0);
-            auto load_addend = [&](uint32_t c) {
-                const uint32_t b = c & pair, at = staging + b * 2 * kNsSlotBytes;
-                const uint32_t bar = smem_u32(&stage_bar[b]);
-                mbar_expect_tx(bar, (lo ? 2 : 1) * kNsSlotBytes);
-                tma_load(at, src, bar, col0 + c * 64, row0, t.index);
-                if (lo) tma_load(at + kNsSlotBytes, src + kMapLo, bar, col0 + c * 64, row0, t.index);
-            };
-            if (ok && !end && addend && first) {
-                ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
-                if (ok) {
-                    fence_async_proxy();
-                    load_addend(0);
-                    if (pair && chunks > 1) load_addend(1);
-                }
-            }
-            if (ok && !end) ok = bar_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
-            if (!ok) s_cfail[q & 1] = 1;
-            consumers_sync<kEpi>();
-            if (s_cfail[q & 1] || end) break;
-            if (first) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
-            tc_fence_after();
-            const float ca = a.coef[t.step][0], cb = a.coef[t.step][1], cc = a.coef[t.step][2];
-            bool bad = false;
-            for (uint32_t c = 0; c < chunks; ++c) {
-                const uint32_t b = c & pair, at = staging + b * 2 * kNsSlotBytes;
-                float v[32];
+        // ---- the epilogue, in units of a buffer: a chunk of 64 columns, or (three
+        // products of a symmetric matrix) a chunk and then its mirror image ----
+        struct Unit {
+            uint32_t row0, col0;
+            bool sym, three, lo, some, addend, mirror;
+            uint32_t chunks, per, units;
+        };
+        auto units_of = [&](const NsTask& t) {
+            Unit u;
+            u.row0 = t.row * kNsTileM + rank * kNsRows;
+            u.col0 = t.col * 32u;
+            u.sym = t.kind <= kNsAA;
+            u.three = t.three != 0;
+            u.lo = !u.sym || u.three;       // operand and result have a lo part
+            u.some = u.row0 < t.m;          // this CTA has rows in the tile
+            u.addend = t.kind != kNsXXt;
+            u.mirror = u.sym && u.col0 >= (t.row + 1u) * kNsTileM;  // right of the diagonal's block
+            u.chunks = (t.width + 63u) / 64u;
+            u.per = u.three && u.mirror ? 2 : 1;
+            u.units = u.some ? u.chunks * u.per : 0;
+            return u;
+        };
+        uint32_t g = 0;  // units before this tile
+        if (warp == 2) {
+            // ---- copies: what a unit adds to in, what it makes out ----
+            fence_async_proxy();
+            bool early = false;  // the next tile's first units are on their way
+            for (uint32_t q = 0;; ++q) {
+                const uint32_t slot = q % kRing;
+                bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+                if (!ok) break;
+                const NsTask t = s_task[slot];
+                if (t.stack == kEnd) break;
                 __syncwarp();
-                tmem_ld32(tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32, v);
-                if (three) {
-                    float w[32];
-                    tmem_ld32(tmem + buf * kNsTileN + kNsTileN / 2 + ((quad * 32u) << 16) + c * 64 + half * 32, w);
-                    // (a depth of one stage has no second accumulator)
-                    if ((t.kind == kNsXXt ? t.n : t.m) > kNsTileK) {
+                if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+                const Unit u = units_of(t);
+                auto bring = [&](const NsTask& w, const Unit& v, uint32_t base, uint32_t i) {
+                    const uint32_t b = (base + i) % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
+                    const uint32_t bar = smem_u32(&in_full[b]);
+                    if (!v.addend || (v.per == 2 && (i & 1))) {
+                        mbar_arrive(bar);
+                        return;
+                    }
+                    const CUtensorMap* src = a.maps + static_cast<uint64_t>(w.stack) * kMapsPerStack +
+                                             (v.sym ? kMapA : w.step & 1 ? kMapX1 : kMapX0);
+                    const uint32_t x = v.col0 + (v.per == 2 ? i >> 1 : i) * 64;
+                    mbar_expect_tx(bar, (v.lo ? 2 : 1) * kNsSlotBytes);
+                    tma_load(at, src, bar, x, v.row0, w.index);
+                    if (v.lo) tma_load(at + kNsSlotBytes, src + kMapLo, bar, x, v.row0, w.index);
+                };
+                if (u.units && !early) {
+                    if (u.addend) {
+                        if (lane == 0) ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
+                        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+                        fence_async_proxy();
+                    }
+                    if (elect_one()) {
+                        bring(t, u, g, 0);
+                        if (u.units > 1) bring(t, u, g, 1);
+                    }
+                }
+                early = false;
+                const bool last = t.kind == kNsLast;
+                const CUtensorMap* dst =
+                    a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
+                    (t.kind == kNsXXt ? kMapA : t.kind == kNsAA ? kMapB : t.step & 1 ? kMapX0 : kMapX1);
+                for (uint32_t i = 0; i < u.units; ++i) {
+                    const uint32_t b = (g + i) % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
+                    ok = warp_wait(smem_u32(&out_full[b]), ((g + i) / kNsBuffers) & 1, &s_err);
+                    if (!ok) break;
+                    if (elect_one()) {
+                        const uint32_t x = u.col0 + (u.per == 2 ? i >> 1 : i) * 64;
+                        const bool image_only = u.per == 2 && (i & 1);
+                        if (!last) {
+                            if (!image_only) {
+                                tma_store(dst, at, x, u.row0, t.index);
+                                if (u.lo) tma_store(dst + kMapLo, at + kNsSlotBytes, x, u.row0, t.index);
+                            }
+                            if (u.mirror && (image_only || !u.three)) {
+                                const uint32_t image = at + (image_only ? 0 : kNsSlotBytes);
+                                for (uint32_t h = 0; h < 2 && u.row0 + h * 64 < t.m; ++h) {
+                                    tma_store(dst + kMap64, image + h * kNsBoxBytes, u.row0 + h * 64, x, t.index);
+                                    if (image_only)
+                                        tma_store(dst + kMapLo + kMap64, at + kNsSlotBytes + h * kNsBoxBytes,
+                                                  u.row0 + h * 64, x, t.index);
+                                }
+                            }
+                            bulk_commit();
+                        }
+                        if (i + 2 < u.units) {
+                            if (!last) bulk_wait_read<1>();  // the unit before has left its buffer
+                            bring(t, u, g, i + 2);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                g += u.units;
+                // the next tile's first units, if their input is there already
+                const uint32_t next = (q + 1) % kRing;
+                if (__all_sync(0xFFFFFFFFu, mbar_try_cluster(smem_u32(&task_full[next]), ((q + 1) / kRing) & 1))) {
+                    const NsTask w = s_task[next];
+                    if (w.stack != kEnd) {
+                        const Unit v = units_of(w);
+                        if (v.units && (!v.addend || __all_sync(0xFFFFFFFFu, ld_acquire(a.done + w.matrix) >= w.need))) {
+                            fence_async_proxy();
+                            early = true;
+                            if (elect_one()) {
+                                bulk_wait_read<1>();
+                                bring(w, v, g, 0);
+                                if (v.units > 1) bring(w, v, g, 1);
+                            }
+                        }
+                    }
+                }
+                if (u.units && !last && elect_one()) {
+                    bulk_wait_all();  // this tile's stores, before it counts as done
+                    fence_async_proxy();
+                    __threadfence();
+                    red_release_add1(a.done + t.matrix);
+                }
+                __syncwarp();
+            }
+        } else {
+            // ---- arithmetic: eight warps, each 32 rows of 32 columns of a chunk ----
+            const uint32_t mw = warp - 3, quad = warp & 3, half = mw >> 2;
+            const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
+            for (uint32_t q = 0;; ++q) {
+                const uint32_t slot = q % kRing, buf = q & 1;
+                bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+                const NsTask t = s_task[slot];
+                const bool end = ok && t.stack == kEnd;
+                const Unit u = units_of(t);
+                Target target{};
+                if (ok && !end) {
+                    if (t.kind == kNsLast) {
+                        const NsStack& s = a.stacks[t.stack];
+                        target.dst = kMuon ? s.param : s.dst;
+                        target.master = s.master;
+                        target.ema = s.mom + step.ema_delta;
+                        target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
+                                            : static_cast<uint64_t>(t.index) * s.dst_mat;
+                        target.pitch = kMuon ? s.cols : s.dst_row;
+                        target.lr_wd = __fmul_rn(step.lr, s.wd);
+                        target.lr_s = __fmul_rn(step.lr, s.factor);
+                    }
+                    ok = warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
+                }
+                if (!ok) s_cfail[q & 1] = 1;
+                consumers_sync<kMath>();  // all go on, or none
+                if (s_cfail[q & 1] || end) break;
+                if (threadIdx.x == kFirstMath) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+                tc_fence_after();
+                const float ca = a.coef[t.step][0], cb = a.coef[t.step][1], cc = a.coef[t.step][2];
+                const bool two = u.three && (t.kind == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
+                // v = fx addend + fv accumulator
+                const float fx = u.sym ? cb : ca;
+                const float fv = t.kind == kNsXXt ? kNsScaleA / (t.sx * t.sx)
+                                                  : t.kind == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
+                for (uint32_t c = 0; c < u.chunks; ++c) {
+                    const uint32_t i = g + c * u.per, b = i % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
+                    float v[32];
+                    const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32;
+                    __syncwarp();
+                    tmem_ld32(acc, v);
+                    if (two) {
+                        float w[32];
+                        tmem_ld32(acc + kNsTileN / 2, w);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] += w[j];
                     }
-                }
-                if (c + 1 == chunks) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
-                }
-                if (!some) continue;
-                const uint32_t col = col0 + c * 64;
-                if (addend) {
-                    if (!bar_wait(smem_u32(&stage_bar[b]), uses[b] & 1, &s_err)) bad = true;
-                    ++uses[b];
-                    float x[32];
-                    slot_read<false>(at, trow, half, x);
-                    if (lo) slot_read<true>(at + kNsSlotBytes, trow, half, x);
-                    const float fx = sym ? cb : ca, fv = sym ? cc / kNsScaleA : 1.0f / kNsScaleA;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(fx, x[j], fv * v[j]);
-                } else {
-                    const float f = kNsScaleA / (t.sx * t.sx);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] *= f;
-                    // the buffer's last stores have read it
-                    if (first) {
-                        if (pair && c > 0) bulk_wait_read<1>();
-                        else bulk_wait_read<0>();
+                    if (c + 1 == u.chunks) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
                     }
-                    consumers_sync<kEpi>();
-                }
-                if (t.kind == kNsLast) {
-                    // through shared memory as floats, so that the result is written row by row
-                    // of the caller's matrix
-                    const float f = 1.0f / t.sx;
-                    float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
-                    consumers_sync<kEpi>();  // (all have read their addend)
+                    if (!u.some) continue;
+                    const uint32_t col = u.col0 + c * 64;
+                    // (a wait that runs out has set s_err: the next tile ends the loop)
+                    warp_wait(smem_u32(&in_full[b]), (i / kNsBuffers) & 1, &s_err);
+                    if (u.addend) {
+                        float x[32];
+                        slot_read<false>(at, trow, half, x);
+                        if (u.lo) slot_read<true>(at + kNsSlotBytes, trow, half, x);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
-                    consumers_sync<kEpi>();
+                        for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(fx, x[j], fv * v[j]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] *= fv;
+                    }
+                    if (t.kind == kNsLast) {
+                        // through shared memory as floats, so that the result is written row by
+                        // row of the caller's matrix
+                        const float f = 1.0f / t.sx;
+                        float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
+                        consumers_sync<kMath>();  // (all have read their addend)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
+                        consumers_sync<kMath>();
 #pragma unroll 1
-                    for (int g = 0; g < 4; ++g) {
-                        uint64_t to[8];
-                        float o[8];
-                        uint32_t valid = 0;
+                        for (int k = 0; k < 4; ++k) {
+                            uint64_t to[8];
+                            float o[8];
+                            uint32_t valid = 0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t e = g * 8 + i;
-                            const uint32_t rr = t.transposed ? lane + 32 * (e & 3) : ew * 16 + (e >> 1);
-                            const uint32_t rc = t.transposed ? ew * 8 + (e >> 2) : lane + 32 * (e & 1);
-                            const uint32_t y = row0 + rr, x = col + rc;
-                            to[i] = target.base + (t.transposed ? x * target.pitch + y : y * target.pitch + x);
-                            o[i] = fs[float_at(rr, rc)];
-                            if (y < t.m && x < t.n) valid |= 1u << i;
+                            for (int l = 0; l < 8; ++l) {
+                                const uint32_t e = k * 8 + l;
+                                const uint32_t rr = t.transposed ? lane + 32 * (e & 3) : mw * 16 + (e >> 1);
+                                const uint32_t rc = t.transposed ? mw * 8 + (e >> 2) : lane + 32 * (e & 1);
+                                const uint32_t y = u.row0 + rr, x = col + rc;
+                                to[l] = target.base + (t.transposed ? x * target.pitch + y : y * target.pitch + x);
+                                o[l] = fs[float_at(rr, rc)];
+                                if (y < t.m && x < t.n) valid |= 1u << l;
+                            }
+                            put_result<kDst>(step, target, a.ema != 0, to, o, valid);
                         }
-                        put_result<kDst>(step, target, a.ema != 0, to, o, valid);
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&out_full[b]));
+                        continue;
+                    }
+                    // hi and lo in place of the addend; the mirror image in the second slot, or
+                    // in the next buffer
+                    const uint32_t b1 = (i + 1) % kNsBuffers;
+                    const uint32_t image = u.per == 2 ? staging + b1 * 2 * kNsSlotBytes : at + kNsSlotBytes;
+                    if (u.per == 2) warp_wait(smem_u32(&in_full[b1]), ((i + 1) / kNsBuffers) & 1, &s_err);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t h[4], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
+                        const uint32_t o = slot_at(trow, half * 4 + j);
+                        sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
+                        if (u.lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
+                        if (u.mirror) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
+                                const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
+                                sts16(image + m0, h[e] & 0xFFFFu);
+                                sts16(image + m1, h[e] >> 16);
+                                if (u.lo) {
+                                    sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
+                                    sts16(image + kNsSlotBytes + m1, l[e] >> 16);
+                                }
+                            }
+                        }
                     }
                     fence_async_shared();
-                    consumers_sync<kEpi>();
-                    if (first && c + 2 < chunks) load_addend(c + 2);
-                    continue;
-                }
-                // hi and lo in place of the addend, and the mirror image beside them
-                const bool mirror = sym && col >= (t.row + 1u) * kNsTileM;
-                const uint32_t image = at + (lo ? 2 : 1) * kNsSlotBytes;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t h[4], l[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
-                    const uint32_t o = slot_at(trow, half * 4 + j);
-                    sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
-                    if (lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
-                    if (mirror) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
-                            const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
-                            sts16(image + m0, h[e] & 0xFFFFu);
-                            sts16(image + m1, h[e] >> 16);
-                            if (lo) {
-                                sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
-                                sts16(image + kNsSlotBytes + m1, l[e] >> 16);
-                            }
-                        }
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&out_full[b]));
+                        if (u.per == 2) mbar_arrive(smem_u32(&out_full[b1]));
                     }
                 }
-                fence_async_shared();
-                consumers_sync<kEpi>();
-                if (first) {
-                    const CUtensorMap* dst =
-                        maps + (t.kind == kNsXXt ? kMapA : t.kind == kNsAA ? kMapB : in ? kMapX0 : kMapX1);
-                    tma_store(dst, at, col, row0, t.index);
-                    if (lo) tma_store(dst + kMapLo, at + kNsSlotBytes, col, row0, t.index);
-                    for (uint32_t i = 0; mirror && i < 2 && row0 + i * 64 < t.m; ++i) {
-                        tma_store(dst + kMap64, image + i * kNsBoxBytes, row0 + i * 64, col, t.index);
-                        if (lo)
-                            tma_store(dst + kMapLo + kMap64, image + kNsSlotBytes + i * kNsBoxBytes,
-                                      row0 + i * 64, col, t.index);
-                    }
-                    bulk_commit();
-                    if (addend) {
-                        // the next chunk but one of a pair of buffers (the next of one): its
-                        // buffer's stores have read it
-                        if (!pair) {
-                            if (c + 1 < chunks) {
-                                bulk_wait_read<0>();
-                                load_addend(c + 1);
-                            }
-                        } else if (c >= 1 && c + 1 < chunks) {
-                            bulk_wait_read<1>();
-                            load_addend(c + 1);
-                        }
-                    }
-                }
-            }
-            if (bad) s_cfail[(q + 1) & 1] = 1;  // (read after the next tile's first barrier)
-            if (first) {
-                bulk_wait_all();  // this tile's stores, before it counts as done
-                fence_async_proxy();
-                __threadfence();
-                red_release_add1(a.done + t.matrix);
+                g += u.units;
             }
         }
     }

@@ -46,15 +46,15 @@ constexpr int kNsTileM = 256;
 constexpr int kNsTileN = 256;
 constexpr int kNsRows = 128;   // a CTA's share of the rows
 constexpr int kNsTileK = 64;   // depth of one stage
-constexpr int kNsStages = 5;
-constexpr int kNsEpilogueWarps = 8;
-constexpr int kNsThreads = (2 + kNsEpilogueWarps) * 32;  // TMA warp, MMA warp, epilogue
+constexpr int kNsStages = 4;
+constexpr int kNsMathWarps = 8;
+constexpr int kNsThreads = (3 + kNsMathWarps) * 32;  // operand copies, products, epilogue copies, epilogue
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
 constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
-constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue staging: 128 rows of 64 fp16
-constexpr int kNsSlots = 4;
+constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue: 128 rows of 64 fp16
+constexpr int kNsBuffers = 3;                       // epilogue buffers of two slots
 constexpr size_t kNsSmemBytes =
-    static_cast<size_t>(kNsStages) * kNsStageBytes + kNsSlots * kNsSlotBytes + 1024;
+    static_cast<size_t>(kNsStages) * kNsStageBytes + 2 * kNsBuffers * kNsSlotBytes + 1024;
 
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
@@ -149,7 +149,7 @@ struct MatrixArgs {
     double* partials;      // one per preparation tile
     uint32_t* tickets;     // per matrix: preparation tiles summed (0 between launches)
     float* inv;            // per matrix: sx / (norm + eps)
-    uint32_t* done;        // per matrix: product tiles done, counted by each CTA of a pair
+    uint32_t* done;        // per matrix: product tiles done, counted by each CTA with rows in one
     uint32_t* next;        // tasks handed out
     MatrixStep* step;
     int* err;              // nonzero: a wait ran out

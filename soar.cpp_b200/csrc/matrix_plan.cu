@@ -209,9 +209,12 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     }
 
     // The tasks, in an order in which every tile's inputs come before it: lists
-    // of matrices whose operands fit in the L2 cache together go through their
-    // products side by side, one such list after another.
-    constexpr uint64_t kWaveBytes = 48ull << 20;
+    // ("waves") of matrices go through their products side by side, one list
+    // after another. A list is long enough that a product of it occupies every
+    // pair of CTAs twice (or the tiles of its next product wait), and else as
+    // short as half of the L2 cache, which then holds its operands.
+    constexpr uint64_t kWaveBytes = 64ull << 20;
+    const uint64_t wave_tiles = static_cast<uint64_t>(plan->sms);
     std::vector<NsTask> tasks;
     struct Run {
         uint32_t stack, from, to;
@@ -253,30 +256,34 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                             k.step = static_cast<uint8_t>(step);
                             tasks.push_back(k);
                         }
-                    counted[w] += 2 * static_cast<uint32_t>(tiles.size());
+                    // (a CTA without rows in a tile does not count it)
+                    for (const Tile& t : tiles)
+                        counted[w] += s.m - t.row * kNsTileM > kNsRows ? 2 : 1;
                 }
             }
         }
         wave.clear();
         wave_bytes = 0;
     };
+    uint64_t tiles_in_wave = 0;
     for (uint32_t si = 0; si < stacks.size(); ++si) {
         const NsStack& s = stacks[si];
         const uint64_t each = 2ull * s.m * (4ull * s.ldx + (three ? 4ull : 2ull) * s.lda);
-        uint32_t i = 0;
-        while (i < s.count) {
-            const uint64_t room = wave_bytes < kWaveBytes ? (kWaveBytes - wave_bytes) / each : 0;
-            uint32_t k = static_cast<uint32_t>(std::min<uint64_t>(room, s.count - i));
-            if (k == 0) {
-                if (!wave.empty()) {
-                    flush();
-                    continue;
-                }
-                k = 1;
-            }
-            wave.push_back({si, i, i + k});
+        const uint64_t tiles = product_tiles(s, kNsXXt, kNsTileN).size();
+        for (uint32_t i = 0; i < s.count;) {
+            // as many as the wave still takes: until it has both the bytes and the tiles
+            uint64_t k = 1;
+            if (wave_bytes < kWaveBytes) k = std::max(k, (kWaveBytes - wave_bytes) / each);
+            if (tiles_in_wave < wave_tiles) k = std::max(k, (wave_tiles - tiles_in_wave) / tiles);
+            k = std::min<uint64_t>(k, s.count - i);
+            wave.push_back({si, i, i + static_cast<uint32_t>(k)});
             wave_bytes += each * k;
-            i += k;
+            tiles_in_wave += tiles * k;
+            i += static_cast<uint32_t>(k);
+            if (wave_bytes >= kWaveBytes && tiles_in_wave >= wave_tiles) {
+                flush();
+                tiles_in_wave = 0;
+            }
         }
     }
     flush();
