@@ -14,9 +14,9 @@
 //                   that waits, waits only for tiles that running CTAs hold,
 //                   whatever else runs on the GPU.
 //                   One warp loads operand tiles by TMA, one thread issues
-//                   tcgen05.mma into one of two TMEM accumulators, four warps
+//                   tcgen05.mma into one of two TMEM accumulators, eight warps
 //                   turn finished accumulators into the next operand: A, B =
-//                   bA + cAA, X = aX + BX, or the result (for Muon: the
+//                   aI + bA + cAA, X = BX, or the result (for Muon: the
 //                   weights' update). A and B are symmetric: only tiles on or
 //                   above the diagonal are computed, and each is stored twice.
 #include <algorithm>
@@ -271,7 +271,13 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* s_e
         if (!p.more(s_err)) return false;
     return true;
 }
-// warp_wait for a barrier the other CTA arrives on.
+// The same for a barrier the other CTA arrives on.
+__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
+    Patience p;
+    while (!mbar_try_cluster(bar, parity))
+        if (!p.more(s_err)) return false;
+    return true;
+}
 __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
     Patience p;
     while (!__all_sync(0xFFFFFFFFu, mbar_try_cluster(bar, parity)))
@@ -433,18 +439,17 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
 
-// x[32] += (or =) the thread's 32 columns of its row.
-template <bool kAdd>
-__device__ __forceinline__ void slot_read(uint32_t slot, uint32_t row, uint32_t half, float (&x)[32]) {
+// v += f times the thread's 32 columns of its row.
+__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, uint32_t half, float f, float (&v)[32]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const uint4 q = lds128(slot + slot_at(row, half * 4 + j));
         const __half2* h = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float2 f = __half22float2(h[e]);
-            x[j * 8 + 2 * e] = kAdd ? x[j * 8 + 2 * e] + f.x : f.x;
-            x[j * 8 + 2 * e + 1] = kAdd ? x[j * 8 + 2 * e + 1] + f.y : f.y;
+            const float2 x = __half22float2(h[e]);
+            v[j * 8 + 2 * e] = __fmaf_rn(f, x.x, v[j * 8 + 2 * e]);
+            v[j * 8 + 2 * e + 1] = __fmaf_rn(f, x.y, v[j * 8 + 2 * e + 1]);
         }
     }
 }
@@ -513,14 +518,15 @@ template <int kDst>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
-    constexpr int kRing = 4;  // tasks taken ahead
+    constexpr int kRing = 4;  // tasks handed out ahead
     constexpr int kMath = kNsMathWarps * 32;
-    constexpr int kFirstMath = 3 * 32;
+    constexpr int kMathWarp = 5;            // the first of them
     constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t in_full[kNsBuffers], out_full[kNsBuffers], drain_bar;
+    __shared__ __align__(8) uint64_t in_full[kNsIn], in_empty[kNsIn], out_full[kNsOut], out_empty[kNsOut];
+    __shared__ __align__(8) uint64_t drain_bar;
     __shared__ __align__(16) NsTask s_task[kRing];
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_drain_err, s_cfail[2];
@@ -533,7 +539,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     }
     const uint32_t rank = blockIdx.x & 1u;  // 0 leads the pair: hands out tasks, issues products
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t staging = smem + kNsStages * kNsStageBytes;
+    const uint32_t in_slots = smem + kNsStages * kNsStageBytes;
+    const uint32_t out_slots = in_slots + kNsIn * kNsSlotBytes;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNsStages; ++i) {
             mbar_init(smem_u32(&full_bar[i]), 1);
@@ -543,13 +550,17 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             mbar_init(smem_u32(&acc_full[i]), 1);
             mbar_init(smem_u32(&acc_empty[i]), 2 * kNsMathWarps);  // both CTAs' warps
         }
-        for (int i = 0; i < kNsBuffers; ++i) {
+        for (int i = 0; i < kNsIn; ++i) {
             mbar_init(smem_u32(&in_full[i]), 1);
+            mbar_init(smem_u32(&in_empty[i]), kNsMathWarps);
+        }
+        for (int i = 0; i < kNsOut; ++i) {
             mbar_init(smem_u32(&out_full[i]), kNsMathWarps);
+            mbar_init(smem_u32(&out_empty[i]), 1);
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            mbar_init(smem_u32(&task_empty[i]), 6);  // products, the other CTA's copies, two epilogues' two parts
+            mbar_init(smem_u32(&task_empty[i]), 9);  // five readers here, four in the other CTA
         }
         mbar_init(smem_u32(&drain_bar), 1);
         s_err = s_drain_err = s_cfail[0] = s_cfail[1] = 0;
@@ -566,69 +577,62 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     cluster_sync();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    // A reader of the tasks is done with slot q (one lane).
+    auto release_task = [&](uint32_t slot) {
+        mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+    };
+
+    // What the epilogue does with a tile: chunks of 64 columns, `ins` slots to add to each and
+    // `outs` buffers made of each.
+    struct Tile {
+        uint32_t row0, col0, chunks, ins, outs;
+        bool sym, three, lo, some, mirror;
+    };
+    auto tile_of = [&](const NsTask& t) {
+        Tile u;
+        u.row0 = t.row() + rank * kNsRows;
+        u.col0 = t.col();
+        u.chunks = (t.width() + 63u) / 64u;
+        u.sym = t.kind() <= kNsAA;
+        u.three = t.three();
+        u.lo = !u.sym || u.three;                   // made of hi and lo
+        u.some = u.row0 < t.m;                      // this CTA has rows in the tile
+        u.mirror = u.sym && u.col0 >= t.row() + kNsTileM;  // right of the diagonal's block
+        // A (and its lo), or X's lo where the product takes hi alone
+        u.ins = t.kind() == kNsXXt ? 0 : u.sym ? (u.three ? 2 : 1) : (u.three ? 0 : 1);
+        u.outs = u.three && u.mirror ? 2 : 1;
+        return u;
+    };
 
     if (warp == 0) {
-        // ---- takes tasks, waits for their inputs, loads operand tiles ----
-        fence_async_proxy();  // (X of the kernel before)
+        // ---- loads operand tiles ----
         uint32_t st = 0, phase = 1;  // the next stage; its empty barrier's phase to wait for
         uint32_t issued = 0;
         const uint32_t lead_full = uniform(map_to(smem_u32(&full_bar[0]), 0));
-        // a task is read one task ahead, and its number taken two ahead
-        NsTask ahead{};
-        uint32_t claim = 0;
-        auto read_ahead = [&]() {
-            if (claim < a.n_tasks) ahead = a.tasks[claim];
-            else ahead.stack = kEnd;
-            claim = atomicAdd(a.next, 1u);
-        };
-        if (rank == 0 && lane == 0) {
-            claim = atomicAdd(a.next, 1u);
-            read_ahead();
-        }
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
-            bool ok = true;
-            if (rank == 0) {
-                if (q >= kRing) ok = warp_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err);
-                if (ok && lane == 0) {
-                    s_task[slot] = ahead;
-                    mbar_arrive(smem_u32(&task_full[slot]));
-                    const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i)  // (the rest is padding)
-                        st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&ahead)[i]);
-                    mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
-                    if (ahead.stack != kEnd) read_ahead();
-                }
-                __syncwarp();
-            } else {
-                ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
-            }
+            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
-            const NsTask& t = s_task[slot];
-            const uint32_t stack = uniform(t.stack);
+            const uint32_t stack = uniform(s_task[slot].stack);
             if (stack == kEnd) break;
-            const uint32_t index = uniform(t.index), kind = uniform(t.kind), three = uniform(t.three);
-            const uint32_t tm = uniform(t.m), tn = uniform(t.n), need = uniform(t.need);
-            const uint32_t odd = uniform(t.step) & 1u, width = uniform(t.width);
-            const uint32_t row = uniform(t.row) * kNsTileM + rank * kNsRows;
-            const uint32_t col0 = uniform(t.col) * 32u;
-            const uint32_t* done = a.done + t.matrix;
-            if (rank == 1 && lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
-            if (need) {
-                if (lane == 0) ok = wait_done(done, need, &s_err, a.err);
-                if (!__all_sync(0xFFFFFFFFu, ok)) break;
-                fence_async_proxy();  // (other SMs' stores, by TMA)
-            }
+            const uint32_t index = uniform(s_task[slot].index), place = uniform(s_task[slot].place);
+            const uint32_t shape = uniform(s_task[slot].shape);
+            const uint32_t tm = uniform(s_task[slot].m), tn = uniform(s_task[slot].n);
+            __syncwarp();
+            if (lane == 0) release_task(slot);
+            fence_async_proxy();  // (other SMs' stores, by TMA)
+            const uint32_t width = shape & 0xFFFFu, kind = shape >> 16 & 15u, three = shape >> 20 & 1u;
             const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
             const bool bx = kind >= kNsBX;
-            const uint32_t xmap = odd ? kMapX1 : kMapX0;
+            const uint32_t xmap = shape >> 24 & 1u ? kMapX1 : kMapX0;
             // this CTA's 128 rows of the first operand, its half of the second one's columns
             const bool narrow = width <= kNsTileN / 2;
             const uint32_t n_half = narrow ? kNsTileN / 4 : kNsTileN / 2;
-            const uint32_t col = col0 + rank * n_half;
+            const uint32_t row = (place & 0xFFFFu) * kNsTileM + rank * kNsRows;
+            const uint32_t col = (place >> 16) * 32u + rank * n_half;
             const uint32_t ma = kind == kNsXXt ? xmap : kind == kNsAA ? kMapA : kMapB;
-            const uint32_t mb = (kind == kNsAA ? static_cast<uint32_t>(kMapA) : xmap) + (bx ? kMapN : 0) + (narrow ? kMap64 : 0);
+            const uint32_t mb = (kind == kNsAA ? static_cast<uint32_t>(kMapA) : xmap) + (bx ? kMapN : 0) +
+                                (narrow ? kMap64 : 0);
             const uint32_t depth = kind == kNsXXt ? tn : tm;
             // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
             const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
@@ -668,14 +672,14 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t st = 0, phase = 0;
         for (uint32_t q = 0; rank == 0; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
-            const NsTask& t = s_task[slot];
-            if (uniform(t.stack) == kEnd) break;
-            const uint32_t kind = uniform(t.kind), three = uniform(t.three), width = uniform(t.width);
-            const uint32_t depth = uniform(kind == kNsXXt ? t.n : t.m);
+            if (uniform(s_task[slot].stack) == kEnd) break;
+            const uint32_t shape = uniform(s_task[slot].shape);
+            const uint32_t width = shape & 0xFFFFu, kind = shape >> 16 & 15u, three = shape >> 20 & 1u;
+            const uint32_t depth = uniform(kind == kNsXXt ? s_task[slot].n : s_task[slot].m);
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&task_empty[slot]));
+            if (lane == 0) release_task(slot);
             const bool bx = kind >= kNsBX;
             const uint32_t idesc = instr_desc(width <= kNsTileN / 2 ? kNsTileN / 2 : kNsTileN, bx);
             const uint32_t d = uniform(tmem) + buf * kNsTileN;
@@ -717,263 +721,274 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             bar_wait(smem_u32(&drain_bar), 0, &s_drain_err);
         }
         __syncwarp();
-    } else {
-        // ---- the epilogue, in units of a buffer: a chunk of 64 columns, or (three
-        // products of a symmetric matrix) a chunk and then its mirror image ----
-        struct Unit {
-            uint32_t row0, col0;
-            bool sym, three, lo, some, addend, mirror;
-            uint32_t chunks, per, units;
-        };
-        auto units_of = [&](const NsTask& t) {
-            Unit u;
-            u.row0 = t.row * kNsTileM + rank * kNsRows;
-            u.col0 = t.col * 32u;
-            u.sym = t.kind <= kNsAA;
-            u.three = t.three != 0;
-            u.lo = !u.sym || u.three;       // operand and result have a lo part
-            u.some = u.row0 < t.m;          // this CTA has rows in the tile
-            u.addend = t.kind != kNsXXt;
-            u.mirror = u.sym && u.col0 >= (t.row + 1u) * kNsTileM;  // right of the diagonal's block
-            u.chunks = (t.width + 63u) / 64u;
-            u.per = u.three && u.mirror ? 2 : 1;
-            u.units = u.some ? u.chunks * u.per : 0;
-            return u;
-        };
-        uint32_t g = 0;  // units before this tile
-        if (warp == 2) {
-            // ---- copies: what a unit adds to in, what it makes out ----
-            fence_async_proxy();
-            bool early = false;  // the next tile's first units are on their way
+    } else if (warp == 2) {
+        // ---- the leader hands out tasks, to both CTAs, once their inputs are there ----
+        if (rank == 0 && lane == 0) {
+            // a task is read one task ahead, and its number taken two ahead
+            NsTask ahead{};
+            uint32_t claim = atomicAdd(a.next, 1u);
+            auto read_ahead = [&]() {
+                if (claim < a.n_tasks) ahead = a.tasks[claim];
+                else ahead.stack = kEnd;
+                claim = atomicAdd(a.next, 1u);
+            };
+            read_ahead();
             for (uint32_t q = 0;; ++q) {
                 const uint32_t slot = q % kRing;
-                bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
-                if (!ok) break;
-                const NsTask t = s_task[slot];
+                const NsTask t = ahead;
+                if (t.stack != kEnd) {
+                    read_ahead();
+                    if (t.need && !wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
+                }
+                if (q >= kRing && !bar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
+                    break;
+                s_task[slot] = t;
+                const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&t)[i]);
+                mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 0));
+                mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
                 if (t.stack == kEnd) break;
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
-                const Unit u = units_of(t);
-                auto bring = [&](const NsTask& w, const Unit& v, uint32_t base, uint32_t i) {
-                    const uint32_t b = (base + i) % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
-                    const uint32_t bar = smem_u32(&in_full[b]);
-                    if (!v.addend || (v.per == 2 && (i & 1))) {
-                        mbar_arrive(bar);
-                        return;
-                    }
-                    const CUtensorMap* src = a.maps + static_cast<uint64_t>(w.stack) * kMapsPerStack +
-                                             (v.sym ? kMapA : w.step & 1 ? kMapX1 : kMapX0);
-                    const uint32_t x = v.col0 + (v.per == 2 ? i >> 1 : i) * 64;
-                    mbar_expect_tx(bar, (v.lo ? 2 : 1) * kNsSlotBytes);
-                    tma_load(at, src, bar, x, v.row0, w.index);
-                    if (v.lo) tma_load(at + kNsSlotBytes, src + kMapLo, bar, x, v.row0, w.index);
-                };
-                if (u.units && !early) {
-                    if (u.addend) {
-                        if (lane == 0) ok = wait_done(a.done + t.matrix, t.need, &s_err, a.err);
-                        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-                        fence_async_proxy();
-                    }
-                    if (elect_one()) {
-                        bring(t, u, g, 0);
-                        if (u.units > 1) bring(t, u, g, 1);
-                    }
-                }
-                early = false;
-                const bool last = t.kind == kNsLast;
-                const CUtensorMap* dst =
-                    a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
-                    (t.kind == kNsXXt ? kMapA : t.kind == kNsAA ? kMapB : t.step & 1 ? kMapX0 : kMapX1);
-                for (uint32_t i = 0; i < u.units; ++i) {
-                    const uint32_t b = (g + i) % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
-                    ok = warp_wait(smem_u32(&out_full[b]), ((g + i) / kNsBuffers) & 1, &s_err);
-                    if (!ok) break;
-                    if (elect_one()) {
-                        const uint32_t x = u.col0 + (u.per == 2 ? i >> 1 : i) * 64;
-                        const bool image_only = u.per == 2 && (i & 1);
-                        if (!last) {
-                            if (!image_only) {
-                                tma_store(dst, at, x, u.row0, t.index);
-                                if (u.lo) tma_store(dst + kMapLo, at + kNsSlotBytes, x, u.row0, t.index);
-                            }
-                            if (u.mirror && (image_only || !u.three)) {
-                                const uint32_t image = at + (image_only ? 0 : kNsSlotBytes);
-                                for (uint32_t h = 0; h < 2 && u.row0 + h * 64 < t.m; ++h) {
-                                    tma_store(dst + kMap64, image + h * kNsBoxBytes, u.row0 + h * 64, x, t.index);
-                                    if (image_only)
-                                        tma_store(dst + kMapLo + kMap64, at + kNsSlotBytes + h * kNsBoxBytes,
-                                                  u.row0 + h * 64, x, t.index);
-                                }
-                            }
-                            bulk_commit();
-                        }
-                        if (i + 2 < u.units) {
-                            if (!last) bulk_wait_read<1>();  // the unit before has left its buffer
-                            bring(t, u, g, i + 2);
-                        }
-                    }
-                    __syncwarp();
-                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        // ---- brings what the epilogue adds ----
+        uint32_t g = 0;  // slots filled
+        for (uint32_t q = 0;; ++q) {
+            const uint32_t slot = q % kRing;
+            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            if (!ok) break;
+            const NsTask t = s_task[slot];
+            if (t.stack == kEnd) break;
+            __syncwarp();
+            if (lane == 0) release_task(slot);
+            const Tile u = tile_of(t);
+            if (!u.some || !u.ins) continue;
+            fence_async_proxy();  // (other SMs' stores, by TMA)
+            const CUtensorMap* src = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
+                                     (u.sym ? static_cast<int>(kMapA) : kMapLo + (t.step() & 1 ? kMapX1 : kMapX0));
+            for (uint32_t i = 0; i < u.chunks * u.ins; ++i, ++g) {
+                const uint32_t b = g % kNsIn;
+                ok = warp_wait(smem_u32(&in_empty[b]), (g / kNsIn + 1) & 1, &s_err);
                 if (!ok) break;
-                g += u.units;
-                // the next tile's first units, if their input is there already
-                const uint32_t next = (q + 1) % kRing;
-                if (__all_sync(0xFFFFFFFFu, mbar_try_cluster(smem_u32(&task_full[next]), ((q + 1) / kRing) & 1))) {
-                    const NsTask w = s_task[next];
-                    if (w.stack != kEnd) {
-                        const Unit v = units_of(w);
-                        if (v.units && (!v.addend || __all_sync(0xFFFFFFFFu, ld_acquire(a.done + w.matrix) >= w.need))) {
-                            fence_async_proxy();
-                            early = true;
-                            if (elect_one()) {
-                                bulk_wait_read<1>();
-                                bring(w, v, g, 0);
-                                if (v.units > 1) bring(w, v, g, 1);
-                            }
-                        }
-                    }
-                }
-                if (u.units && !last && elect_one()) {
-                    bulk_wait_all();  // this tile's stores, before it counts as done
-                    fence_async_proxy();
-                    __threadfence();
-                    red_release_add1(a.done + t.matrix);
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&in_full[b]);
+                    mbar_expect_tx(bar, kNsSlotBytes);
+                    tma_load(in_slots + b * kNsSlotBytes, src + (u.ins == 2 && (i & 1) ? kMapLo : 0), bar,
+                             u.col0 + (u.ins == 2 ? i >> 1 : i) * 64, u.row0, t.index);
                 }
                 __syncwarp();
             }
-        } else {
-            // ---- arithmetic: eight warps, each 32 rows of 32 columns of a chunk ----
-            const uint32_t mw = warp - 3, quad = warp & 3, half = mw >> 2;
-            const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
-            for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q % kRing, buf = q & 1;
-                bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
-                const NsTask t = s_task[slot];
-                const bool end = ok && t.stack == kEnd;
-                const Unit u = units_of(t);
-                Target target{};
-                if (ok && !end) {
-                    if (t.kind == kNsLast) {
-                        const NsStack& s = a.stacks[t.stack];
-                        target.dst = kMuon ? s.param : s.dst;
-                        target.master = s.master;
-                        target.ema = s.mom + step.ema_delta;
-                        target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
-                                            : static_cast<uint64_t>(t.index) * s.dst_mat;
-                        target.pitch = kMuon ? s.cols : s.dst_row;
-                        target.lr_wd = __fmul_rn(step.lr, s.wd);
-                        target.lr_s = __fmul_rn(step.lr, s.factor);
+            if (!ok) break;
+        }
+        if (*reinterpret_cast<volatile int*>(&s_err))
+            // copies in flight land before the CTA may end
+            for (uint32_t j = g > kNsIn ? g - kNsIn : 0; j < g; ++j)
+                bar_wait(smem_u32(&in_full[j % kNsIn]), (j / kNsIn) & 1, &s_drain_err);
+        __syncwarp();
+    } else if (warp == 4) {
+        // ---- stores what it makes ----
+        uint32_t g = 0;  // buffers stored
+        for (uint32_t q = 0;; ++q) {
+            const uint32_t slot = q % kRing;
+            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            if (!ok) break;
+            const NsTask t = s_task[slot];
+            if (t.stack == kEnd) break;
+            __syncwarp();
+            if (lane == 0) release_task(slot);
+            const Tile u = tile_of(t);
+            // (the last product's result leaves with the arithmetic)
+            if (!u.some || t.kind() == kNsLast) continue;
+            const CUtensorMap* dst = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
+                                     (t.kind() == kNsXXt ? kMapA
+                                      : u.sym            ? kMapB
+                                      : t.step() & 1     ? kMapX0
+                                                         : kMapX1);
+            const uint32_t units = u.chunks * u.outs;
+            for (uint32_t i = 0; i < units; ++i, ++g) {
+                const uint32_t b = g % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
+                ok = warp_wait(smem_u32(&out_full[b]), (g / kNsOut) & 1, &s_err);
+                if (!ok) break;
+                if (elect_one()) {
+                    const uint32_t x = u.col0 + (u.outs == 2 ? i >> 1 : i) * 64;
+                    const bool image_only = u.outs == 2 && (i & 1);
+                    if (!image_only) {
+                        tma_store(dst, at, x, u.row0, t.index);
+                        if (u.lo) tma_store(dst + kMapLo, at + kNsSlotBytes, x, u.row0, t.index);
                     }
-                    ok = warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
+                    if (u.mirror && (image_only || !u.three)) {
+                        const uint32_t image = at + (image_only ? 0 : kNsSlotBytes);
+                        for (uint32_t h = 0; h < 2 && u.row0 + h * 64 < t.m; ++h) {
+                            tma_store(dst + kMap64, image + h * kNsBoxBytes, u.row0 + h * 64, x, t.index);
+                            if (image_only)
+                                tma_store(dst + kMapLo + kMap64, at + kNsSlotBytes + h * kNsBoxBytes,
+                                          u.row0 + h * 64, x, t.index);
+                        }
+                    }
+                    bulk_commit();
+                    // a buffer is free once its stores have read it: seen when the next one's are
+                    // on their way, or now where the next chunk takes both buffers or none comes
+                    const bool at_once = i + 1 == units || (u.outs == 2 && (i & 1));
+                    const uint32_t other = smem_u32(&out_empty[(g + kNsOut - 1) % kNsOut]);
+                    if (at_once) {
+                        bulk_wait_read<0>();
+                        if (i > 0) mbar_arrive(other);
+                        mbar_arrive(smem_u32(&out_empty[b]));
+                    } else if (i > 0 && u.outs == 1) {
+                        bulk_wait_read<1>();
+                        mbar_arrive(other);
+                    }
+                    if (i + 1 == units) {
+                        bulk_wait_all();  // this tile's stores, before it counts as done
+                        fence_async_proxy();
+                        __threadfence();
+                        red_release_add1(a.done + t.matrix);
+                    }
                 }
-                if (!ok) s_cfail[q & 1] = 1;
-                consumers_sync<kMath>();  // all go on, or none
-                if (s_cfail[q & 1] || end) break;
-                if (threadIdx.x == kFirstMath) mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
-                tc_fence_after();
-                const float ca = a.coef[t.step][0], cb = a.coef[t.step][1], cc = a.coef[t.step][2];
-                const bool two = u.three && (t.kind == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
-                // v = fx addend + fv accumulator
-                const float fx = u.sym ? cb : ca;
-                const float fv = t.kind == kNsXXt ? kNsScaleA / (t.sx * t.sx)
-                                                  : t.kind == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
-                for (uint32_t c = 0; c < u.chunks; ++c) {
-                    const uint32_t i = g + c * u.per, b = i % kNsBuffers, at = staging + b * 2 * kNsSlotBytes;
-                    float v[32];
-                    const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32;
+                __syncwarp();
+            }
+            if (!ok) break;
+        }
+        __syncwarp();
+    } else {
+        // ---- arithmetic: eight warps, each 32 rows of 32 columns of a chunk ----
+        const uint32_t mw = warp - kMathWarp, quad = warp & 3, half = mw >> 2;
+        const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
+        uint32_t gi = 0, go = 0;                 // slots taken, buffers made
+        for (uint32_t q = 0;; ++q) {
+            const uint32_t slot = q % kRing, buf = q & 1;
+            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            const NsTask t = s_task[slot];
+            const bool end = ok && t.stack == kEnd;
+            const Tile u = tile_of(t);
+            const bool last = t.kind() == kNsLast;
+            Target target{};
+            if (ok && !end) {
+                if (last) {
+                    const NsStack& s = a.stacks[t.stack];
+                    target.dst = kMuon ? s.param : s.dst;
+                    target.master = s.master;
+                    target.ema = s.mom + step.ema_delta;
+                    target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
+                                        : static_cast<uint64_t>(t.index) * s.dst_mat;
+                    target.pitch = kMuon ? s.cols : s.dst_row;
+                    target.lr_wd = __fmul_rn(step.lr, s.wd);
+                    target.lr_s = __fmul_rn(step.lr, s.factor);
+                }
+                ok = warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
+            }
+            if (!ok) s_cfail[q & 1] = 1;
+            consumers_sync<kMath>();  // all go on, or none
+            if (s_cfail[q & 1] || end) break;
+            if (mw == 0 && lane == 0) release_task(slot);
+            tc_fence_after();
+            const float ca = a.coef[t.step()][0], cb = a.coef[t.step()][1], cc = a.coef[t.step()][2];
+            const bool two = u.three && (t.kind() == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
+            // v = fv accumulator + fx addend (+ fd on the diagonal)
+            const float fx = u.sym ? cb : ca;
+            const float fv = t.kind() == kNsXXt ? kNsScaleA / (t.sx * t.sx)
+                                                : t.kind() == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
+            for (uint32_t c = 0; c < u.chunks; ++c) {
+                float v[32];
+                const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32;
+                __syncwarp();
+                tmem_ld32(acc, v);
+                if (two) {
+                    float w[32];
+                    tmem_ld32(acc + kNsTileN / 2, w);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] += w[j];
+                }
+                if (c + 1 == u.chunks) {
+                    tc_fence_before();
                     __syncwarp();
-                    tmem_ld32(acc, v);
-                    if (two) {
-                        float w[32];
-                        tmem_ld32(acc + kNsTileN / 2, w);
+                    if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+                }
+                if (!u.some) continue;
+                const uint32_t col = u.col0 + c * 64;
+                // (a wait that runs out has set s_err: the next tile ends the loop)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] += w[j];
-                    }
-                    if (c + 1 == u.chunks) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
-                    }
-                    if (!u.some) continue;
-                    const uint32_t col = u.col0 + c * 64;
-                    // (a wait that runs out has set s_err: the next tile ends the loop)
-                    warp_wait(smem_u32(&in_full[b]), (i / kNsBuffers) & 1, &s_err);
-                    if (u.addend) {
-                        float x[32];
-                        slot_read<false>(at, trow, half, x);
-                        if (u.lo) slot_read<true>(at + kNsSlotBytes, trow, half, x);
+                for (int j = 0; j < 32; ++j) v[j] *= fv;
+                for (uint32_t i = 0; i < u.ins; ++i, ++gi) {
+                    const uint32_t b = gi % kNsIn;
+                    warp_wait(smem_u32(&in_full[b]), (gi / kNsIn) & 1, &s_err);
+                    slot_add(in_slots + b * kNsSlotBytes, trow, half, fx, v);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&in_empty[b]));
+                }
+                if (last) {
+                    // through shared memory as floats, so that the result is written row by row of
+                    // the caller's matrix; in the two out buffers by turns, between which the
+                    // barrier keeps the warps within a chunk of each other
+                    const uint32_t b = c % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
+                    const uint32_t use = go + (go + b) % kNsOut;  // (the stores before have left it)
+                    warp_wait(smem_u32(&out_empty[b]), (use / kNsOut + 1) & 1, &s_err);
+                    const float f = 1.0f / t.sx;
+                    float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __fmaf_rn(fx, x[j], fv * v[j]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] *= fv;
-                    }
-                    if (t.kind == kNsLast) {
-                        // through shared memory as floats, so that the result is written row by
-                        // row of the caller's matrix
-                        const float f = 1.0f / t.sx;
-                        float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
-                        consumers_sync<kMath>();  // (all have read their addend)
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
-                        consumers_sync<kMath>();
+                    for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
+                    consumers_sync<kMath>();
 #pragma unroll 1
-                        for (int k = 0; k < 4; ++k) {
-                            uint64_t to[8];
-                            float o[8];
-                            uint32_t valid = 0;
+                    for (int k = 0; k < 4; ++k) {
+                        uint64_t to[8];
+                        float o[8];
+                        uint32_t valid = 0;
 #pragma unroll
-                            for (int l = 0; l < 8; ++l) {
-                                const uint32_t e = k * 8 + l;
-                                const uint32_t rr = t.transposed ? lane + 32 * (e & 3) : mw * 16 + (e >> 1);
-                                const uint32_t rc = t.transposed ? mw * 8 + (e >> 2) : lane + 32 * (e & 1);
-                                const uint32_t y = u.row0 + rr, x = col + rc;
-                                to[l] = target.base + (t.transposed ? x * target.pitch + y : y * target.pitch + x);
-                                o[l] = fs[float_at(rr, rc)];
-                                if (y < t.m && x < t.n) valid |= 1u << l;
-                            }
-                            put_result<kDst>(step, target, a.ema != 0, to, o, valid);
+                        for (int l = 0; l < 8; ++l) {
+                            const uint32_t e = k * 8 + l;
+                            const uint32_t rr = t.transposed() ? lane + 32 * (e & 3) : mw * 16 + (e >> 1);
+                            const uint32_t rc = t.transposed() ? mw * 8 + (e >> 2) : lane + 32 * (e & 1);
+                            const uint32_t y = u.row0 + rr, x = col + rc;
+                            to[l] = target.base + (t.transposed() ? x * target.pitch + y : y * target.pitch + x);
+                            o[l] = fs[float_at(rr, rc)];
+                            if (y < t.m && x < t.n) valid |= 1u << l;
                         }
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&out_full[b]));
-                        continue;
+                        put_result<kDst>(step, target, a.ema != 0, to, o, valid);
                     }
-                    // hi and lo in place of the addend; the mirror image in the second slot, or
-                    // in the next buffer
-                    const uint32_t b1 = (i + 1) % kNsBuffers;
-                    const uint32_t image = u.per == 2 ? staging + b1 * 2 * kNsSlotBytes : at + kNsSlotBytes;
-                    if (u.per == 2) warp_wait(smem_u32(&in_full[b1]), ((i + 1) / kNsBuffers) & 1, &s_err);
+                    continue;
+                }
+                const uint32_t b = go % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
+                if (t.kind() == kNsAA) {
+                    const uint32_t diag = u.row0 + trow - (col + half * 32);  // (no match: no column)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t h[4], l[4];
+                    for (int j = 0; j < 32; ++j) v[j] += diag == static_cast<uint32_t>(j) ? ca * kNsScaleA : 0.0f;
+                }
+                // hi and lo; the mirror image in the second slot, or in the next buffer
+                warp_wait(smem_u32(&out_empty[b]), (go / kNsOut + 1) & 1, &s_err);
+                const uint32_t b1 = (go + 1) % kNsOut;
+                const uint32_t image = u.outs == 2 ? out_slots + b1 * 2 * kNsSlotBytes : at + kNsSlotBytes;
+                if (u.outs == 2) warp_wait(smem_u32(&out_empty[b1]), ((go + 1) / kNsOut + 1) & 1, &s_err);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
-                        const uint32_t o = slot_at(trow, half * 4 + j);
-                        sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
-                        if (u.lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
-                        if (u.mirror) {
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h[4], l[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
-                                const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
-                                sts16(image + m0, h[e] & 0xFFFFu);
-                                sts16(image + m1, h[e] >> 16);
-                                if (u.lo) {
-                                    sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
-                                    sts16(image + kNsSlotBytes + m1, l[e] >> 16);
-                                }
+                    for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
+                    const uint32_t o = slot_at(trow, half * 4 + j);
+                    sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
+                    if (u.lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
+                    if (u.mirror) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
+                            const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
+                            sts16(image + m0, h[e] & 0xFFFFu);
+                            sts16(image + m1, h[e] >> 16);
+                            if (u.lo) {
+                                sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
+                                sts16(image + kNsSlotBytes + m1, l[e] >> 16);
                             }
                         }
-                    }
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&out_full[b]));
-                        if (u.per == 2) mbar_arrive(smem_u32(&out_full[b1]));
                     }
                 }
-                g += u.units;
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(smem_u32(&out_full[b]));
+                    if (u.outs == 2) mbar_arrive(smem_u32(&out_full[b1]));
+                }
+                go += u.outs;
             }
         }
     }

@@ -4,23 +4,23 @@
 //
 // For a matrix G with shorter side m and longer side n (transposed where it
 // has more rows than columns, so that X is m x n):
-//   X = G / (|G|_F + eps);  per iteration:  A = X X^T,  B = b A + c A A,
-//   X <- a X + B X.
+//   X = G / (|G|_F + eps);  per iteration:  A = X X^T,  B = a I + b A + c A A,
+//   X <- B X.
 //
 // Numbers: the products run on the tensor cores with fp16 operands and fp32
-// sums. X is kept as hi + lo, two fp16 numbers of 11 bits each, and a X is
-// taken from both; only the operands of products are rounded to hi. A rounding
-// of X's small singular directions would otherwise grow by a factor of a (3.4)
-// per iteration: with X in hi alone, a matrix of a few strong directions over
-// noise comes out 0.6 % to 7 % off (bf16 operands: 5 % to 60 %), with hi + lo
-// 0.03 % to 0.2 %. That is below the rounding of a bf16 result (0.17 % rms).
-// For fp32 results every product is taken as hi hi + hi lo + lo hi of both
-// operands (22 bits).
+// sums. X is kept as hi + lo, two fp16 numbers of 11 bits each: with B = a I +
+// b A + c A A, X becomes B hi + a lo, so that only products of small entries
+// lose lo. A rounding of X's small singular directions would otherwise grow by
+// a factor of a (3.4) per iteration: with X in hi alone, a matrix of a few
+// strong directions over noise comes out 0.6 % to 7 % off (bf16 operands: 5 %
+// to 60 %), with hi + lo 0.03 % to 0.2 %. That is below the rounding of a bf16
+// result (0.17 % rms). For fp32 results every product is taken as hi hi + hi lo
+// + lo hi of both operands (22 bits).
 //
 // fp16's range is met by powers of two: X is held times sx = 2^floor(log2 sqrt(m n))
 // (within 2^6 .. 2^12), which gives its elements an rms of about 1 at the start
 // and of at most sqrt(m) at the end; A and B are held times 2^10, where their
-// eigenvalues (at most about 1.5, and 3) stay below 2^12 and entries down to
+// eigenvalues (at most about 1.5, and 4) stay below 2^12 and entries down to
 // 2^-34 still count.
 #pragma once
 
@@ -48,13 +48,15 @@ constexpr int kNsRows = 128;   // a CTA's share of the rows
 constexpr int kNsTileK = 64;   // depth of one stage
 constexpr int kNsStages = 4;
 constexpr int kNsMathWarps = 8;
-constexpr int kNsThreads = (3 + kNsMathWarps) * 32;  // operand copies, products, epilogue copies, epilogue
+// operand copies, products, hand-out, epilogue's copies in, and out, arithmetic
+constexpr int kNsThreads = (5 + kNsMathWarps) * 32;
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
 constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
 constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue: 128 rows of 64 fp16
-constexpr int kNsBuffers = 3;                       // epilogue buffers of two slots
-constexpr size_t kNsSmemBytes =
-    static_cast<size_t>(kNsStages) * kNsStageBytes + 2 * kNsBuffers * kNsSlotBytes + 1024;
+constexpr int kNsIn = 2;   // slots of what it adds
+constexpr int kNsOut = 2;  // buffers of two slots of what it makes
+constexpr size_t kNsSmemBytes = static_cast<size_t>(kNsStages) * kNsStageBytes +
+                                (kNsIn + 2 * kNsOut) * kNsSlotBytes + 1024;
 
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
@@ -114,21 +116,25 @@ struct PrepTile {
 enum NsKind : uint32_t { kNsXXt = 0, kNsAA = 1, kNsBX = 2, kNsLast = 3 };
 struct __align__(16) NsTask {
     uint32_t stack;
-    uint32_t index;     // matrix of the stack
-    uint32_t matrix;    // matrix of the plan
-    uint32_t need;      // CTAs' tiles of this matrix that must be done before
-    uint16_t row, col;  // first row and column, in units of 256 and 32
-    uint16_t width;     // columns
-    uint8_t kind;
-    uint8_t step;
+    uint32_t index;   // matrix of the stack
+    uint32_t place;   // first row / 256 | first column / 32 << 16
+    uint32_t shape;   // columns | kind << 16 | three products << 20 | transposed << 21 | step << 24
     // of the stack, so that a tile needs one read
     uint32_t m, n;
     float sx;
-    uint8_t three, transposed;
-    uint8_t pad[2];
-    uint32_t pad2[5];
+    uint32_t matrix;  // matrix of the plan
+    uint32_t need;    // CTAs' tiles of this matrix that must be done before
+    uint32_t pad[3];
+
+    __host__ __device__ uint32_t row() const { return (place & 0xFFFFu) * kNsTileM; }
+    __host__ __device__ uint32_t col() const { return (place >> 16) * 32u; }
+    __host__ __device__ uint32_t width() const { return shape & 0xFFFFu; }
+    __host__ __device__ uint32_t kind() const { return shape >> 16 & 15u; }
+    __host__ __device__ bool three() const { return shape >> 20 & 1u; }
+    __host__ __device__ bool transposed() const { return shape >> 21 & 1u; }
+    __host__ __device__ uint32_t step() const { return shape >> 24; }
 };
-static_assert(sizeof(NsTask) == 64, "a task is four 16-byte loads");
+static_assert(sizeof(NsTask) == 48, "a task is three 16-byte loads");
 
 // A Muon step's decision, from its first kernel for the others.
 struct MatrixStep {

@@ -241,19 +241,15 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                             NsTask k{};
                             k.stack = wave[w].stack;
                             k.index = i;
-                            k.matrix = s.first + i;
-                            k.need = counted[w];
+                            k.place = t.row | static_cast<uint32_t>(t.col) << 16;
+                            k.shape = t.width |
+                                      (kind == kNsBX && step + 1 == opts.steps ? kNsLast : kind) << 16 |
+                                      s.three << 20 | s.transposed << 21 | static_cast<uint32_t>(step) << 24;
                             k.m = s.m;
                             k.n = s.n;
                             k.sx = s.sx;
-                            k.three = static_cast<uint8_t>(s.three);
-                            k.transposed = static_cast<uint8_t>(s.transposed);
-                            k.row = t.row;
-                            k.col = t.col;
-                            k.width = t.width;
-                            k.kind = static_cast<uint8_t>(
-                                kind == kNsBX && step + 1 == opts.steps ? kNsLast : kind);
-                            k.step = static_cast<uint8_t>(step);
+                            k.matrix = s.first + i;
+                            k.need = counted[w];
                             tasks.push_back(k);
                         }
                     // (a CTA without rows in a tile does not count it)
