@@ -14,7 +14,7 @@
 //                   that waits, waits only for tiles that running CTAs hold,
 //                   whatever else runs on the GPU.
 //                   One warp loads operand tiles by TMA, one thread issues
-//                   tcgen05.mma into one of two TMEM accumulators, eight warps
+//                   tcgen05.mma into one of two TMEM accumulators, sixteen warps
 //                   turn finished accumulators into the next operand: A, B =
 //                   aI + bA + cAA, X = BX, or the result (for Muon: the
 //                   weights' update). A and B are symmetric: only tiles on or
@@ -354,22 +354,19 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         "h"(static_cast<uint16_t>(3))
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
-    uint32_t r[32];
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[14]), "=r"(r[15])
         : "r"(addr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -439,11 +436,11 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
 
-// v += f times the thread's 32 columns of its row.
-__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, uint32_t half, float f, float (&v)[32]) {
+// v += f times the thread's 16 columns (a quarter of the chunk) of its row.
+__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, uint32_t part, float f, float (&v)[16]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint4 q = lds128(slot + slot_at(row, half * 4 + j));
+    for (int j = 0; j < 2; ++j) {
+        const uint4 q = lds128(slot + slot_at(row, part * 2 + j));
         const __half2* h = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -853,8 +850,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         }
         __syncwarp();
     } else {
-        // ---- arithmetic: eight warps, each 32 rows of 32 columns of a chunk ----
-        const uint32_t mw = warp - kMathWarp, quad = warp & 3, half = mw >> 2;
+        // ---- arithmetic: sixteen warps, each 32 rows of 16 columns of a chunk ----
+        const uint32_t mw = warp - kMathWarp, quad = warp & 3, part = mw >> 2;
         const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
         uint32_t gi = 0, go = 0;                 // slots taken, buffers made
         for (uint32_t q = 0;; ++q) {
@@ -891,15 +888,15 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const float fv = t.kind() == kNsXXt ? kNsScaleA / (t.sx * t.sx)
                                                 : t.kind() == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
             for (uint32_t c = 0; c < u.chunks; ++c) {
-                float v[32];
-                const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + half * 32;
+                float v[16];
+                const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + part * 16;
                 __syncwarp();
-                tmem_ld32(acc, v);
+                tmem_ld16(acc, v);
                 if (two) {
-                    float w[32];
-                    tmem_ld32(acc + kNsTileN / 2, w);
+                    float w[16];
+                    tmem_ld16(acc + kNsTileN / 2, w);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += w[j];
+                    for (int j = 0; j < 16; ++j) v[j] += w[j];
                 }
                 if (c + 1 == u.chunks) {
                     tc_fence_before();
@@ -910,11 +907,11 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 const uint32_t col = u.col0 + c * 64;
                 // (a wait that runs out has set s_err: the next tile ends the loop)
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= fv;
+                for (int j = 0; j < 16; ++j) v[j] *= fv;
                 for (uint32_t i = 0; i < u.ins; ++i, ++gi) {
                     const uint32_t b = gi % kNsIn;
                     warp_wait(smem_u32(&in_full[b]), (gi / kNsIn) & 1, &s_err);
-                    slot_add(in_slots + b * kNsSlotBytes, trow, half, fx, v);
+                    slot_add(in_slots + b * kNsSlotBytes, trow, part, fx, v);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&in_empty[b]));
                 }
@@ -928,18 +925,18 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                     const float f = 1.0f / t.sx;
                     float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) fs[float_at(trow, half * 32 + j)] = v[j] * f;
+                    for (int j = 0; j < 16; ++j) fs[float_at(trow, part * 16 + j)] = v[j] * f;
                     consumers_sync<kMath>();
+                    // a warp's eight rows of the chunk (columns, where the matrix is transposed)
 #pragma unroll 1
-                    for (int k = 0; k < 4; ++k) {
+                    for (uint32_t k = 0; k < 2; ++k) {
                         uint64_t to[8];
                         float o[8];
                         uint32_t valid = 0;
 #pragma unroll
-                        for (int l = 0; l < 8; ++l) {
-                            const uint32_t e = k * 8 + l;
-                            const uint32_t rr = t.transposed() ? lane + 32 * (e & 3) : mw * 16 + (e >> 1);
-                            const uint32_t rc = t.transposed() ? mw * 8 + (e >> 2) : lane + 32 * (e & 1);
+                        for (uint32_t l = 0; l < 8; ++l) {
+                            const uint32_t rr = t.transposed() ? lane + 32 * (l & 3) : mw * 8 + k * 4 + (l >> 1);
+                            const uint32_t rc = t.transposed() ? mw * 4 + k * 2 + (l >> 2) : lane + 32 * (l & 1);
                             const uint32_t y = u.row0 + rr, x = col + rc;
                             to[l] = target.base + (t.transposed() ? x * target.pitch + y : y * target.pitch + x);
                             o[l] = fs[float_at(rr, rc)];
@@ -951,9 +948,9 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 }
                 const uint32_t b = go % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
                 if (t.kind() == kNsAA) {
-                    const uint32_t diag = u.row0 + trow - (col + half * 32);  // (no match: no column)
+                    const uint32_t diag = u.row0 + trow - (col + part * 16);  // (no match: no column)
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] += diag == static_cast<uint32_t>(j) ? ca * kNsScaleA : 0.0f;
+                    for (int j = 0; j < 16; ++j) v[j] += diag == static_cast<uint32_t>(j) ? ca * kNsScaleA : 0.0f;
                 }
                 // hi and lo; the mirror image in the second slot, or in the next buffer
                 warp_wait(smem_u32(&out_empty[b]), (go / kNsOut + 1) & 1, &s_err);
@@ -961,18 +958,18 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 const uint32_t image = u.outs == 2 ? out_slots + b1 * 2 * kNsSlotBytes : at + kNsSlotBytes;
                 if (u.outs == 2) warp_wait(smem_u32(&out_empty[b1]), ((go + 1) / kNsOut + 1) & 1, &s_err);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
-                    const uint32_t o = slot_at(trow, half * 4 + j);
+                    const uint32_t o = slot_at(trow, part * 2 + j);
                     sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
                     if (u.lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
                     if (u.mirror) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t m0 = mirror_at(trow, half * 32 + j * 8 + 2 * e);
-                            const uint32_t m1 = mirror_at(trow, half * 32 + j * 8 + 2 * e + 1);
+                            const uint32_t m0 = mirror_at(trow, part * 16 + j * 8 + 2 * e);
+                            const uint32_t m1 = mirror_at(trow, part * 16 + j * 8 + 2 * e + 1);
                             sts16(image + m0, h[e] & 0xFFFFu);
                             sts16(image + m1, h[e] >> 16);
                             if (u.lo) {

@@ -47,7 +47,7 @@ constexpr int kNsTileN = 256;
 constexpr int kNsRows = 128;   // a CTA's share of the rows
 constexpr int kNsTileK = 64;   // depth of one stage
 constexpr int kNsStages = 4;
-constexpr int kNsMathWarps = 8;
+constexpr int kNsMathWarps = 16;  // four to a quarter of the rows: a chunk's latencies overlap
 // operand copies, products, hand-out, epilogue's copies in, and out, arithmetic
 constexpr int kNsThreads = (5 + kNsMathWarps) * 32;
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
