@@ -284,10 +284,12 @@ __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
         if (!__all_sync(0xFFFFFFFFu, p.more(s_err))) return false;
     return true;
 }
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint4& v) {
-    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
-                 "r"(v.z), "r"(v.w)
-                 : "memory");
+// Sixteen bytes into the other CTA's shared memory, counted on a barrier there.
+__device__ __forceinline__ void st_async_v4(uint32_t addr, const uint4& v, uint32_t bar) {
+    asm volatile(
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(addr),
+        "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(bar)
+        : "memory");
 }
 
 // Into this CTA's shared memory; the bytes count on `bar` of either CTA of the pair.
@@ -354,19 +356,22 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         "h"(static_cast<uint16_t>(3))
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
-    uint32_t r[16];
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float* v) {
+    uint32_t r[32];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15])
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -415,10 +420,12 @@ __device__ __forceinline__ uint32_t slot_at(uint32_t row, uint32_t j) {
 __device__ __forceinline__ uint32_t mirror_at(uint32_t row, uint32_t col) {
     return (row >> 6) * kNsBoxBytes + col * 128u + ((((row & 63u) >> 3) ^ (col & 7u)) << 4) + (row & 7u) * 2u;
 }
-// Word offset of (row, col) of a chunk of floats in two slots: rows and
-// columns are both read and written without bank conflicts.
+// Word offset of (row, col) of a chunk of floats in two slots, 32 columns in
+// each, a row where its fp16 are otherwise. Rows and columns are both read and
+// written without bank conflicts.
 __device__ __forceinline__ uint32_t float_at(uint32_t row, uint32_t col) {
-    return row * 64u + (((col >> 2) ^ (row & 15u)) << 2) + ((col + (row >> 3)) & 3u);
+    return (col >> 5) * (kNsSlotBytes / 4) + row * 32u + ((((col & 31u) >> 2) ^ (row & 7u)) << 2) +
+           ((col + (row >> 3)) & 3u);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
@@ -436,11 +443,11 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
 
-// v += f times the thread's 16 columns (a quarter of the chunk) of its row.
-__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, uint32_t part, float f, float (&v)[16]) {
+// v += f times the thread's row of a chunk.
+__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, float f, float (&v)[64]) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const uint4 q = lds128(slot + slot_at(row, part * 2 + j));
+    for (int j = 0; j < 8; ++j) {
+        const uint4 q = lds128(slot + slot_at(row, j));
         const __half2* h = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -516,17 +523,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
     constexpr int kRing = 4;  // tasks handed out ahead
-    constexpr int kMath = kNsMathWarps * 32;
     constexpr int kMathWarp = 5;            // the first of them
     constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t in_full[kNsIn], in_empty[kNsIn], out_full[kNsOut], out_empty[kNsOut];
+    __shared__ __align__(8) uint64_t in_full[kNsGroups], in_empty[kNsGroups], out_full[kNsGroups],
+        out_empty[kNsGroups];
     __shared__ __align__(8) uint64_t drain_bar;
     __shared__ __align__(16) NsTask s_task[kRing];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_err, s_drain_err, s_cfail[2];
+    __shared__ int s_err, s_drain_err;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
@@ -537,7 +544,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     const uint32_t rank = blockIdx.x & 1u;  // 0 leads the pair: hands out tasks, issues products
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t in_slots = smem + kNsStages * kNsStageBytes;
-    const uint32_t out_slots = in_slots + kNsIn * kNsSlotBytes;
+    const uint32_t out_slots = in_slots + kNsGroups * kNsSlotBytes;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNsStages; ++i) {
             mbar_init(smem_u32(&full_bar[i]), 1);
@@ -547,20 +554,20 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             mbar_init(smem_u32(&acc_full[i]), 1);
             mbar_init(smem_u32(&acc_empty[i]), 2 * kNsMathWarps);  // both CTAs' warps
         }
-        for (int i = 0; i < kNsIn; ++i) {
+        for (int i = 0; i < kNsGroups; ++i) {
             mbar_init(smem_u32(&in_full[i]), 1);
-            mbar_init(smem_u32(&in_empty[i]), kNsMathWarps);
-        }
-        for (int i = 0; i < kNsOut; ++i) {
-            mbar_init(smem_u32(&out_full[i]), kNsMathWarps);
+            mbar_init(smem_u32(&in_empty[i]), kNsMathWarps / kNsGroups);
+            mbar_init(smem_u32(&out_full[i]), kNsMathWarps / kNsGroups);
             mbar_init(smem_u32(&out_empty[i]), 1);
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            mbar_init(smem_u32(&task_empty[i]), 9);  // five readers here, four in the other CTA
+            // four readers and the arithmetic here, three and the arithmetic in the other CTA
+            mbar_init(smem_u32(&task_empty[i]), 7 + 2 * kNsMathWarps);
+            if (rank == 1) mbar_expect_tx(smem_u32(&task_full[i]), sizeof(NsTask));
         }
         mbar_init(smem_u32(&drain_bar), 1);
-        s_err = s_drain_err = s_cfail[0] = s_cfail[1] = 0;
+        s_err = s_drain_err = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -579,8 +586,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
     };
 
-    // What the epilogue does with a tile: chunks of 64 columns, `ins` slots to add to each and
-    // `outs` buffers made of each.
+    // What the epilogue does with a tile: chunks of 64 columns, taken by the two groups of its
+    // warps by turns, `ins` slots to add to each and `outs` buffers made of each.
     struct Tile {
         uint32_t row0, col0, chunks, ins, outs;
         bool sym, three, lo, some, mirror;
@@ -603,8 +610,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
 
     if (warp == 0) {
         // ---- loads operand tiles ----
-        uint32_t st = 0, phase = 1;  // the next stage; its empty barrier's phase to wait for
-        uint32_t issued = 0;
+        fence_async_proxy();  // (X of the kernel before)
+        uint32_t phases = ~0u;  // by stage: its empty barrier's phase to wait for
         const uint32_t lead_full = uniform(map_to(smem_u32(&full_bar[0]), 0));
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
@@ -616,8 +623,11 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint32_t shape = uniform(s_task[slot].shape);
             const uint32_t tm = uniform(s_task[slot].m), tn = uniform(s_task[slot].n);
             __syncwarp();
-            if (lane == 0) release_task(slot);
-            fence_async_proxy();  // (other SMs' stores, by TMA)
+            if (lane == 0) {
+                // (the record of the slot's next task counts on its barrier as it comes)
+                if (rank == 1) mbar_expect_tx(smem_u32(&task_full[slot]), sizeof(NsTask));
+                release_task(slot);
+            }
             const uint32_t width = shape & 0xFFFFu, kind = shape >> 16 & 15u, three = shape >> 20 & 1u;
             const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
             const bool bx = kind >= kNsBX;
@@ -633,13 +643,18 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint32_t depth = kind == kNsXXt ? tn : tm;
             // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
             const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
-            for (uint32_t p = three ? 0 : 2; p < 3 && ok; ++p) {
-                // the small products first: lo hi, hi lo, hi hi
-                const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
-                const CUtensorMap* mapb = maps + mb + (p == 1 ? kMapLo : 0);
-                for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK) {
-                    ok = warp_wait(smem_u32(&empty_bar[st]), phase, &s_err);
+            // three products: the small ones first, lo hi, hi lo, hi hi
+            uint32_t p = three ? 0 : 2, k0 = 0;
+            const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
+            const CUtensorMap* mapb = maps + mb;
+            // (a tile starts at the first stage: addresses in the loop are constants)
+            while (ok && p < 3) {
+#pragma unroll
+                for (uint32_t st = 0; st < kNsStages; ++st) {
+                    if (p == 3) break;
+                    ok = warp_wait(smem_u32(&empty_bar[st]), phases >> st & 1u, &s_err);
                     if (!ok) break;
+                    phases ^= 1u << st;
                     if (elect_one()) {
                         const uint32_t bar = lead_full + st * 8;
                         const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
@@ -650,23 +665,26 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         else
                             tma_load_pair(sb, mapb, bar, k0, col, index);
                     }
-                    ++issued;
-                    if (++st == kNsStages) {
-                        st = 0;
-                        phase ^= 1;
+                    k0 += kNsTileK;
+                    if (k0 >= depth) {
+                        k0 = 0;
+                        ++p;
+                        mapa = maps + ma;
+                        mapb = maps + mb + (p == 1 ? kMapLo : 0);
                     }
                 }
             }
             if (!ok) break;
         }
         if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0 && lane == 0) {
-            // copies in flight land before the CTA may end
-            for (uint32_t j = issued > kNsStages ? issued - kNsStages : 0; j < issued; ++j)
-                bar_wait(smem_u32(&full_bar[j % kNsStages]), (j / kNsStages) & 1, &s_drain_err);
+            // copies in flight land before the CTA may end (a stage's next phase to wait for on
+            // its empty barrier is also the one its last copies complete on its full barrier)
+            for (uint32_t st = 0; st < kNsStages; ++st)
+                bar_wait(smem_u32(&full_bar[st]), phases >> st & 1u, &s_drain_err);
         }
     } else if (warp == 1) {
         // ---- the leader's second warp issues the pair's products ----
-        uint32_t st = 0, phase = 0;
+        uint32_t phases = 0;  // by stage: its full barrier's phase to wait for
         for (uint32_t q = 0; rank == 0; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
             bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
@@ -691,24 +709,27 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             if (q >= 2) ok = warp_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err);
             if (!ok) break;
             tc_fence_after();
-            for (uint32_t j = 0; j < steps; ++j) {
-                ok = warp_wait(smem_u32(&full_bar[st]), phase, &s_err);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
+            for (uint32_t j = 0; j < steps && ok;) {
+#pragma unroll
+                for (uint32_t st = 0; st < kNsStages; ++st) {
+                    if (j == steps) break;
+                    ok = warp_wait(smem_u32(&full_bar[st]), phases >> st & 1u, &s_err);
+                    if (!ok) break;
+                    phases ^= 1u << st;
+                    tc_fence_after();
                     const bool second = j >= from && j < to;
                     const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
                     const bool fresh = j == 0 || (second && j == from);
-                    const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
+                    if (elect_one()) {
+                        const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
+                        mma_f16(dd, da, db, idesc, !fresh);
 #pragma unroll
-                    for (uint32_t k = 0; k < kNsTileK / 16; ++k)
-                        mma_f16(dd, da + k * 2, db + k * db_k, idesc, !(fresh && k == 0));
-                    mma_commit(smem_u32(&empty_bar[st]));
-                    if (j + 1 == steps) mma_commit(smem_u32(&acc_full[buf]));
-                }
-                if (++st == kNsStages) {
-                    st = 0;
-                    phase ^= 1;
+                        for (uint32_t k = 1; k < kNsTileK / 16; ++k)
+                            mma_f16(dd, da + k * 2, db + k * db_k, idesc, true);
+                        mma_commit(smem_u32(&empty_bar[st]));
+                        if (j + 1 == steps) mma_commit(smem_u32(&acc_full[buf]));
+                    }
+                    ++j;
                 }
             }
             if (!ok) break;
@@ -735,23 +756,28 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 const NsTask t = ahead;
                 if (t.stack != kEnd) {
                     read_ahead();
-                    if (t.need && !wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
+                    if (t.need) {
+                        if (!wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
+                        fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
+                    }
                 }
                 if (q >= kRing && !bar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
                     break;
-                s_task[slot] = t;
                 const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
 #pragma unroll
-                for (int i = 0; i < 3; ++i) st_cluster_v4(there + 16 * i, reinterpret_cast<const uint4*>(&t)[i]);
-                mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 0));
-                mbar_arrive_cluster(map_to(smem_u32(&task_full[slot]), 1));
+                for (int i = 0; i < 3; ++i)
+                    st_async_v4(there + 16 * i, reinterpret_cast<const uint4*>(&t)[i],
+                                map_to(smem_u32(&task_full[slot]), 1));
+                s_task[slot] = t;
+                mbar_arrive(smem_u32(&task_full[slot]));
                 if (t.stack == kEnd) break;
             }
         }
         __syncwarp();
     } else if (warp == 3) {
         // ---- brings what the epilogue adds ----
-        uint32_t g = 0;  // slots filled
+        fence_async_proxy();  // (X of the kernel before)
+        uint32_t chunk = 0, phases = ~0u;  // chunks so far; by group: its empty slot's phase to wait for
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
             bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
@@ -761,32 +787,32 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             __syncwarp();
             if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
-            if (!u.some || !u.ins) continue;
-            fence_async_proxy();  // (other SMs' stores, by TMA)
             const CUtensorMap* src = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
                                      (u.sym ? static_cast<int>(kMapA) : kMapLo + (t.step() & 1 ? kMapX1 : kMapX0));
-            for (uint32_t i = 0; i < u.chunks * u.ins; ++i, ++g) {
-                const uint32_t b = g % kNsIn;
-                ok = warp_wait(smem_u32(&in_empty[b]), (g / kNsIn + 1) & 1, &s_err);
+            for (uint32_t i = 0; u.some && ok && i < u.chunks * u.ins; ++i) {
+                const uint32_t c = u.ins == 2 ? i >> 1 : i, g = (chunk + c) % kNsGroups;
+                ok = warp_wait(smem_u32(&in_empty[g]), phases >> g & 1u, &s_err);
                 if (!ok) break;
+                phases ^= 1u << g;
                 if (elect_one()) {
-                    const uint32_t bar = smem_u32(&in_full[b]);
+                    const uint32_t bar = smem_u32(&in_full[g]);
                     mbar_expect_tx(bar, kNsSlotBytes);
-                    tma_load(in_slots + b * kNsSlotBytes, src + (u.ins == 2 && (i & 1) ? kMapLo : 0), bar,
-                             u.col0 + (u.ins == 2 ? i >> 1 : i) * 64, u.row0, t.index);
+                    tma_load(in_slots + g * kNsSlotBytes, src + (u.ins == 2 && (i & 1) ? kMapLo : 0), bar,
+                             u.col0 + c * 64, u.row0, t.index);
                 }
                 __syncwarp();
             }
             if (!ok) break;
+            if (u.some) chunk += u.chunks;
         }
         if (*reinterpret_cast<volatile int*>(&s_err))
             // copies in flight land before the CTA may end
-            for (uint32_t j = g > kNsIn ? g - kNsIn : 0; j < g; ++j)
-                bar_wait(smem_u32(&in_full[j % kNsIn]), (j / kNsIn) & 1, &s_drain_err);
+            for (uint32_t g = 0; g < kNsGroups; ++g)
+                bar_wait(smem_u32(&in_full[g]), phases >> g & 1u, &s_drain_err);
         __syncwarp();
     } else if (warp == 4) {
         // ---- stores what it makes ----
-        uint32_t g = 0;  // buffers stored
+        uint32_t chunk = 0, phases = 0;  // chunks so far; by group: its full buffer's phase to wait for
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
             bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
@@ -796,147 +822,163 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             __syncwarp();
             if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
-            // (the last product's result leaves with the arithmetic)
-            if (!u.some || t.kind() == kNsLast) continue;
+            if (!u.some) continue;
+            const bool last = t.kind() == kNsLast;
             const CUtensorMap* dst = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
                                      (t.kind() == kNsXXt ? kMapA
                                       : u.sym            ? kMapB
                                       : t.step() & 1     ? kMapX0
                                                          : kMapX1);
             const uint32_t units = u.chunks * u.outs;
-            for (uint32_t i = 0; i < units; ++i, ++g) {
-                const uint32_t b = g % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
-                ok = warp_wait(smem_u32(&out_full[b]), (g / kNsOut) & 1, &s_err);
+            for (uint32_t i = 0; i < units; ++i) {
+                const uint32_t c = u.outs == 2 ? i >> 1 : i, g = (chunk + c) % kNsGroups;
+                const uint32_t at = out_slots + g * 2 * kNsSlotBytes;
+                ok = warp_wait(smem_u32(&out_full[g]), phases >> g & 1u, &s_err);
                 if (!ok) break;
+                phases ^= 1u << g;
                 if (elect_one()) {
-                    const uint32_t x = u.col0 + (u.outs == 2 ? i >> 1 : i) * 64;
-                    const bool image_only = u.outs == 2 && (i & 1);
-                    if (!image_only) {
-                        tma_store(dst, at, x, u.row0, t.index);
-                        if (u.lo) tma_store(dst + kMapLo, at + kNsSlotBytes, x, u.row0, t.index);
-                    }
-                    if (u.mirror && (image_only || !u.three)) {
-                        const uint32_t image = at + (image_only ? 0 : kNsSlotBytes);
-                        for (uint32_t h = 0; h < 2 && u.row0 + h * 64 < t.m; ++h) {
-                            tma_store(dst + kMap64, image + h * kNsBoxBytes, u.row0 + h * 64, x, t.index);
-                            if (image_only)
-                                tma_store(dst + kMapLo + kMap64, at + kNsSlotBytes + h * kNsBoxBytes,
-                                          u.row0 + h * 64, x, t.index);
+                    if (last) {  // (the result has left with the arithmetic)
+                        mbar_arrive(smem_u32(&out_empty[g]));
+                    } else {
+                        const uint32_t x = u.col0 + c * 64;
+                        const bool image_only = u.outs == 2 && (i & 1);
+                        if (!image_only) {
+                            tma_store(dst, at, x, u.row0, t.index);
+                            if (u.lo) tma_store(dst + kMapLo, at + kNsSlotBytes, x, u.row0, t.index);
                         }
-                    }
-                    bulk_commit();
-                    // a buffer is free once its stores have read it: seen when the next one's are
-                    // on their way, or now where the next chunk takes both buffers or none comes
-                    const bool at_once = i + 1 == units || (u.outs == 2 && (i & 1));
-                    const uint32_t other = smem_u32(&out_empty[(g + kNsOut - 1) % kNsOut]);
-                    if (at_once) {
-                        bulk_wait_read<0>();
-                        if (i > 0) mbar_arrive(other);
-                        mbar_arrive(smem_u32(&out_empty[b]));
-                    } else if (i > 0 && u.outs == 1) {
-                        bulk_wait_read<1>();
-                        mbar_arrive(other);
-                    }
-                    if (i + 1 == units) {
-                        bulk_wait_all();  // this tile's stores, before it counts as done
-                        fence_async_proxy();
-                        __threadfence();
-                        red_release_add1(a.done + t.matrix);
+                        if (u.mirror && (image_only || !u.three)) {
+                            const uint32_t image = at + (image_only ? 0 : kNsSlotBytes);
+                            for (uint32_t h = 0; h < 2 && u.row0 + h * 64 < t.m; ++h) {
+                                tma_store(dst + kMap64, image + h * kNsBoxBytes, u.row0 + h * 64, x, t.index);
+                                if (image_only)
+                                    tma_store(dst + kMapLo + kMap64, at + kNsSlotBytes + h * kNsBoxBytes,
+                                              u.row0 + h * 64, x, t.index);
+                            }
+                        }
+                        bulk_commit();
+                        // a buffer is free once its stores have read it: seen when the other group's
+                        // are on their way, or now where it is the same group's turn again or nobody's
+                        const bool at_once = u.outs == 2 || i + 1 == units;
+                        if (i > 0 && u.outs == 1) {
+                            if (at_once) bulk_wait_read<0>();
+                            else bulk_wait_read<1>();
+                            mbar_arrive(smem_u32(&out_empty[(g + 1) % kNsGroups]));
+                        }
+                        if (at_once) {
+                            bulk_wait_read<0>();
+                            mbar_arrive(smem_u32(&out_empty[g]));
+                        }
+                        if (i + 1 == units) {
+                            bulk_wait_all();  // this tile's stores, before it counts as done
+                            fence_async_proxy();
+                            __threadfence();
+                            red_release_add1(a.done + t.matrix);
+                        }
                     }
                 }
                 __syncwarp();
             }
             if (!ok) break;
+            chunk += u.chunks;
         }
         __syncwarp();
     } else {
-        // ---- arithmetic: sixteen warps, each 32 rows of 16 columns of a chunk ----
-        const uint32_t mw = warp - kMathWarp, quad = warp & 3, part = mw >> 2;
+        // ---- arithmetic: two groups of four warps; a warp has 32 rows of its group's chunks ----
+        const uint32_t quad = warp & 3, group = (warp - kMathWarp) >> 2;
         const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
-        uint32_t gi = 0, go = 0;                 // slots taken, buffers made
+        const uint32_t in_slot = in_slots + group * kNsSlotBytes, at = out_slots + group * 2 * kNsSlotBytes;
+        const uint32_t in_bar = smem_u32(&in_full[group]), in_free = smem_u32(&in_empty[group]);
+        const uint32_t out_bar = smem_u32(&out_full[group]), out_free = smem_u32(&out_empty[group]);
+        uint32_t chunk = 0, in_phase = 0, out_phase = 1;
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            if (!warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
             const NsTask t = s_task[slot];
-            const bool end = ok && t.stack == kEnd;
+            if (t.stack == kEnd) break;
+            __syncwarp();
+            if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
             const bool last = t.kind() == kNsLast;
             Target target{};
-            if (ok && !end) {
-                if (last) {
-                    const NsStack& s = a.stacks[t.stack];
-                    target.dst = kMuon ? s.param : s.dst;
-                    target.master = s.master;
-                    target.ema = s.mom + step.ema_delta;
-                    target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
-                                        : static_cast<uint64_t>(t.index) * s.dst_mat;
-                    target.pitch = kMuon ? s.cols : s.dst_row;
-                    target.lr_wd = __fmul_rn(step.lr, s.wd);
-                    target.lr_s = __fmul_rn(step.lr, s.factor);
-                }
-                ok = warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err);
+            if (last) {
+                const NsStack& s = a.stacks[t.stack];
+                target.dst = kMuon ? s.param : s.dst;
+                target.master = s.master;
+                target.ema = s.mom + step.ema_delta;
+                target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
+                                    : static_cast<uint64_t>(t.index) * s.dst_mat;
+                target.pitch = kMuon ? s.cols : s.dst_row;
+                target.lr_wd = __fmul_rn(step.lr, s.wd);
+                target.lr_s = __fmul_rn(step.lr, s.factor);
             }
-            if (!ok) s_cfail[q & 1] = 1;
-            consumers_sync<kMath>();  // all go on, or none
-            if (s_cfail[q & 1] || end) break;
-            if (mw == 0 && lane == 0) release_task(slot);
-            tc_fence_after();
             const float ca = a.coef[t.step()][0], cb = a.coef[t.step()][1], cc = a.coef[t.step()][2];
             const bool two = u.three && (t.kind() == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
-            // v = fv accumulator + fx addend (+ fd on the diagonal)
+            // v = fv accumulator + fx addend (+ ca on the diagonal)
             const float fx = u.sym ? cb : ca;
             const float fv = t.kind() == kNsXXt ? kNsScaleA / (t.sx * t.sx)
                                                 : t.kind() == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
-            for (uint32_t c = 0; c < u.chunks; ++c) {
-                float v[16];
-                const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64 + part * 16;
+            if (!warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err)) break;
+            tc_fence_after();
+            bool ok = true, held = true;
+            for (uint32_t c = 0; c < u.chunks && ok; ++c) {
+                if (((u.some ? chunk : 0) + c) % kNsGroups != group) continue;
+                const uint32_t col = u.col0 + c * 64;
+                float v[64];
+                const uint32_t acc = tmem + buf * kNsTileN + ((quad * 32u) << 16) + c * 64;
                 __syncwarp();
-                tmem_ld16(acc, v);
+                tmem_ld32(acc, v);
+                tmem_ld32(acc + 32, v + 32);
                 if (two) {
-                    float w[16];
-                    tmem_ld16(acc + kNsTileN / 2, w);
+                    float w[32];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] += w[j];
+                    for (int h = 0; h < 2; ++h) {
+                        tmem_ld32(acc + kNsTileN / 2 + h * 32, w);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[h * 32 + j] += w[j];
+                    }
                 }
-                if (c + 1 == u.chunks) {
+                if (c + kNsGroups >= u.chunks) {  // the group's last of this tile
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+                    held = false;
                 }
                 if (!u.some) continue;
-                const uint32_t col = u.col0 + c * 64;
-                // (a wait that runs out has set s_err: the next tile ends the loop)
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] *= fv;
-                for (uint32_t i = 0; i < u.ins; ++i, ++gi) {
-                    const uint32_t b = gi % kNsIn;
-                    warp_wait(smem_u32(&in_full[b]), (gi / kNsIn) & 1, &s_err);
-                    slot_add(in_slots + b * kNsSlotBytes, trow, part, fx, v);
+                for (int j = 0; j < 64; ++j) v[j] *= fv;
+                for (uint32_t i = 0; i < u.ins && ok; ++i) {
+                    ok = warp_wait(in_bar, in_phase, &s_err);
+                    in_phase ^= 1;
+                    slot_add(in_slot, trow, fx, v);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&in_empty[b]));
+                    if (lane == 0) mbar_arrive(in_free);
                 }
+                if (t.kind() == kNsAA) {
+                    const uint32_t diag = u.row0 + trow - col;  // (no match: no column)
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) v[j] += diag == static_cast<uint32_t>(j) ? ca * kNsScaleA : 0.0f;
+                }
+                ok = ok && warp_wait(out_free, out_phase, &s_err);
+                if (!ok) break;
+                out_phase ^= 1;
                 if (last) {
-                    // through shared memory as floats, so that the result is written row by row of
-                    // the caller's matrix; in the two out buffers by turns, between which the
-                    // barrier keeps the warps within a chunk of each other
-                    const uint32_t b = c % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
-                    const uint32_t use = go + (go + b) % kNsOut;  // (the stores before have left it)
-                    warp_wait(smem_u32(&out_empty[b]), (use / kNsOut + 1) & 1, &s_err);
+                    // through shared memory as floats, the warp's own 32 rows, so that the result is
+                    // written along the rows of the caller's matrix
                     const float f = 1.0f / t.sx;
                     float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) fs[float_at(trow, part * 16 + j)] = v[j] * f;
-                    consumers_sync<kMath>();
-                    // a warp's eight rows of the chunk (columns, where the matrix is transposed)
+                    for (int j = 0; j < 64; ++j) fs[float_at(trow, j)] = v[j] * f;
+                    __syncwarp();
 #pragma unroll 1
-                    for (uint32_t k = 0; k < 2; ++k) {
+                    for (uint32_t k = 0; k < 64; k += 8) {
                         uint64_t to[8];
                         float o[8];
                         uint32_t valid = 0;
 #pragma unroll
                         for (uint32_t l = 0; l < 8; ++l) {
-                            const uint32_t rr = t.transposed() ? lane + 32 * (l & 3) : mw * 8 + k * 4 + (l >> 1);
-                            const uint32_t rc = t.transposed() ? mw * 4 + k * 2 + (l >> 2) : lane + 32 * (l & 1);
+                            const uint32_t e = k + l;  // a row's half, or a column
+                            const uint32_t rr = t.transposed() ? trow : quad * 32 + (e >> 1);
+                            const uint32_t rc = t.transposed() ? e : lane + 32 * (e & 1);
                             const uint32_t y = u.row0 + rr, x = col + rc;
                             to[l] = target.base + (t.transposed() ? x * target.pitch + y : y * target.pitch + x);
                             o[l] = fs[float_at(rr, rc)];
@@ -944,49 +986,54 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         }
                         put_result<kDst>(step, target, a.ema != 0, to, o, valid);
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(out_bar);
                     continue;
                 }
-                const uint32_t b = go % kNsOut, at = out_slots + b * 2 * kNsSlotBytes;
-                if (t.kind() == kNsAA) {
-                    const uint32_t diag = u.row0 + trow - (col + part * 16);  // (no match: no column)
+                // hi and lo; the mirror image in the second slot, or (hi and lo) in the buffer after them
+                uint32_t h[32], l[32];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] += diag == static_cast<uint32_t>(j) ? ca * kNsScaleA : 0.0f;
+                for (int j = 0; j < 32; ++j) split2(v[2 * j], v[2 * j + 1], h[j], l[j]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t o = slot_at(trow, j);
+                    sts128(at + o, make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]));
+                    if (u.lo)
+                        sts128(at + kNsSlotBytes + o, make_uint4(l[4 * j], l[4 * j + 1], l[4 * j + 2], l[4 * j + 3]));
                 }
-                // hi and lo; the mirror image in the second slot, or in the next buffer
-                warp_wait(smem_u32(&out_empty[b]), (go / kNsOut + 1) & 1, &s_err);
-                const uint32_t b1 = (go + 1) % kNsOut;
-                const uint32_t image = u.outs == 2 ? out_slots + b1 * 2 * kNsSlotBytes : at + kNsSlotBytes;
-                if (u.outs == 2) warp_wait(smem_u32(&out_empty[b1]), ((go + 1) / kNsOut + 1) & 1, &s_err);
+                if (u.mirror) {
+                    uint32_t image = at + kNsSlotBytes;
+                    if (u.outs == 2) {
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(out_bar);
+                        ok = warp_wait(out_free, out_phase, &s_err);
+                        if (!ok) break;
+                        out_phase ^= 1;
+                        image = at;
+                    }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t h[4], l[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) split2(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], h[e], l[e]);
-                    const uint32_t o = slot_at(trow, part * 2 + j);
-                    sts128(at + o, make_uint4(h[0], h[1], h[2], h[3]));
-                    if (u.lo) sts128(at + kNsSlotBytes + o, make_uint4(l[0], l[1], l[2], l[3]));
-                    if (u.mirror) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t m0 = mirror_at(trow, part * 16 + j * 8 + 2 * e);
-                            const uint32_t m1 = mirror_at(trow, part * 16 + j * 8 + 2 * e + 1);
-                            sts16(image + m0, h[e] & 0xFFFFu);
-                            sts16(image + m1, h[e] >> 16);
-                            if (u.lo) {
-                                sts16(image + kNsSlotBytes + m0, l[e] & 0xFFFFu);
-                                sts16(image + kNsSlotBytes + m1, l[e] >> 16);
-                            }
+                    for (int j = 0; j < 32; ++j) {
+                        const uint32_t m0 = mirror_at(trow, 2 * j), m1 = mirror_at(trow, 2 * j + 1);
+                        sts16(image + m0, h[j] & 0xFFFFu);
+                        sts16(image + m1, h[j] >> 16);
+                        if (u.lo) {
+                            sts16(image + kNsSlotBytes + m0, l[j] & 0xFFFFu);
+                            sts16(image + kNsSlotBytes + m1, l[j] >> 16);
                         }
                     }
                 }
                 fence_async_shared();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(smem_u32(&out_full[b]));
-                    if (u.outs == 2) mbar_arrive(smem_u32(&out_full[b1]));
-                }
-                go += u.outs;
+                if (lane == 0) mbar_arrive(out_bar);
             }
+            if (!ok) break;
+            if (held) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+            }
+            if (u.some) chunk += u.chunks;
         }
     }
     tc_fence_before();

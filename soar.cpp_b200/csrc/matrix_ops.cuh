@@ -47,16 +47,15 @@ constexpr int kNsTileN = 256;
 constexpr int kNsRows = 128;   // a CTA's share of the rows
 constexpr int kNsTileK = 64;   // depth of one stage
 constexpr int kNsStages = 4;
-constexpr int kNsMathWarps = 16;  // four to a quarter of the rows: a chunk's latencies overlap
+constexpr int kNsMathWarps = 8;  // two groups of four, each with every other chunk of 64 columns
 // operand copies, products, hand-out, epilogue's copies in, and out, arithmetic
 constexpr int kNsThreads = (5 + kNsMathWarps) * 32;
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
 constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
 constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue: 128 rows of 64 fp16
-constexpr int kNsIn = 2;   // slots of what it adds
-constexpr int kNsOut = 2;  // buffers of two slots of what it makes
-constexpr size_t kNsSmemBytes = static_cast<size_t>(kNsStages) * kNsStageBytes +
-                                (kNsIn + 2 * kNsOut) * kNsSlotBytes + 1024;
+constexpr int kNsGroups = 2;  // each with a slot of what it adds, and two of what it makes
+constexpr size_t kNsSmemBytes =
+    static_cast<size_t>(kNsStages) * kNsStageBytes + 3 * kNsGroups * kNsSlotBytes + 1024;
 
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
