@@ -523,13 +523,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
     constexpr int kRing = 4;  // tasks handed out ahead
-    constexpr int kMathWarp = 5;            // the first of them
+    constexpr int kMathWarp = 6;            // the first of them
     constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t in_full[kNsGroups], in_empty[kNsGroups], out_full[kNsGroups],
-        out_empty[kNsGroups];
+    __shared__ __align__(8) uint64_t in_full[kNsGroups], in_empty[kNsGroups], out_empty[kNsGroups];
+    __shared__ __align__(8) uint64_t out_full[2][kNsGroups];  // of even and of odd tiles
     __shared__ __align__(8) uint64_t drain_bar;
     __shared__ __align__(16) NsTask s_task[kRing];
     __shared__ uint32_t s_tmem;
@@ -557,13 +557,13 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         for (int i = 0; i < kNsGroups; ++i) {
             mbar_init(smem_u32(&in_full[i]), 1);
             mbar_init(smem_u32(&in_empty[i]), kNsMathWarps / kNsGroups);
-            mbar_init(smem_u32(&out_full[i]), kNsMathWarps / kNsGroups);
+            for (int odd = 0; odd < 2; ++odd) mbar_init(smem_u32(&out_full[odd][i]), kNsMathWarps / kNsGroups);
             mbar_init(smem_u32(&out_empty[i]), 1);
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            // four readers and the arithmetic here, three and the arithmetic in the other CTA
-            mbar_init(smem_u32(&task_empty[i]), 7 + 2 * kNsMathWarps);
+            // five readers and the arithmetic here, four and the arithmetic in the other CTA
+            mbar_init(smem_u32(&task_empty[i]), 9 + 2 * kNsMathWarps);
             if (rank == 1) mbar_expect_tx(smem_u32(&task_full[i]), sizeof(NsTask));
         }
         mbar_init(smem_u32(&drain_bar), 1);
@@ -810,8 +810,10 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             for (uint32_t g = 0; g < kNsGroups; ++g)
                 bar_wait(smem_u32(&in_full[g]), phases >> g & 1u, &s_drain_err);
         __syncwarp();
-    } else if (warp == 4) {
-        // ---- stores what it makes ----
+    } else if (warp < kMathWarp) {
+        // ---- two warps, by turns, store what a tile makes: one waits for its tile's stores to
+        // land while the other issues the next one's ----
+        const uint32_t odd = warp & 1u;
         uint32_t chunk = 0, phases = 0;  // chunks so far; by group: its full buffer's phase to wait for
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
@@ -823,6 +825,10 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
             if (!u.some) continue;
+            if ((q & 1) != odd) {
+                chunk += u.chunks;
+                continue;
+            }
             const bool last = t.kind() == kNsLast;
             const CUtensorMap* dst = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
                                      (t.kind() == kNsXXt ? kMapA
@@ -833,7 +839,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             for (uint32_t i = 0; i < units; ++i) {
                 const uint32_t c = u.outs == 2 ? i >> 1 : i, g = (chunk + c) % kNsGroups;
                 const uint32_t at = out_slots + g * 2 * kNsSlotBytes;
-                ok = warp_wait(smem_u32(&out_full[g]), phases >> g & 1u, &s_err);
+                ok = warp_wait(smem_u32(&out_full[odd][g]), phases >> g & 1u, &s_err);
                 if (!ok) break;
                 phases ^= 1u << g;
                 if (elect_one()) {
@@ -888,7 +894,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
         const uint32_t in_slot = in_slots + group * kNsSlotBytes, at = out_slots + group * 2 * kNsSlotBytes;
         const uint32_t in_bar = smem_u32(&in_full[group]), in_free = smem_u32(&in_empty[group]);
-        const uint32_t out_bar = smem_u32(&out_full[group]), out_free = smem_u32(&out_empty[group]);
+        const uint32_t out_free = smem_u32(&out_empty[group]);
         uint32_t chunk = 0, in_phase = 0, out_phase = 1;
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
@@ -899,6 +905,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
             const bool last = t.kind() == kNsLast;
+            const uint32_t out_bar = smem_u32(&out_full[q & 1][group]);
             Target target{};
             if (last) {
                 const NsStack& s = a.stacks[t.stack];

@@ -48,8 +48,8 @@ constexpr int kNsRows = 128;   // a CTA's share of the rows
 constexpr int kNsTileK = 64;   // depth of one stage
 constexpr int kNsStages = 4;
 constexpr int kNsMathWarps = 8;  // two groups of four, each with every other chunk of 64 columns
-// operand copies, products, hand-out, epilogue's copies in, and out, arithmetic
-constexpr int kNsThreads = (5 + kNsMathWarps) * 32;
+// operand copies, products, hand-out, epilogue's copies in, and out (two), arithmetic
+constexpr int kNsThreads = (6 + kNsMathWarps) * 32;
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
 constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
 constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue: 128 rows of 64 fp16
