@@ -74,7 +74,7 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     // the product kernel of the run before is done: its counters start at 0 again
     for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < a.n_matrices; i += gridDim.x * kThreads)
         a.done[i] = 0u;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.next = 0u;
+    if (blockIdx.x == 0 && threadIdx.x < 2) a.next[threadIdx.x] = 0u;
     StepCoeffs k{1.0f, 1.0f, 0.0f, 1.0f, 1};
     if constexpr (kMuon) {
         if (threadIdx.x == 0) s_d = decide_step(step, ctl);
@@ -139,6 +139,25 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     }
 }
 
+// Two values as e5m2, the first in the low byte.
+__device__ __forceinline__ uint32_t e5m2x2(float a, float b) {
+    uint16_t d;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(d) : "f"(b), "f"(a));
+    return d;
+}
+
+// X's element as hi and lo, lo in 16 or in 8 bits.
+__device__ __forceinline__ void put_x(const NsStack& s, uint64_t matrix, uint64_t at, float v) {
+    __half hi, lo;
+    split_half(v, hi, lo);
+    s.x[0][matrix + at] = hi;
+    if (s.panel)
+        reinterpret_cast<uint8_t*>(s.xl[0])[matrix + at] =
+            static_cast<uint8_t>(e5m2x2((v - __half2float(hi)) * kPanelLoScale, 0.0f));
+    else
+        s.xl[0][matrix + at] = lo;
+}
+
 template <int kSrc>
 __global__ void __launch_bounds__(kThreads)
 k_matrix_split(MatrixArgs a) {
@@ -159,8 +178,7 @@ k_matrix_split(MatrixArgs a) {
         const uint32_t lc = threadIdx.x % kPrepTile, lr = threadIdx.x / kPrepTile;
         const uint32_t c = t.tc * kPrepTile + lc;
         const float inv = a.inv[s.first + t.index];
-        __half* xh = s.x[0] + static_cast<uint64_t>(t.index) * s.m * s.ldx;
-        __half* xl = s.xl[0] + static_cast<uint64_t>(t.index) * s.m * s.ldx;
+        const uint64_t matrix = static_cast<uint64_t>(t.index) * s.m * s.ldx;
 #pragma unroll 4
         for (uint32_t i = 0; i < kPrepTile; i += kThreads / kPrepTile) {
             const uint32_t r = t.tr * kPrepTile + lr + i;
@@ -177,11 +195,7 @@ k_matrix_split(MatrixArgs a) {
             if (s.transposed) {
                 s_t[lr + i][lc] = v;
             } else {
-                __half hi, lo;
-                split_half(v, hi, lo);
-                const uint64_t at = static_cast<uint64_t>(r) * s.ldx + c;
-                xh[at] = hi;
-                xl[at] = lo;
+                put_x(s, matrix, static_cast<uint64_t>(r) * s.ldx + c, v);
             }
         }
         if (s.transposed) {
@@ -191,11 +205,7 @@ k_matrix_split(MatrixArgs a) {
             for (uint32_t i = 0; i < kPrepTile; i += kThreads / kPrepTile) {
                 const uint32_t xc = t.tc * kPrepTile + lr + i;  // X's row
                 if (r >= s.rows || xc >= s.cols) continue;
-                __half hi, lo;
-                split_half(s_t[lc][lr + i], hi, lo);
-                const uint64_t at = static_cast<uint64_t>(xc) * s.ldx + r;
-                xh[at] = hi;
-                xl[at] = lo;
+                put_x(s, matrix, static_cast<uint64_t>(xc) * s.ldx + r, s_t[lc][lr + i]);
             }
             __syncthreads();
         }
@@ -456,6 +466,16 @@ __device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, float f, f
             v[j * 8 + 2 * e + 1] = __fmaf_rn(f, x.y, v[j * 8 + 2 * e + 1]);
         }
     }
+}
+
+// Byte offset of sixteen columns (group j of 4) of a row of a slot of 8-bit lo:
+// rows of 64 bytes, 64-byte swizzle.
+__device__ __forceinline__ uint32_t lo8_at(uint32_t row, uint32_t j) {
+    return row * 64u + ((j ^ (row >> 1 & 3u)) << 4);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Two values as packed fp16 (hi), and what is left of them (lo).
@@ -1058,6 +1078,546 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// ----------------------------------------------------- one pair, one matrix ---
+// k_panel: the whole iteration of a matrix with at most 256 rows (of X) by one
+// pair of CTAs, 128 rows each. B (fp16) stays in shared memory as the first
+// operand of B X. X goes by in blocks of 128 columns, read once and written once
+// per iteration through the L2 cache; the block's new hi part, in shared memory
+// on its way out, is at once the operand of its share of the next A = X X^T,
+// which adds up in TMEM. Between two passes over X, A passes through shared
+// memory for A A. So a matrix waits for nobody, and its 15 products cost two
+// exchanges with the L2 cache per iteration. (In k_ns, tiles of such matrices
+// spent most of their time waiting for one another: 64 matrices of 256 x 1024
+// took 276 us there.)
+//
+// Shared memory per CTA: four slots of 128 rows x 64 fp16 for A, or for the hi
+// parts of two blocks; four for B; two blocks of X (64 columns of all rows); four
+// slots of lo. TMEM: two accumulators of 128 columns (A A: both), one of 256 (A).
+template <int kDst>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPanelThreads, 1)
+k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
+    constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
+    constexpr int kMathWarp = 4, kMathWarps = 8;
+    constexpr uint32_t kEnd = 0xFFFFFFFFu;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t mat_full[2], mat_empty[2], mat_done;
+    __shared__ __align__(8) uint64_t g0_full[4], g0_empty[4];       // X's slots of the first A
+    __shared__ __align__(8) uint64_t x_full[2], x_empty[2], x_done;  // blocks of X; X of an iteration written
+    __shared__ __align__(8) uint64_t lo_full[4], lo_empty[4];
+    __shared__ __align__(8) uint64_t hi_full[4], hi_out[4], hi_empty[4];  // for products, for stores; free
+    __shared__ __align__(8) uint64_t d_full[2], d_empty[2], a_full, aa_full, a_ready, b_ready, drain_bar;
+    __shared__ __align__(16) uint4 s_mat[2];  // stack, matrix of the stack, m, n
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_err, s_drain_err;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+    if constexpr (kMuon) {
+        if (a.step->skip) return;
+    }
+    const uint32_t rank = blockIdx.x & 1u;  // 0 leads the pair
+    const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t a_slots = smem, b_slots = smem + 4 * kNsSlotBytes;
+    const uint32_t x_blocks = b_slots + 4 * kNsSlotBytes, lo_slots = x_blocks + 2 * kPanelBlockBytes;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&mat_full[i]), 1);
+            // copies in, products, copies out, arithmetic here; all but the products there
+            mbar_init(smem_u32(&mat_empty[i]), 5 + 2 * kMathWarps);
+            mbar_init(smem_u32(&x_full[i]), 1);
+            mbar_init(smem_u32(&x_empty[i]), 1);
+            mbar_init(smem_u32(&d_full[i]), 1);
+            mbar_init(smem_u32(&d_empty[i]), 2 * kMathWarps);
+            if (rank == 1) mbar_expect_tx(smem_u32(&mat_full[i]), sizeof(uint4));
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(smem_u32(&g0_full[i]), 1);
+            mbar_init(smem_u32(&g0_empty[i]), 1);
+            mbar_init(smem_u32(&lo_full[i]), 1);
+            mbar_init(smem_u32(&lo_empty[i]), 1);
+            mbar_init(smem_u32(&hi_full[i]), kMathWarps);      // both CTAs' group of four warps
+            mbar_init(smem_u32(&hi_out[i]), kMathWarps / 2);
+            mbar_init(smem_u32(&hi_empty[i]), 2);              // its product, its store
+        }
+        mbar_init(smem_u32(&mat_done), kMathWarps);
+        mbar_init(smem_u32(&x_done), 2);
+        mbar_init(smem_u32(&a_full), 1);
+        mbar_init(smem_u32(&aa_full), 1);
+        mbar_init(smem_u32(&a_ready), 2 * kMathWarps);
+        mbar_init(smem_u32(&b_ready), 2 * kMathWarps);
+        mbar_init(smem_u32(&drain_bar), 1);
+        s_err = s_drain_err = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_u32(&s_tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t steps = static_cast<uint32_t>(a.steps);
+    auto release_mat = [&](uint32_t slot) { mbar_arrive_cluster(map_to(smem_u32(&mat_empty[slot]), 0)); };
+    auto lead = [&](uint64_t* bar) { return map_to(smem_u32(bar), 0); };
+    // Copies of this CTA's that landed or not when something failed are waited for by this barrier's
+    // owner below; nothing else may touch shared memory after that.
+
+    if (warp == 0) {
+        // ---- copies in ----
+        fence_async_proxy();  // (X of the kernel before)
+        uint32_t g0_phase = 0xF, x_phase = 3, lo_phase = 0xF, done_phase = 0;
+        const uint32_t lead_g0 = uniform(lead(&g0_full[0])), lead_x = uniform(lead(&x_full[0]));
+        bool ok = true;
+        for (uint32_t q = 0; ok; ++q) {
+            const uint32_t slot = q & 1;
+            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            if (!ok) break;
+            const uint32_t stack = uniform(s_mat[slot].x), index = uniform(s_mat[slot].y);
+            const uint32_t m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 1) mbar_expect_tx(smem_u32(&mat_full[slot]), sizeof(uint4));
+                release_mat(slot);
+            }
+            if (stack == kEnd) break;
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(stack) * kMapsPerStack;
+            const uint32_t kb = (m + 63) / 64, chunks = (n + 63) / 64, blocks = (chunks + 1) / 2;
+            // the matrix before is done with the slots
+            if (q > 0) ok = warp_wait(smem_u32(&mat_done), (q + 1) & 1, &s_err);
+            for (uint32_t c = 0; c < chunks && ok; ++c) {
+                const uint32_t b = c & 3;
+                ok = warp_wait(smem_u32(&g0_empty[b]), g0_phase >> b & 1, &s_err);
+                if (!ok) break;
+                g0_phase ^= 1u << b;
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(smem_u32(&g0_full[b]), 2 * kNsSlotBytes);
+                    tma_load_pair(a_slots + b * kNsSlotBytes, maps + kMapX0, lead_g0 + b * 8, c * 64, rank * kNsRows, index);
+                }
+                __syncwarp();
+            }
+            for (uint32_t it = 0; it < steps && ok; ++it) {
+                const CUtensorMap* x = maps + (it & 1 ? kMapX1 : kMapX0);
+                if (it > 0) {
+                    // both CTAs' stores of the iteration before have landed
+                    ok = warp_wait_cluster(smem_u32(&x_done), done_phase, &s_err);
+                    done_phase ^= 1;
+                    fence_async_proxy();
+                }
+                for (uint32_t j = 0; j < blocks && ok; ++j) {
+                    const uint32_t b = j & 1;
+                    ok = warp_wait(smem_u32(&x_empty[b]), x_phase >> b & 1, &s_err);
+                    if (!ok) break;
+                    x_phase ^= 1u << b;
+                    if (elect_one()) {
+                        if (rank == 0) mbar_expect_tx(smem_u32(&x_full[b]), 2 * kb * kNsBoxBytes);
+                        for (uint32_t k = 0; k < kb; ++k)
+                            tma_load_pair(x_blocks + b * kPanelBlockBytes + k * kNsBoxBytes, x + kMapN + kMap64,
+                                          lead_x + b * 8, 0, k * 64, 2 * j + rank, index);
+                    }
+                    __syncwarp();
+                    for (uint32_t g = 0; g < 2 && 2 * j + g < chunks && ok; ++g) {
+                        const uint32_t l = 2 * b + g;
+                        ok = warp_wait(smem_u32(&lo_empty[l]), lo_phase >> l & 1, &s_err);
+                        if (!ok) break;
+                        lo_phase ^= 1u << l;
+                        if (elect_one()) {
+                            mbar_expect_tx(smem_u32(&lo_full[l]), kPanelLoBytes);
+                            tma_load(lo_slots + l * kPanelLoBytes, x + kMapLo, smem_u32(&lo_full[l]), (2 * j + g) * 64,
+                                     rank * kNsRows, index);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        if (*reinterpret_cast<volatile int*>(&s_err)) {
+            // copies in flight land before the CTA may end
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (rank == 0) bar_wait(smem_u32(&g0_full[i]), g0_phase >> i & 1, &s_drain_err);
+                bar_wait(smem_u32(&lo_full[i]), lo_phase >> i & 1, &s_drain_err);
+            }
+            for (uint32_t i = 0; i < 2 && rank == 0; ++i) bar_wait(smem_u32(&x_full[i]), x_phase >> i & 1, &s_drain_err);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- products, issued by the leader ----
+        uint32_t g0_phase = 0, x_phase = 0, d_phase = 3, hi_phase = 0, a_phase = 0;
+        bool ok = true;
+        const uint32_t acc = uniform(tmem), gram = acc + 256;
+        // one product of 64 columns' depth
+        auto product = [&](uint32_t d, uint32_t first, uint32_t second, bool mn, uint32_t n, bool fresh) {
+            const uint64_t da = operand_desc(first, 16), db = operand_desc(second, mn ? kNsBoxBytes : 16);
+            const uint32_t db_k = mn ? 2048 >> 4 : 32 >> 4;
+            const uint32_t idesc = instr_desc(n, mn);
+            mma_f16(d, da, db, idesc, !fresh);
+#pragma unroll
+            for (uint32_t k = 1; k < 4; ++k) mma_f16(d, da + k * 2, db + k * db_k, idesc, true);
+        };
+        for (uint32_t q = 0; rank == 0 && ok; ++q) {
+            const uint32_t slot = q & 1;
+            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            if (!ok) break;
+            const uint32_t stack = uniform(s_mat[slot].x), m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
+            __syncwarp();
+            if (lane == 0) release_mat(slot);
+            if (stack == kEnd) break;
+            const uint32_t kb = (m + 63) / 64, chunks = (n + 63) / 64, blocks = (chunks + 1) / 2;
+            for (uint32_t c = 0; c < chunks && ok; ++c) {
+                const uint32_t b = c & 3, s = a_slots + b * kNsSlotBytes;
+                ok = warp_wait(smem_u32(&g0_full[b]), g0_phase >> b & 1, &s_err);
+                if (!ok) break;
+                g0_phase ^= 1u << b;
+                tc_fence_after();
+                if (elect_one()) {
+                    product(gram, s, s, false, 256, c == 0);
+                    mma_commit(smem_u32(&g0_empty[b]));
+                    if (c + 1 == chunks) mma_commit(smem_u32(&a_full));
+                }
+                __syncwarp();
+            }
+            for (uint32_t it = 0; it < steps && ok; ++it) {
+                ok = warp_wait_cluster(smem_u32(&a_ready), a_phase, &s_err);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    for (uint32_t k = 0; k < kb; ++k)
+                        product(acc, a_slots + k * kNsSlotBytes, a_slots + k * kNsSlotBytes, false, 256, k == 0);
+                    mma_commit(smem_u32(&aa_full));
+                }
+                __syncwarp();
+                ok = warp_wait_cluster(smem_u32(&b_ready), a_phase, &s_err);
+                if (!ok) break;
+                a_phase ^= 1;
+                // the next A takes block j - 1 while block j's product is under way
+                for (uint32_t j = 0; j <= blocks && ok; ++j) {
+                    const uint32_t b = j & 1;
+                    if (j < blocks) {
+                        ok = warp_wait(smem_u32(&x_full[b]), x_phase >> b & 1, &s_err) &&
+                             warp_wait_cluster(smem_u32(&d_empty[b]), d_phase >> b & 1, &s_err);
+                        if (!ok) break;
+                        x_phase ^= 1u << b;
+                        d_phase ^= 1u << b;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            for (uint32_t k = 0; k < kb; ++k)
+                                product(acc + b * 128, b_slots + k * kNsSlotBytes,
+                                        x_blocks + b * kPanelBlockBytes + k * kNsBoxBytes, true, 128, k == 0);
+                            mma_commit(smem_u32(&x_empty[b]));
+                            mma_commit(smem_u32(&d_full[b]));
+                        }
+                        __syncwarp();
+                    }
+                    if (j == 0 || it + 1 == steps) continue;
+                    for (uint32_t g = 0; g < 2 && 2 * (j - 1) + g < chunks && ok; ++g) {
+                        const uint32_t h = 2 * ((j - 1) & 1) + g, s = a_slots + h * kNsSlotBytes;
+                        ok = warp_wait_cluster(smem_u32(&hi_full[h]), hi_phase >> h & 1, &s_err);
+                        if (!ok) break;
+                        hi_phase ^= 1u << h;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            product(gram, s, s, false, 256, j == 1 && g == 0);
+                            mma_commit(smem_u32(&hi_empty[h]));
+                            if (j == blocks && (g == 1 || 2 * (j - 1) + 1 == chunks)) mma_commit(smem_u32(&a_full));
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0) {
+            if (elect_one()) mma_commit(smem_u32(&drain_bar));
+            bar_wait(smem_u32(&drain_bar), 0, &s_drain_err);
+        }
+        __syncwarp();
+    } else if (warp == 2) {
+        // ---- the leader hands out matrices, to both CTAs ----
+        if (rank == 0 && lane == 0) {
+            for (uint32_t q = 0;; ++q) {
+                const uint32_t slot = q & 1, claim = atomicAdd(a.next + 1, 1u);
+                uint4 w = make_uint4(kEnd, 0, 0, 0);
+                if (claim < a.n_panels) {
+                    const uint2 p = a.panels[claim];
+                    const NsStack& s = a.stacks[p.x];
+                    w = make_uint4(p.x, p.y, s.m, s.n);
+                }
+                if (q >= 2 && !bar_wait_cluster(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
+                st_async_v4(map_to(smem_u32(&s_mat[slot]), 1), w, map_to(smem_u32(&mat_full[slot]), 1));
+                s_mat[slot] = w;
+                mbar_arrive(smem_u32(&mat_full[slot]));
+                if (w.x == kEnd) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 3) {
+        // ---- copies out ----
+        uint32_t out_phase = 0;
+        bool ok = true;
+        for (uint32_t q = 0; ok; ++q) {
+            const uint32_t slot = q & 1;
+            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            if (!ok) break;
+            const uint4 w = s_mat[slot];
+            __syncwarp();
+            if (lane == 0) release_mat(slot);
+            if (w.x == kEnd) break;
+            const CUtensorMap* maps = a.maps + static_cast<uint64_t>(w.x) * kMapsPerStack;
+            const bool some = rank * kNsRows < w.z;  // this CTA has rows
+            const uint32_t chunks = (w.w + 63) / 64;
+            for (uint32_t it = 0; it < steps && ok; ++it) {
+                const CUtensorMap* x = maps + (it & 1 ? kMapX0 : kMapX1);
+                for (uint32_t c = 0; c < chunks; ++c) {
+                    const uint32_t h = c & 3;
+                    ok = warp_wait(smem_u32(&hi_out[h]), out_phase >> h & 1, &s_err);
+                    if (!ok) break;
+                    out_phase ^= 1u << h;
+                    if (elect_one()) {
+                        if (it + 1 == steps) {  // (the result has left with the arithmetic)
+                            mbar_arrive(smem_u32(&lo_empty[h]));
+                        } else {
+                            if (some) {
+                                tma_store(x, a_slots + h * kNsSlotBytes, c * 64, rank * kNsRows, w.y);
+                                tma_store(x + kMapLo, lo_slots + h * kPanelLoBytes, c * 64, rank * kNsRows, w.y);
+                            }
+                            bulk_commit();
+                            // a slot is free once its store has read it: the one before's has when
+                            // this one's is on its way
+                            if (c > 0) {
+                                bulk_wait_read<1>();
+                                mbar_arrive(smem_u32(&hi_empty[(h + 3) & 3]));
+                                mbar_arrive(smem_u32(&lo_empty[(h + 3) & 3]));
+                            }
+                            if (c + 1 == chunks) {
+                                bulk_wait_read<0>();
+                                mbar_arrive(smem_u32(&hi_empty[h]));
+                                mbar_arrive(smem_u32(&lo_empty[h]));
+                                bulk_wait_all();  // all of X has landed
+                                fence_async_proxy();
+                                mbar_arrive_cluster(map_to(smem_u32(&x_done), 0));
+                                mbar_arrive_cluster(map_to(smem_u32(&x_done), 1));
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- arithmetic: two groups of four warps, each with every other 64 columns ----
+        const uint32_t quad = warp & 3, group = (warp - kMathWarp) >> 2;
+        const uint32_t trow = quad * 32 + lane, row = rank * kNsRows + trow;
+        const uint32_t lanes = tmem + ((quad * 32u) << 16);
+        uint32_t a_phase = 0, d_phase = 0, lo_phase = 0, hi_phase = 0, hi_used = 0;
+        bool ok = true;
+        for (uint32_t q = 0; ok; ++q) {
+            const uint32_t slot = q & 1;
+            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            if (!ok) break;
+            const uint4 w = s_mat[slot];
+            __syncwarp();
+            if (lane == 0) release_mat(slot);
+            if (w.x == kEnd) break;
+            const NsStack& s = a.stacks[w.x];
+            const uint32_t m = w.z, n = w.w, kb = (m + 63) / 64, chunks = (n + 63) / 64, blocks = (chunks + 1) / 2;
+            const float sx = s.sx;
+            const bool transposed = s.transposed != 0;
+            Target target{};
+            target.dst = kMuon ? s.param : s.dst;
+            target.master = s.master;
+            target.ema = s.mom + step.ema_delta;
+            target.base = kMuon ? static_cast<uint64_t>(w.y) * s.rows * s.cols : static_cast<uint64_t>(w.y) * s.dst_mat;
+            target.pitch = kMuon ? s.cols : s.dst_row;
+            target.lr_wd = __fmul_rn(step.lr, s.wd);
+            target.lr_s = __fmul_rn(step.lr, s.factor);
+            for (uint32_t it = 0; it < steps && ok; ++it) {
+                const float ca = a.coef[it][0], cb = a.coef[it][1], cc = a.coef[it][2];
+                const bool last = it + 1 == steps;
+                // A, from its accumulator to shared memory (the slots' last blocks have left them)
+                ok = warp_wait(smem_u32(&a_full), a_phase, &s_err);
+                for (uint32_t h = 0; h < 4 && ok; ++h)
+                    if (hi_used >> h & 1) ok = warp_wait(smem_u32(&hi_empty[h]), (hi_phase >> h & 1) ^ 1, &s_err);
+                if (!ok) break;
+                tc_fence_after();
+                for (uint32_t c = group; c < kb; c += 2) {
+                    float v[64];
+                    __syncwarp();
+                    tmem_ld32(lanes + 256 + c * 64, reinterpret_cast<float(&)[32]>(v[0]));
+                    tmem_ld32(lanes + 256 + c * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                    const float f = kNsScaleA / (sx * sx);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) h[e] = pack2(v[8 * j + 2 * e] * f, v[8 * j + 2 * e + 1] * f);
+                        sts128(a_slots + c * kNsSlotBytes + slot_at(trow, j), make_uint4(h[0], h[1], h[2], h[3]));
+                    }
+                }
+                fence_async_shared();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead(&a_ready));
+                // B = a I + b A + c A A
+                ok = warp_wait(smem_u32(&aa_full), a_phase, &s_err);
+                if (!ok) break;
+                a_phase ^= 1;
+                tc_fence_after();
+                for (uint32_t c = group; c < kb; c += 2) {
+                    float v[64];
+                    __syncwarp();
+                    tmem_ld32(lanes + c * 64, reinterpret_cast<float(&)[32]>(v[0]));
+                    tmem_ld32(lanes + c * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                    const float f2 = cc / (kNsScaleA * kNsScaleA), f1 = cb / kNsScaleA;
+                    const uint32_t diag = row - c * 64;  // (no match: no column)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint4 p = lds128(a_slots + c * kNsSlotBytes + slot_at(trow, j));
+                        const __half2* ah = reinterpret_cast<const __half2*>(&p);
+                        uint32_t h[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 x = __half22float2(ah[e]);
+                            const int i = 8 * j + 2 * e;
+                            float y0 = __fmaf_rn(f1, x.x, f2 * v[i]), y1 = __fmaf_rn(f1, x.y, f2 * v[i + 1]);
+                            y0 += diag == static_cast<uint32_t>(i) ? ca : 0.0f;
+                            y1 += diag == static_cast<uint32_t>(i + 1) ? ca : 0.0f;
+                            h[e] = pack2(y0, y1);
+                        }
+                        sts128(b_slots + c * kNsSlotBytes + slot_at(trow, j), make_uint4(h[0], h[1], h[2], h[3]));
+                    }
+                }
+                fence_async_shared();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(lead(&b_ready));
+                // X = B X, block by block
+                for (uint32_t j = 0; j < blocks && ok; ++j) {
+                    const uint32_t b = j & 1, c = 2 * j + group, h = 2 * b + group;
+                    ok = warp_wait(smem_u32(&d_full[b]), d_phase >> b & 1, &s_err);
+                    if (!ok) break;
+                    d_phase ^= 1u << b;
+                    tc_fence_after();
+                    float v[64];
+                    if (c < chunks) {
+                        __syncwarp();
+                        tmem_ld32(lanes + b * 128 + group * 64, reinterpret_cast<float(&)[32]>(v[0]));
+                        tmem_ld32(lanes + b * 128 + group * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(lead(&d_empty[b]));
+                    if (c >= chunks) continue;
+                    ok = warp_wait(smem_u32(&lo_full[h]), lo_phase >> h & 1, &s_err);
+                    if (!ok) break;
+                    lo_phase ^= 1u << h;
+                    const uint32_t lo = lo_slots + h * kPanelLoBytes;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 p = lds128(lo + lo8_at(trow, k));
+                        const uint32_t word[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            // (an e5m2 number is the upper byte of an fp16 one)
+                            const uint32_t lo01 = __byte_perm(word[e], 0, 0x1404), lo23 = __byte_perm(word[e], 0, 0x3424);
+                            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo01));
+                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lo23));
+                            const float f = ca / kPanelLoScale;
+                            float* o = v + 16 * k + 4 * e;
+                            o[0] = __fmaf_rn(f, x.x, o[0]);
+                            o[1] = __fmaf_rn(f, x.y, o[1]);
+                            o[2] = __fmaf_rn(f, y.x, o[2]);
+                            o[3] = __fmaf_rn(f, y.y, o[3]);
+                        }
+                    }
+                    if (last) {
+                        // through shared memory as floats, the warp's own 32 rows, so that the result
+                        // is written along the rows of the caller's matrix (in the group's two slots,
+                        // which nothing else uses by now)
+                        const float f = 1.0f / sx;
+                        float* fs = reinterpret_cast<float*>(
+                            smem_raw + (a_slots - smem_u32(smem_raw) + group * 2 * kNsSlotBytes));
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 64; ++k) fs[float_at(trow, k)] = v[k] * f;
+                        __syncwarp();
+#pragma unroll 1
+                        for (uint32_t k = 0; k < 64; k += 8) {
+                            uint64_t to[8];
+                            float o[8];
+                            uint32_t valid = 0;
+#pragma unroll
+                            for (uint32_t l = 0; l < 8; ++l) {
+                                const uint32_t e = k + l;  // a row's half, or a column
+                                const uint32_t rr = transposed ? trow : quad * 32 + (e >> 1);
+                                const uint32_t rc = transposed ? e : lane + 32 * (e & 1);
+                                const uint32_t y = rank * kNsRows + rr, x = c * 64 + rc;
+                                to[l] = target.base + (transposed ? x * target.pitch + y : y * target.pitch + x);
+                                o[l] = fs[float_at(rr, rc)];
+                                if (y < m && x < n) valid |= 1u << l;
+                            }
+                            put_result<kDst>(step, target, a.ema != 0, to, o, valid);
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&hi_out[h]));
+                        continue;
+                    }
+                    // hi, for its store and for the next A; lo in place of the old one
+                    if (hi_used >> h & 1) ok = warp_wait(smem_u32(&hi_empty[h]), (hi_phase >> h & 1) ^ 1, &s_err);
+                    if (!ok) break;
+                    hi_used |= 1u << h;
+                    hi_phase ^= 1u << h;
+                    uint32_t lo_word[16];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        uint32_t hw[4], lw[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 8 * k + 2 * e;
+                            hw[e] = pack2(v[i], v[i + 1]);
+                            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw[e]));
+                            lw[e] = e5m2x2((v[i] - x.x) * kPanelLoScale, (v[i + 1] - x.y) * kPanelLoScale);
+                        }
+                        sts128(a_slots + h * kNsSlotBytes + slot_at(trow, k), make_uint4(hw[0], hw[1], hw[2], hw[3]));
+                        lo_word[2 * k] = lw[0] | lw[1] << 16;
+                        lo_word[2 * k + 1] = lw[2] | lw[3] << 16;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        sts128(lo + lo8_at(trow, k), make_uint4(lo_word[4 * k], lo_word[4 * k + 1], lo_word[4 * k + 2],
+                                                                lo_word[4 * k + 3]));
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive_cluster(lead(&hi_full[h]));
+                        mbar_arrive(smem_u32(&hi_out[h]));
+                    }
+                }
+            }
+            // the slots are the next matrix's
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&mat_done));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && (s_err | s_drain_err)) {
+        atomicOr(a.err, 1);
+        // the other CTA's copies may still be landing here, or counting on barriers here
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 2000000ull) {}
+    }
+    __syncthreads();
+    cluster_sync();  // the other CTA may use this one's shared memory until it is done too
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
 template <int kSrc>
 cudaError_t launch_prep(const MatrixArgs& a, Ctl* ctl, const ApplyArgs& step, int sms,
                         cudaStream_t stream) {
@@ -1069,20 +1629,32 @@ cudaError_t launch_prep(const MatrixArgs& a, Ctl* ctl, const ApplyArgs& step, in
 
 template <int kDst>
 cudaError_t launch_ns(const MatrixArgs& a, const ApplyArgs& step, int sms, cudaStream_t stream) {
-    const int pairs = static_cast<int>(std::min<uint64_t>(a.n_tasks, static_cast<uint64_t>(sms / 2)));
-    return launch_pdl(k_ns<kDst>, dim3(2 * pairs), dim3(kNsThreads), kNsSmemBytes, stream, a, step);
+    const uint64_t pairs = static_cast<uint64_t>(sms / 2);
+    cudaError_t e = cudaSuccess;
+    if (a.n_tasks)
+        e = launch_pdl(k_ns<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_tasks, pairs))),
+                       dim3(kNsThreads), kNsSmemBytes, stream, a, step);
+    if (e == cudaSuccess && a.n_panels)
+        e = launch_pdl(k_panel<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_panels, pairs))),
+                       dim3(kPanelThreads), kPanelSmemBytes, stream, a, step);
+    return e;
 }
 
 }  // namespace
 
 cudaError_t prepare_matrix_kernels() {
-    const void* fns[] = {reinterpret_cast<const void*>(k_ns<kDstF32>),
-                         reinterpret_cast<const void*>(k_ns<kDstBf16>),
-                         reinterpret_cast<const void*>(k_ns<kDstParamF32>),
-                         reinterpret_cast<const void*>(k_ns<kDstParamMixed>)};
-    for (const void* f : fns) {
-        const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   static_cast<int>(kNsSmemBytes));
+    const std::pair<const void*, size_t> fns[] = {
+        {reinterpret_cast<const void*>(k_ns<kDstF32>), kNsSmemBytes},
+        {reinterpret_cast<const void*>(k_ns<kDstBf16>), kNsSmemBytes},
+        {reinterpret_cast<const void*>(k_ns<kDstParamF32>), kNsSmemBytes},
+        {reinterpret_cast<const void*>(k_ns<kDstParamMixed>), kNsSmemBytes},
+        {reinterpret_cast<const void*>(k_panel<kDstF32>), kPanelSmemBytes},
+        {reinterpret_cast<const void*>(k_panel<kDstBf16>), kPanelSmemBytes},
+        {reinterpret_cast<const void*>(k_panel<kDstParamF32>), kPanelSmemBytes},
+        {reinterpret_cast<const void*>(k_panel<kDstParamMixed>), kPanelSmemBytes}};
+    for (const auto& f : fns) {
+        const cudaError_t e = cudaFuncSetAttribute(f.first, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(f.second));
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -1099,7 +1671,7 @@ cudaError_t launch_matrix_ops(const MatrixArgs& a, int source, int dest, Ctl* ct
         case kSrcGradF32: e = launch_prep<kSrcGradF32>(a, ctl, st, sms, stream); break;
         default: e = launch_prep<kSrcGradBf16>(a, ctl, st, sms, stream); break;
     }
-    if (e != cudaSuccess || a.n_tasks == 0) return e;
+    if (e != cudaSuccess) return e;
     switch (dest) {
         case kDstF32: return launch_ns<kDstF32>(a, st, sms, stream);
         case kDstBf16: return launch_ns<kDstBf16>(a, st, sms, stream);

@@ -57,6 +57,18 @@ constexpr int kNsGroups = 2;  // each with a slot of what it adds, and two of wh
 constexpr size_t kNsSmemBytes =
     static_cast<size_t>(kNsStages) * kNsStageBytes + 3 * kNsGroups * kNsSlotBytes + 1024;
 
+// Matrices whose shorter side is at most this, and whose result takes one
+// product, are worked on whole by one pair of CTAs (k_panel): A and B stay in
+// shared memory, X streams through it once per iteration. X's lo is then held
+// in 8 bits (e5m2, times 2^8: 3 bits more of X, errors of 0.05 % to 0.25 %).
+constexpr uint32_t kPanelSide = 256;
+constexpr float kPanelLoScale = 256.0f;
+constexpr int kPanelThreads = 384;  // copies in, products, hand-out, copies out, eight warps of arithmetic
+constexpr uint32_t kPanelLoBytes = 128 * 64;       // 128 rows of 64 lo
+constexpr uint32_t kPanelBlockBytes = 4 * 64 * 64 * 2;  // a CTA's 64 columns of X, 256 rows
+constexpr size_t kPanelSmemBytes =
+    8 * 2 * kNsBoxBytes + 2 * kPanelBlockBytes + 4 * kPanelLoBytes + 1024;
+
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
 // ("N": boxes of 64 rows of two or one groups of 64 columns). The lo parts'
@@ -87,6 +99,7 @@ struct NsStack {
     uint32_t first;       // index of its first matrix in the plan
     uint32_t transposed;  // rows > cols: X is the transpose
     uint32_t three;       // products in three parts
+    uint32_t panel;       // worked on by k_panel; xl then holds 8-bit numbers, of the same pitch
     uint32_t tiles;       // preparation tiles per matrix
     uint32_t first_tile;
     float sx;             // power of two X is held by
@@ -148,6 +161,8 @@ struct MatrixArgs {
     const CUtensorMap* maps;
     const NsTask* tasks;
     uint32_t n_tasks;
+    const uint2* panels;   // k_panel's matrices: stack, matrix of the stack
+    uint32_t n_panels;
     const PrepTile* prep;
     uint32_t n_prep;
     uint32_t n_matrices;
@@ -155,7 +170,8 @@ struct MatrixArgs {
     uint32_t* tickets;     // per matrix: preparation tiles summed (0 between launches)
     float* inv;            // per matrix: sx / (norm + eps)
     uint32_t* done;        // per matrix: product tiles done, counted by each CTA with rows in one
-    uint32_t* next;        // tasks handed out
+    uint32_t* next;        // tasks handed out, and k_panel's matrices
+    int steps;
     MatrixStep* step;
     int* err;              // nonzero: a wait ran out
     float coef[kNsMaxSteps][3];

@@ -46,6 +46,16 @@ bool encode_rows(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* ba
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+// X's lo in 8 bits, in boxes of 128 rows of 64 columns (a row of `ld` bytes).
+bool encode_lo8(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
+                uint32_t cols, uint32_t ld, uint32_t count) {
+    const cuuint64_t dims[3] = {cols, rows, count};
+    const cuuint64_t strides[2] = {ld, static_cast<cuuint64_t>(ld) * rows};
+    const cuuint32_t box[3] = {64, 128, 1}, es[3] = {1, 1, 1};
+    return f(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // The same as groups of 64 columns, in boxes of 64 rows of `groups` groups, a
 // group after another. (Columns of the last group that are padding come with
 // it; they are columns of a product that nobody stores.)
@@ -165,6 +175,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.three = three;
         s.m = std::min(s.rows, s.cols);
         s.n = std::max(s.rows, s.cols);
+        s.panel = !three && s.m <= kPanelSide;
         s.ldx = static_cast<uint32_t>(up(s.n, 64));
         s.lda = static_cast<uint32_t>(up(s.m, 8));
         s.first = static_cast<uint32_t>(matrices);
@@ -196,10 +207,12 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
         for (int k = 0; k < 2; ++k) {
             p.x[k] = take(xb);
-            p.xl[k] = take(xb);
+            p.xl[k] = take(s.panel ? xb / 2 : xb);
         }
-        p.a = take(ab);
-        p.b = take(ab);
+        if (!s.panel) {
+            p.a = take(ab);
+            p.b = take(ab);
+        }
         if (three) {
             p.al = take(ab);
             p.bl = take(ab);
@@ -264,6 +277,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     uint64_t tiles_in_wave = 0;
     for (uint32_t si = 0; si < stacks.size(); ++si) {
         const NsStack& s = stacks[si];
+        if (s.panel) continue;
         const uint64_t each = 2ull * s.m * (4ull * s.ldx + (three ? 4ull : 2ull) * s.lda);
         const uint64_t tiles = product_tiles(s, kNsXXt, kNsTileN).size();
         for (uint32_t i = 0; i < s.count;) {
@@ -283,6 +297,16 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         }
     }
     flush();
+    // k_panel's matrices, the longest first
+    std::vector<uint2> panels;
+    {
+        std::vector<uint32_t> by;
+        for (uint32_t si = 0; si < stacks.size(); ++si)
+            if (stacks[si].panel) by.push_back(si);
+        std::stable_sort(by.begin(), by.end(), [&](uint32_t x, uint32_t y) { return stacks[x].n > stacks[y].n; });
+        for (uint32_t si : by)
+            for (uint32_t i = 0; i < stacks[si].count; ++i) panels.push_back(make_uint2(si, i));
+    }
     if (tasks.size() > 0xFFFF0000ull || prep.size() > 0xFFFF0000ull || matrices > 0xFFFF0000ull) {
         *why = "too many matrices in one list";
         return nullptr;
@@ -294,6 +318,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     const size_t o_maps = take(stacks.size() * kMapsPerStack * sizeof(CUtensorMap));
     const size_t o_tasks = take(tasks.size() * sizeof(NsTask));
     const size_t o_prep = take(prep.size() * sizeof(PrepTile));
+    const size_t o_panels = take(panels.size() * sizeof(uint2));
     const size_t tables_end = off;
     const size_t o_partials = take(prep.size() * sizeof(double));
     const size_t o_inv = take(matrices * sizeof(float));
@@ -323,7 +348,13 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.al = three ? reinterpret_cast<__half*>(at(p.al)) : s.a;
         s.bl = three ? reinterpret_cast<__half*>(at(p.bl)) : s.b;
         CUtensorMap* m = maps.data() + i * kMapsPerStack;
-        for (int lo = 0; lo < 2; ++lo) {
+        for (int k = 0; s.panel && k < 2; ++k) {
+            CUtensorMap* qx = m + (k ? kMapX1 : kMapX0);
+            ok = ok && encode_rows(encoder, qx, s.x[k], s.m, s.n, s.ldx, s.count, 128) &&
+                 encode_groups(encoder, qx + kMapN + kMap64, s.x[k], s.m, s.ldx, s.count, 1) &&
+                 encode_lo8(encoder, qx + kMapLo, s.xl[k], s.m, s.n, s.ldx, s.count);
+        }
+        for (int lo = 0; !s.panel && lo < 2; ++lo) {
             CUtensorMap* q = m + (lo ? kMapLo : 0);
             for (int k = 0; k < 2; ++k) {
                 __half* x = lo ? s.xl[k] : s.x[k];
@@ -346,6 +377,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     put(o_maps, maps.data(), maps.size() * sizeof(CUtensorMap));
     put(o_tasks, tasks.data(), tasks.size() * sizeof(NsTask));
     put(o_prep, prep.data(), prep.size() * sizeof(PrepTile));
+    put(o_panels, panels.data(), panels.size() * sizeof(uint2));
     if (ok) {
         e = cudaMemset(plan->slab, 0, operand_bytes);
         if (e == cudaSuccess) e = cudaMemcpy(at(operand_bytes), host.data(), host.size(), cudaMemcpyHostToDevice);
@@ -364,6 +396,9 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     a.n_tasks = static_cast<uint32_t>(tasks.size());
     a.prep = reinterpret_cast<const PrepTile*>(at(o_prep));
     a.n_prep = static_cast<uint32_t>(prep.size());
+    a.panels = reinterpret_cast<const uint2*>(at(o_panels));
+    a.n_panels = static_cast<uint32_t>(panels.size());
+    a.steps = opts.steps;
     a.n_matrices = static_cast<uint32_t>(matrices);
     a.partials = reinterpret_cast<double*>(at(o_partials));
     a.inv = reinterpret_cast<float*>(at(o_inv));
