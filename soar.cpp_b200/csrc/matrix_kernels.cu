@@ -235,11 +235,18 @@ __device__ __forceinline__ void cluster_sync() {
         "barrier.cluster.wait.acquire.aligned;" ::
             : "memory");
 }
-// Arrives on a barrier of either CTA of the pair.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+// Arrives on a barrier of either CTA of the pair. What such a barrier orders is
+// shared memory and TMEM that the pair's products read and write (through the
+// async proxy, fenced for that), not global memory: a release at cluster scope
+// would first wait for all of the thread's global accesses, about a microsecond.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// The same where it does order global memory.
+__device__ __forceinline__ void mbar_arrive_release(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_try_acquire(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
@@ -249,6 +256,7 @@ __device__ __forceinline__ bool mbar_try_cluster(uint32_t bar, uint32_t parity) 
         : "memory");
     return ok != 0;
 }
+
 // Bounded waits, as pipeline.cuh's mbar_wait and wait_flags; the clock is first
 // read after a thousand failed tries (%globaltimer is slow to read).
 struct Patience {
@@ -281,16 +289,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, int* s_e
         if (!p.more(s_err)) return false;
     return true;
 }
-// The same for a barrier the other CTA arrives on.
-__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
+// The same for what mbar_arrive_release orders.
+__device__ __forceinline__ bool warp_wait_acquire(uint32_t bar, uint32_t parity, int* s_err) {
     Patience p;
-    while (!mbar_try_cluster(bar, parity))
-        if (!p.more(s_err)) return false;
-    return true;
-}
-__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity, int* s_err) {
-    Patience p;
-    while (!__all_sync(0xFFFFFFFFu, mbar_try_cluster(bar, parity)))
+    while (!__all_sync(0xFFFFFFFFu, mbar_try_acquire(bar, parity)))
         if (!__all_sync(0xFFFFFFFFu, p.more(s_err))) return false;
     return true;
 }
@@ -433,9 +435,11 @@ __device__ __forceinline__ uint32_t mirror_at(uint32_t row, uint32_t col) {
 // Word offset of (row, col) of a chunk of floats in two slots, 32 columns in
 // each, a row where its fp16 are otherwise. Rows and columns are both read and
 // written without bank conflicts.
+__device__ __forceinline__ uint32_t block_at(uint32_t row, uint32_t col) {  // of a warp's 32 x 32
+    return row * 32u + (((col >> 2) ^ (row & 7u)) << 2) + ((col + (row >> 3)) & 3u);
+}
 __device__ __forceinline__ uint32_t float_at(uint32_t row, uint32_t col) {
-    return (col >> 5) * (kNsSlotBytes / 4) + row * 32u + ((((col & 31u) >> 2) ^ (row & 7u)) << 2) +
-           ((col + (row >> 3)) & 3u);
+    return (col >> 5) * (kNsSlotBytes / 4) + (row & ~31u) * 32u + block_at(row & 31u, col & 31u);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;
@@ -489,8 +493,6 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 
 // --------------------------------------------------------------- products ---
 
-// One wave of eight elements of the result, each lane's own: the stack's
-// destination, or Muon's update of the weights there.
 // Where a stack's result goes, in registers.
 struct Target {
     void* dst;          // the destination, or the parameters
@@ -500,42 +502,66 @@ struct Target {
     float lr_wd, lr_s;  // Muon: lr times the weight decay, and times the shape factor
 };
 
+// A 32 x 32 block of the result, from floats in shared memory (`fs`, rows of 32,
+// block_at), to the stack's destination or into Muon's update of the weights
+// there. A lane has one column of it (`by_rows`) or one row, whose `count`
+// elements lie `inc` apart from `to` on: either way a warp's accesses are
+// consecutive. Sixteen weights at a time are read before the first is written,
+// so that a block costs two round trips to memory.
 template <int kDst>
-__device__ __forceinline__ void put_result(const ApplyArgs& step, const Target& s, bool ema,
-                                           const uint64_t (&at)[8], const float (&o)[8], uint32_t valid) {
+__device__ __forceinline__ void put_block(const ApplyArgs& step, const Target& s, bool ema, const float* fs,
+                                          bool by_rows, uint32_t lane, uint64_t to, uint64_t inc,
+                                          uint32_t count) {
+    auto value = [&](uint32_t i) { return by_rows ? fs[block_at(i, lane)] : fs[block_at(lane, i)]; };
     if constexpr (kDst == kDstF32 || kDst == kDstBf16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!(valid >> i & 1u)) continue;
-            if constexpr (kDst == kDstF32)
-                static_cast<float*>(s.dst)[at[i]] = o[i];
-            else
-                static_cast<uint16_t*>(s.dst)[at[i]] = f32_to_bf16_rn(o[i]);
+        if constexpr (kDst == kDstF32) {
+            float* p = static_cast<float*>(s.dst) + to;
+#pragma unroll 8
+            for (uint32_t i = 0; i < count; ++i, p += inc) *p = value(i);
+        } else {
+            uint16_t* p = static_cast<uint16_t*>(s.dst) + to;
+#pragma unroll 8
+            for (uint32_t i = 0; i < count; ++i, p += inc) *p = f32_to_bf16_rn(value(i));
         }
     } else {
-        float w[8], e[8];
+#pragma unroll 1
+        for (uint32_t from = 0; from < count; from += 16, to += 16 * inc) {
+            float w[16];
+            const float* r = s.master + to;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = valid >> i & 1u ? s.master[at[i]] : 0.0f;
-        if (ema) {
+            for (uint32_t i = 0; i < 16; ++i, r += inc) w[i] = from + i < count ? *r : 0.0f;
+            float* q = s.master + to;
+            uint16_t* p = static_cast<uint16_t*>(s.dst) + to;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = valid >> i & 1u ? s.ema[at[i]] : 0.0f;
-        }
+            for (uint32_t i = 0; i < 16; ++i, q += inc, p += inc) {
+                if (s.lr_wd != 0.0f) w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_wd, w[i]));
+                w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_s, value(from + i)));
+                if (from + i >= count) continue;
+                *q = w[i];
+                if constexpr (kDst == kDstParamMixed) *p = f32_to_bf16_rn(w[i]);
+            }
+            if (ema) {
+                float* e = s.ema + to;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (s.lr_wd != 0.0f) w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_wd, w[i]));
-            w[i] = __fsub_rn(w[i], __fmul_rn(s.lr_s, o[i]));
-            if (!(valid >> i & 1u)) continue;
-            s.master[at[i]] = w[i];
-            if constexpr (kDst == kDstParamMixed)
-                static_cast<uint16_t*>(s.dst)[at[i]] = f32_to_bf16_rn(w[i]);
-        }
-        if (ema) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (valid >> i & 1u)
-                    s.ema[at[i]] = __fadd_rn(__fmul_rn(step.ema_decay, e[i]), __fmul_rn(step.ema_omd, w[i]));
+                for (uint32_t i = 0; i < 16; ++i, e += inc)
+                    if (from + i < count)
+                        *e = __fadd_rn(__fmul_rn(step.ema_decay, *e), __fmul_rn(step.ema_omd, w[i]));
+            }
         }
     }
+}
+
+// The block of X at (y, x), which is the caller's matrix or its transpose.
+template <int kDst>
+__device__ __forceinline__ void put_transposed_or_not(const ApplyArgs& step, const Target& s, bool ema,
+                                                      const float* fs, bool transposed, uint32_t lane, uint32_t y,
+                                                      uint32_t x, uint32_t m, uint32_t n) {
+    const uint32_t mine = (transposed ? y : x) + lane, first = transposed ? x : y;
+    if (mine >= (transposed ? m : n)) return;
+    const uint32_t end = transposed ? n : m;
+    const uint32_t count = first >= end ? 0 : end - first < 32 ? end - first : 32;
+    put_block<kDst>(step, s, ema, fs, !transposed, lane, s.base + static_cast<uint64_t>(first) * s.pitch + mine,
+                    s.pitch, count);
 }
 
 template <int kDst>
@@ -603,7 +629,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     const uint32_t tmem = s_tmem;
     // A reader of the tasks is done with slot q (one lane).
     auto release_task = [&](uint32_t slot) {
-        mbar_arrive_cluster(map_to(smem_u32(&task_empty[slot]), 0));
+        mbar_arrive_pair(map_to(smem_u32(&task_empty[slot]), 0));
     };
 
     // What the epilogue does with a tile: chunks of 64 columns, taken by the two groups of its
@@ -635,7 +661,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         const uint32_t lead_full = uniform(map_to(smem_u32(&full_bar[0]), 0));
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
-            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const uint32_t stack = uniform(s_task[slot].stack);
             if (stack == kEnd) break;
@@ -707,7 +733,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t phases = 0;  // by stage: its full barrier's phase to wait for
         for (uint32_t q = 0; rank == 0; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             if (uniform(s_task[slot].stack) == kEnd) break;
             const uint32_t shape = uniform(s_task[slot].shape);
@@ -726,7 +752,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint64_t da0 = operand_desc(smem, 16);
             const uint64_t db0 = operand_desc(smem + 2 * kNsBoxBytes, bx ? kNsBoxBytes : 16);
             const uint32_t db_k = bx ? 2048 >> 4 : 32 >> 4;
-            if (q >= 2) ok = warp_wait_cluster(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err);
+            if (q >= 2) ok = warp_wait(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err);
             if (!ok) break;
             tc_fence_after();
             for (uint32_t j = 0; j < steps && ok;) {
@@ -781,7 +807,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
                     }
                 }
-                if (q >= kRing && !bar_wait_cluster(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
+                if (q >= kRing && !bar_wait(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
                     break;
                 const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
 #pragma unroll
@@ -800,7 +826,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t chunk = 0, phases = ~0u;  // chunks so far; by group: its empty slot's phase to wait for
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
-            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const NsTask t = s_task[slot];
             if (t.stack == kEnd) break;
@@ -837,7 +863,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t chunk = 0, phases = 0;  // chunks so far; by group: its full buffer's phase to wait for
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
-            bool ok = warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
+            bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const NsTask t = s_task[slot];
             if (t.stack == kEnd) break;
@@ -918,7 +944,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         uint32_t chunk = 0, in_phase = 0, out_phase = 1;
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
-            if (!warp_wait_cluster(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
+            if (!warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
             const NsTask t = s_task[slot];
             if (t.stack == kEnd) break;
             __syncwarp();
@@ -967,7 +993,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (c + kNsGroups >= u.chunks) {  // the group's last of this tile
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+                    if (lane == 0) mbar_arrive_pair(map_to(smem_u32(&acc_empty[buf]), 0));
                     held = false;
                 }
                 if (!u.some) continue;
@@ -997,21 +1023,10 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                     for (int j = 0; j < 64; ++j) fs[float_at(trow, j)] = v[j] * f;
                     __syncwarp();
 #pragma unroll 1
-                    for (uint32_t k = 0; k < 64; k += 8) {
-                        uint64_t to[8];
-                        float o[8];
-                        uint32_t valid = 0;
-#pragma unroll
-                        for (uint32_t l = 0; l < 8; ++l) {
-                            const uint32_t e = k + l;  // a row's half, or a column
-                            const uint32_t rr = t.transposed() ? trow : quad * 32 + (e >> 1);
-                            const uint32_t rc = t.transposed() ? e : lane + 32 * (e & 1);
-                            const uint32_t y = u.row0 + rr, x = col + rc;
-                            to[l] = target.base + (t.transposed() ? x * target.pitch + y : y * target.pitch + x);
-                            o[l] = fs[float_at(rr, rc)];
-                            if (y < t.m && x < t.n) valid |= 1u << l;
-                        }
-                        put_result<kDst>(step, target, a.ema != 0, to, o, valid);
+                    for (uint32_t k = 0; k < 2; ++k) {
+                        const uint32_t y = u.row0 + quad * 32, x = col + k * 32;  // the block's first element
+                        put_transposed_or_not<kDst>(step, target, a.ema != 0, fs + float_at(quad * 32, k * 32),
+                                                    t.transposed(), lane, y, x, t.m, t.n);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(out_bar);
@@ -1058,7 +1073,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             if (held) {
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to(smem_u32(&acc_empty[buf]), 0));
+                if (lane == 0) mbar_arrive_pair(map_to(smem_u32(&acc_empty[buf]), 0));
             }
             if (u.some) chunk += u.chunks;
         }
@@ -1097,7 +1112,7 @@ template <int kDst>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPanelThreads, 1)
 k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
-    constexpr int kMathWarp = 4, kMathWarps = 8;
+    constexpr int kMathWarp = 4, kMathWarps = 16;
     constexpr uint32_t kEnd = 0xFFFFFFFFu;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t mat_full[2], mat_empty[2], mat_done;
@@ -1136,7 +1151,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
             mbar_init(smem_u32(&g0_empty[i]), 1);
             mbar_init(smem_u32(&lo_full[i]), 1);
             mbar_init(smem_u32(&lo_empty[i]), 1);
-            mbar_init(smem_u32(&hi_full[i]), kMathWarps);      // both CTAs' group of four warps
+            mbar_init(smem_u32(&hi_full[i]), kMathWarps);      // both CTAs' eight warps of a chunk
             mbar_init(smem_u32(&hi_out[i]), kMathWarps / 2);
             mbar_init(smem_u32(&hi_empty[i]), 2);              // its product, its store
         }
@@ -1162,7 +1177,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     const uint32_t steps = static_cast<uint32_t>(a.steps);
-    auto release_mat = [&](uint32_t slot) { mbar_arrive_cluster(map_to(smem_u32(&mat_empty[slot]), 0)); };
+    auto release_mat = [&](uint32_t slot) { mbar_arrive_pair(map_to(smem_u32(&mat_empty[slot]), 0)); };
     auto lead = [&](uint64_t* bar) { return map_to(smem_u32(bar), 0); };
     // Copies of this CTA's that landed or not when something failed are waited for by this barrier's
     // owner below; nothing else may touch shared memory after that.
@@ -1175,7 +1190,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
             const uint32_t slot = q & 1;
-            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
             if (!ok) break;
             const uint32_t stack = uniform(s_mat[slot].x), index = uniform(s_mat[slot].y);
             const uint32_t m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
@@ -1204,7 +1219,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                 const CUtensorMap* x = maps + (it & 1 ? kMapX1 : kMapX0);
                 if (it > 0) {
                     // both CTAs' stores of the iteration before have landed
-                    ok = warp_wait_cluster(smem_u32(&x_done), done_phase, &s_err);
+                    ok = warp_wait_acquire(smem_u32(&x_done), done_phase, &s_err);
                     done_phase ^= 1;
                     fence_async_proxy();
                 }
@@ -1260,7 +1275,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         };
         for (uint32_t q = 0; rank == 0 && ok; ++q) {
             const uint32_t slot = q & 1;
-            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
             if (!ok) break;
             const uint32_t stack = uniform(s_mat[slot].x), m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
             __syncwarp();
@@ -1281,7 +1296,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                 __syncwarp();
             }
             for (uint32_t it = 0; it < steps && ok; ++it) {
-                ok = warp_wait_cluster(smem_u32(&a_ready), a_phase, &s_err);
+                ok = warp_wait(smem_u32(&a_ready), a_phase, &s_err);
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -1290,7 +1305,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     mma_commit(smem_u32(&aa_full));
                 }
                 __syncwarp();
-                ok = warp_wait_cluster(smem_u32(&b_ready), a_phase, &s_err);
+                ok = warp_wait(smem_u32(&b_ready), a_phase, &s_err);
                 if (!ok) break;
                 a_phase ^= 1;
                 // the next A takes block j - 1 while block j's product is under way
@@ -1298,7 +1313,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     const uint32_t b = j & 1;
                     if (j < blocks) {
                         ok = warp_wait(smem_u32(&x_full[b]), x_phase >> b & 1, &s_err) &&
-                             warp_wait_cluster(smem_u32(&d_empty[b]), d_phase >> b & 1, &s_err);
+                             warp_wait(smem_u32(&d_empty[b]), d_phase >> b & 1, &s_err);
                         if (!ok) break;
                         x_phase ^= 1u << b;
                         d_phase ^= 1u << b;
@@ -1315,7 +1330,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     if (j == 0 || it + 1 == steps) continue;
                     for (uint32_t g = 0; g < 2 && 2 * (j - 1) + g < chunks && ok; ++g) {
                         const uint32_t h = 2 * ((j - 1) & 1) + g, s = a_slots + h * kNsSlotBytes;
-                        ok = warp_wait_cluster(smem_u32(&hi_full[h]), hi_phase >> h & 1, &s_err);
+                        ok = warp_wait(smem_u32(&hi_full[h]), hi_phase >> h & 1, &s_err);
                         if (!ok) break;
                         hi_phase ^= 1u << h;
                         tc_fence_after();
@@ -1345,7 +1360,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     const NsStack& s = a.stacks[p.x];
                     w = make_uint4(p.x, p.y, s.m, s.n);
                 }
-                if (q >= 2 && !bar_wait_cluster(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
+                if (q >= 2 && !bar_wait(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
                 st_async_v4(map_to(smem_u32(&s_mat[slot]), 1), w, map_to(smem_u32(&mat_full[slot]), 1));
                 s_mat[slot] = w;
                 mbar_arrive(smem_u32(&mat_full[slot]));
@@ -1359,7 +1374,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
             const uint32_t slot = q & 1;
-            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
             if (!ok) break;
             const uint4 w = s_mat[slot];
             __syncwarp();
@@ -1397,8 +1412,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                                 mbar_arrive(smem_u32(&lo_empty[h]));
                                 bulk_wait_all();  // all of X has landed
                                 fence_async_proxy();
-                                mbar_arrive_cluster(map_to(smem_u32(&x_done), 0));
-                                mbar_arrive_cluster(map_to(smem_u32(&x_done), 1));
+                                mbar_arrive_release(map_to(smem_u32(&x_done), 0));
+                                mbar_arrive_release(map_to(smem_u32(&x_done), 1));
                             }
                         }
                     }
@@ -1408,15 +1423,16 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         }
         __syncwarp();
     } else {
-        // ---- arithmetic: two groups of four warps, each with every other 64 columns ----
-        const uint32_t quad = warp & 3, group = (warp - kMathWarp) >> 2;
+        // ---- arithmetic: two groups of eight warps, each with every other 64 columns; a warp
+        // has 32 rows of 32 of them ----
+        const uint32_t quad = warp & 3, group = (warp - kMathWarp) >> 2 & 1, part = (warp - kMathWarp) >> 3;
         const uint32_t trow = quad * 32 + lane, row = rank * kNsRows + trow;
         const uint32_t lanes = tmem + ((quad * 32u) << 16);
         uint32_t a_phase = 0, d_phase = 0, lo_phase = 0, hi_phase = 0, hi_used = 0;
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
             const uint32_t slot = q & 1;
-            ok = warp_wait_cluster(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
             if (!ok) break;
             const uint4 w = s_mat[slot];
             __syncwarp();
@@ -1444,38 +1460,36 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                 if (!ok) break;
                 tc_fence_after();
                 for (uint32_t c = group; c < kb; c += 2) {
-                    float v[64];
+                    float v[32];
                     __syncwarp();
-                    tmem_ld32(lanes + 256 + c * 64, reinterpret_cast<float(&)[32]>(v[0]));
-                    tmem_ld32(lanes + 256 + c * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                    tmem_ld32(lanes + 256 + c * 64 + part * 32, v);
                     const float f = kNsScaleA / (sx * sx);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < 4; ++j) {
                         uint32_t h[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) h[e] = pack2(v[8 * j + 2 * e] * f, v[8 * j + 2 * e + 1] * f);
-                        sts128(a_slots + c * kNsSlotBytes + slot_at(trow, j), make_uint4(h[0], h[1], h[2], h[3]));
+                        sts128(a_slots + c * kNsSlotBytes + slot_at(trow, part * 4 + j), make_uint4(h[0], h[1], h[2], h[3]));
                     }
                 }
                 fence_async_shared();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(lead(&a_ready));
+                if (lane == 0) mbar_arrive_pair(lead(&a_ready));
                 // B = a I + b A + c A A
                 ok = warp_wait(smem_u32(&aa_full), a_phase, &s_err);
                 if (!ok) break;
                 a_phase ^= 1;
                 tc_fence_after();
                 for (uint32_t c = group; c < kb; c += 2) {
-                    float v[64];
+                    float v[32];
                     __syncwarp();
-                    tmem_ld32(lanes + c * 64, reinterpret_cast<float(&)[32]>(v[0]));
-                    tmem_ld32(lanes + c * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                    tmem_ld32(lanes + c * 64 + part * 32, v);
                     const float f2 = cc / (kNsScaleA * kNsScaleA), f1 = cb / kNsScaleA;
-                    const uint32_t diag = row - c * 64;  // (no match: no column)
+                    const uint32_t diag = row - c * 64 - part * 32;  // (no match: no column)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint4 p = lds128(a_slots + c * kNsSlotBytes + slot_at(trow, j));
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 p = lds128(a_slots + c * kNsSlotBytes + slot_at(trow, part * 4 + j));
                         const __half2* ah = reinterpret_cast<const __half2*>(&p);
                         uint32_t h[4];
 #pragma unroll
@@ -1487,13 +1501,13 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                             y1 += diag == static_cast<uint32_t>(i + 1) ? ca : 0.0f;
                             h[e] = pack2(y0, y1);
                         }
-                        sts128(b_slots + c * kNsSlotBytes + slot_at(trow, j), make_uint4(h[0], h[1], h[2], h[3]));
+                        sts128(b_slots + c * kNsSlotBytes + slot_at(trow, part * 4 + j), make_uint4(h[0], h[1], h[2], h[3]));
                     }
                 }
                 fence_async_shared();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(lead(&b_ready));
+                if (lane == 0) mbar_arrive_pair(lead(&b_ready));
                 // X = B X, block by block
                 for (uint32_t j = 0; j < blocks && ok; ++j) {
                     const uint32_t b = j & 1, c = 2 * j + group, h = 2 * b + group;
@@ -1501,23 +1515,22 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     if (!ok) break;
                     d_phase ^= 1u << b;
                     tc_fence_after();
-                    float v[64];
+                    float v[32];
                     if (c < chunks) {
                         __syncwarp();
-                        tmem_ld32(lanes + b * 128 + group * 64, reinterpret_cast<float(&)[32]>(v[0]));
-                        tmem_ld32(lanes + b * 128 + group * 64 + 32, reinterpret_cast<float(&)[32]>(v[32]));
+                        tmem_ld32(lanes + b * 128 + group * 64 + part * 32, v);
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(lead(&d_empty[b]));
+                    if (lane == 0) mbar_arrive_pair(lead(&d_empty[b]));
                     if (c >= chunks) continue;
                     ok = warp_wait(smem_u32(&lo_full[h]), lo_phase >> h & 1, &s_err);
                     if (!ok) break;
                     lo_phase ^= 1u << h;
                     const uint32_t lo = lo_slots + h * kPanelLoBytes;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint4 p = lds128(lo + lo8_at(trow, k));
+                    for (int k = 0; k < 2; ++k) {
+                        const uint4 p = lds128(lo + lo8_at(trow, part * 2 + k));
                         const uint32_t word[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -1542,25 +1555,11 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                             smem_raw + (a_slots - smem_u32(smem_raw) + group * 2 * kNsSlotBytes));
                         __syncwarp();
 #pragma unroll
-                        for (int k = 0; k < 64; ++k) fs[float_at(trow, k)] = v[k] * f;
+                        for (int k = 0; k < 32; ++k) fs[float_at(trow, part * 32 + k)] = v[k] * f;
                         __syncwarp();
-#pragma unroll 1
-                        for (uint32_t k = 0; k < 64; k += 8) {
-                            uint64_t to[8];
-                            float o[8];
-                            uint32_t valid = 0;
-#pragma unroll
-                            for (uint32_t l = 0; l < 8; ++l) {
-                                const uint32_t e = k + l;  // a row's half, or a column
-                                const uint32_t rr = transposed ? trow : quad * 32 + (e >> 1);
-                                const uint32_t rc = transposed ? e : lane + 32 * (e & 1);
-                                const uint32_t y = rank * kNsRows + rr, x = c * 64 + rc;
-                                to[l] = target.base + (transposed ? x * target.pitch + y : y * target.pitch + x);
-                                o[l] = fs[float_at(rr, rc)];
-                                if (y < m && x < n) valid |= 1u << l;
-                            }
-                            put_result<kDst>(step, target, a.ema != 0, to, o, valid);
-                        }
+                        put_transposed_or_not<kDst>(step, target, a.ema != 0, fs + float_at(quad * 32, part * 32),
+                                                    transposed, lane, rank * kNsRows + quad * 32, c * 64 + part * 32,
+                                                    m, n);
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&hi_out[h]));
                         continue;
@@ -1570,9 +1569,9 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     if (!ok) break;
                     hi_used |= 1u << h;
                     hi_phase ^= 1u << h;
-                    uint32_t lo_word[16];
+                    uint32_t lo_word[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
+                    for (int k = 0; k < 4; ++k) {
                         uint32_t hw[4], lw[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -1581,18 +1580,18 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                             const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw[e]));
                             lw[e] = e5m2x2((v[i] - x.x) * kPanelLoScale, (v[i + 1] - x.y) * kPanelLoScale);
                         }
-                        sts128(a_slots + h * kNsSlotBytes + slot_at(trow, k), make_uint4(hw[0], hw[1], hw[2], hw[3]));
+                        sts128(a_slots + h * kNsSlotBytes + slot_at(trow, part * 4 + k), make_uint4(hw[0], hw[1], hw[2], hw[3]));
                         lo_word[2 * k] = lw[0] | lw[1] << 16;
                         lo_word[2 * k + 1] = lw[2] | lw[3] << 16;
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        sts128(lo + lo8_at(trow, k), make_uint4(lo_word[4 * k], lo_word[4 * k + 1], lo_word[4 * k + 2],
+                    for (int k = 0; k < 2; ++k)
+                        sts128(lo + lo8_at(trow, part * 2 + k), make_uint4(lo_word[4 * k], lo_word[4 * k + 1], lo_word[4 * k + 2],
                                                                 lo_word[4 * k + 3]));
                     fence_async_shared();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive_cluster(lead(&hi_full[h]));
+                        mbar_arrive_pair(lead(&hi_full[h]));
                         mbar_arrive(smem_u32(&hi_out[h]));
                     }
                 }

@@ -63,7 +63,7 @@ constexpr size_t kNsSmemBytes =
 // in 8 bits (e5m2, times 2^8: 3 bits more of X, errors of 0.05 % to 0.25 %).
 constexpr uint32_t kPanelSide = 256;
 constexpr float kPanelLoScale = 256.0f;
-constexpr int kPanelThreads = 384;  // copies in, products, hand-out, copies out, eight warps of arithmetic
+constexpr int kPanelThreads = 640;  // copies in, products, hand-out, copies out, sixteen warps of arithmetic
 constexpr uint32_t kPanelLoBytes = 128 * 64;       // 128 rows of 64 lo
 constexpr uint32_t kPanelBlockBytes = 4 * 64 * 64 * 2;  // a CTA's 64 columns of X, 256 rows
 constexpr size_t kPanelSmemBytes =
