@@ -30,36 +30,70 @@ namespace {
 
 // ------------------------------------------------------------- elements -----
 
-__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
-    hi = __float2half_rn(v);
-    lo = __float2half_rn(v - __half2float(hi));
-}
-
-// The matrix element a preparation pass works on: the source, or for Muon
-// u = g + mu m (Nesterov) or m, from the updated momentum m.
-template <int kSrc>
-__device__ __forceinline__ float load_grad(const MatrixArgs& a, const NsStack& s, uint64_t at,
-                                           const StepCoeffs& k) {
-    const void* gp = a.grads[s.tensor];
-    const float raw = kSrc == kSrcGradBf16
-                          ? bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(gp) + at))
-                          : __ldg(static_cast<const float*>(gp) + at);
-    return __fmul_rn(__fmul_rn(raw, k.inv), k.coef);
-}
-
-__device__ __forceinline__ float direction(const MatrixArgs& a, float d, float mom) {
-    return a.nesterov ? __fadd_rn(d, __fmul_rn(a.momentum, mom)) : mom;
-}
-
 template <int kSrc>
 constexpr bool kIsMuon = kSrc == kSrcGradF32 || kSrc == kSrcGradBf16;
+template <int kSrc>
+constexpr bool kIsBf16 = kSrc == kSrcBf16 || kSrc == kSrcGradBf16;
+
+// Up to four adjacent elements from `at` on, as floats (vec: all four, aligned).
+template <bool kBf16>
+__device__ __forceinline__ void read4(const void* p, uint64_t at, bool vec, uint32_t left, float (&v)[4]) {
+    if constexpr (kBf16) {
+        const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+        if (vec) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(q));
+            v[0] = bf16_lo(w.x), v[1] = bf16_hi(w.x), v[2] = bf16_lo(w.y), v[3] = bf16_hi(w.y);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) v[e] = e < left ? bf16_bits_to_f32(__ldg(q + e)) : 0.0f;
+        }
+    } else {
+        const float* q = static_cast<const float*>(p) + at;
+        if (vec) {
+            const float4 w = __ldg(reinterpret_cast<const float4*>(q));
+            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) v[e] = e < left ? __ldg(q + e) : 0.0f;
+        }
+    }
+}
+
+// A preparation tile's 64 x 64 part: sixteen threads to a row, four elements
+// each, sixteen rows at a time.
+struct PrepPart {
+    uint32_t row, col, left;  // this thread's first row and column, and its columns in the matrix
+    const void* src;
+    uint64_t at, pitch;       // of its first element, and from row to row
+    bool vec;
+};
 
 template <int kSrc>
-__device__ __forceinline__ float load_src(const NsStack& s, uint64_t at) {
-    if constexpr (kSrc == kSrcBf16)
-        return bf16_bits_to_f32(__ldg(static_cast<const uint16_t*>(s.src) + at));
-    else
-        return __ldg(static_cast<const float*>(s.src) + at);
+__device__ __forceinline__ PrepPart prep_part(const MatrixArgs& a, const NsStack& s, const PrepTile& t, uint32_t part) {
+    const bool down = s.rows > s.cols;  // a tile's parts lie along the longer side
+    PrepPart p;
+    p.row = (t.tr + (down ? part : 0)) * kPrepTile + threadIdx.x / 16;
+    p.col = (t.tc + (down ? 0 : part)) * kPrepTile + threadIdx.x % 16 * 4;
+    p.left = p.col < s.cols ? s.cols - p.col : 0;
+    if constexpr (kIsMuon<kSrc>) {
+        p.src = a.grads[s.tensor];
+        p.pitch = s.cols;
+        p.at = static_cast<uint64_t>(t.index) * s.rows * s.cols;
+    } else {
+        p.src = s.src;
+        p.pitch = s.src_row;
+        p.at = t.index * s.src_mat;
+    }
+    const uintptr_t vector = kIsBf16<kSrc> ? 8 : 16;
+    p.vec = p.left >= 4 && ((p.at | p.pitch) & 3u) == 0 && reinterpret_cast<uintptr_t>(p.src) % vector == 0 &&
+            (!kIsMuon<kSrc> || reinterpret_cast<uintptr_t>(s.mom) % 16 == 0);
+    p.at += p.row * p.pitch + p.col;
+    return p;
+}
+
+// Unscaled and clipped.
+__device__ __forceinline__ float clipped(float raw, const StepCoeffs& k) {
+    return __fmul_rn(__fmul_rn(raw, k.inv), k.coef);
 }
 
 template <int kSrc>
@@ -71,7 +105,7 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     constexpr bool kMuon = kIsMuon<kSrc>;
     pdl_wait();
     pdl_trigger();
-    // the product kernel of the run before is done: its counters start at 0 again
+    // the product kernels of the run before are done: their counters start at 0 again
     for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < a.n_matrices; i += gridDim.x * kThreads)
         a.done[i] = 0u;
     if (blockIdx.x == 0 && threadIdx.x < 2) a.next[threadIdx.x] = 0u;
@@ -85,26 +119,49 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
         for (uint32_t q = blockIdx.x; q < a.n_prep; q += gridDim.x) {
             const PrepTile t = a.prep[q];
             const NsStack& s = a.stacks[t.stack];
-            const uint32_t c = t.tc * kPrepTile + threadIdx.x % kPrepTile;
-            const uint32_t r0 = t.tr * kPrepTile + threadIdx.x / kPrepTile;
+            const uint32_t rows = s.rows;
+            float* mom = s.mom;
             double acc = 0.0;
-            if (c < s.cols) {
-#pragma unroll 4
-                for (uint32_t i = 0; i < kPrepTile; i += kThreads / kPrepTile) {
-                    const uint32_t r = r0 + i;
-                    if (r >= s.rows) break;
-                    float u;
+            for (uint32_t part = 0; part < t.parts; ++part) {
+                const PrepPart p = prep_part<kSrc>(a, s, t, part);
+                float u[4][4], m[4][4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const bool in = p.left && p.row + 16 * i < rows;
+                    const uint64_t at = p.at + 16 * i * p.pitch;
+                    read4<kIsBf16<kSrc>>(p.src, at, p.vec && in, in ? p.left : 0, u[i]);
                     if constexpr (kMuon) {
-                        const uint64_t at = (static_cast<uint64_t>(t.index) * s.rows + r) * s.cols + c;
-                        const float d = load_grad<kSrc>(a, s, at, k);
-                        const float m = __fadd_rn(__fmul_rn(a.momentum, s.mom[at]), d);
-                        s.mom[at] = m;
-                        u = direction(a, d, m);
-                    } else {
-                        u = load_src<kSrc>(s, t.index * s.src_mat + r * s.src_row + c);
+                        if (p.vec && in) {
+                            *reinterpret_cast<float4*>(m[i]) = *reinterpret_cast<const float4*>(mom + at);
+                        } else {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) m[i][e] = in && e < p.left ? mom[at + e] : 0.0f;
+                        }
                     }
-                    // (the square of a float is exact in 64 bits)
-                    acc = fma(static_cast<double>(u), static_cast<double>(u), acc);
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if constexpr (kMuon) {
+                        const bool in = p.left && p.row + 16 * i < rows;
+                        const uint64_t at = p.at + 16 * i * p.pitch;
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            const float d = clipped(u[i][e], k);
+                            m[i][e] = __fadd_rn(__fmul_rn(a.momentum, m[i][e]), d);
+                            u[i][e] = a.nesterov ? __fadd_rn(d, __fmul_rn(a.momentum, m[i][e])) : m[i][e];
+                        }
+                        if (p.vec && in) {
+                            *reinterpret_cast<float4*>(mom + at) = *reinterpret_cast<const float4*>(m[i]);
+                        } else {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e)
+                                if (in && e < p.left) mom[at + e] = m[i][e];
+                        }
+                    }
+                    // (the square of a float is exact in 64 bits; what is not in the matrix is 0)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e)
+                        acc = fma(static_cast<double>(u[i][e]), static_cast<double>(u[i][e]), acc);
                 }
             }
             const double sum = block_sum(acc, s_red);
@@ -146,16 +203,27 @@ __device__ __forceinline__ uint32_t e5m2x2(float a, float b) {
     return d;
 }
 
-// X's element as hi and lo, lo in 16 or in 8 bits.
-__device__ __forceinline__ void put_x(const NsStack& s, uint64_t matrix, uint64_t at, float v) {
-    __half hi, lo;
-    split_half(v, hi, lo);
-    s.x[0][matrix + at] = hi;
-    if (s.panel)
-        reinterpret_cast<uint8_t*>(s.xl[0])[matrix + at] =
-            static_cast<uint8_t>(e5m2x2((v - __half2float(hi)) * kPanelLoScale, 0.0f));
-    else
-        s.xl[0][matrix + at] = lo;
+// Four adjacent elements of X as hi and lo, lo in 16 or in 8 bits. `at` is a
+// multiple of four, and a row of X goes on to one: the last ones may be padding,
+// which then takes the zeros it has.
+__device__ __forceinline__ void put_x4(const NsStack& s, uint64_t at, const float (&v)[4]) {
+    __half hi[4];
+    float lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = __float2half_rn(v[e]);
+        lo[e] = v[e] - __half2float(hi[e]);
+    }
+    *reinterpret_cast<uint2*>(s.x[0] + at) = *reinterpret_cast<const uint2*>(hi);
+    if (s.panel) {
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(s.xl[0]) + at) =
+            e5m2x2(lo[0] * kPanelLoScale, lo[1] * kPanelLoScale) |
+            e5m2x2(lo[2] * kPanelLoScale, lo[3] * kPanelLoScale) << 16;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hi[e] = __float2half_rn(lo[e]);
+        *reinterpret_cast<uint2*>(s.xl[0] + at) = *reinterpret_cast<const uint2*>(hi);
+    }
 }
 
 template <int kSrc>
@@ -175,39 +243,60 @@ k_matrix_split(MatrixArgs a) {
     for (uint32_t q = blockIdx.x; q < a.n_prep; q += gridDim.x) {
         const PrepTile t = a.prep[q];
         const NsStack& s = a.stacks[t.stack];
-        const uint32_t lc = threadIdx.x % kPrepTile, lr = threadIdx.x / kPrepTile;
-        const uint32_t c = t.tc * kPrepTile + lc;
         const float inv = a.inv[s.first + t.index];
-        const uint64_t matrix = static_cast<uint64_t>(t.index) * s.m * s.ldx;
-#pragma unroll 4
-        for (uint32_t i = 0; i < kPrepTile; i += kThreads / kPrepTile) {
-            const uint32_t r = t.tr * kPrepTile + lr + i;
-            if (r >= s.rows || c >= s.cols) continue;
-            float u;
-            if constexpr (kMuon) {
-                const uint64_t at = (static_cast<uint64_t>(t.index) * s.rows + r) * s.cols + c;
-                const float m = s.mom[at];
-                u = a.nesterov ? direction(a, load_grad<kSrc>(a, s, at, k), m) : m;
-            } else {
-                u = load_src<kSrc>(s, t.index * s.src_mat + r * s.src_row + c);
+        const uint32_t rows = s.rows, cols = s.cols, ldx = s.ldx;
+        const bool transposed = s.transposed != 0;
+        const uint64_t matrix = static_cast<uint64_t>(t.index) * s.m * ldx;
+        for (uint32_t part = 0; part < t.parts; ++part) {
+            const PrepPart p = prep_part<kSrc>(a, s, t, part);
+            float u[4][4], m[4][4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const bool in = p.left && p.row + 16 * i < rows;
+                const uint64_t at = p.at + 16 * i * p.pitch;
+                if (!kMuon || a.nesterov)
+                    read4<kIsBf16<kSrc>>(p.src, at, p.vec && in, in ? p.left : 0, u[i]);
+                if constexpr (kMuon) {
+                    if (p.vec && in) {
+                        *reinterpret_cast<float4*>(m[i]) = *reinterpret_cast<const float4*>(s.mom + at);
+                    } else {
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) m[i][e] = in && e < p.left ? s.mom[at + e] : 0.0f;
+                    }
+                }
             }
-            const float v = __fmul_rn(u, inv);
-            if (s.transposed) {
-                s_t[lr + i][lc] = v;
-            } else {
-                put_x(s, matrix, static_cast<uint64_t>(r) * s.ldx + c, v);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t r = p.row + 16 * i;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    if constexpr (kMuon)
+                        u[i][e] = a.nesterov ? __fadd_rn(clipped(u[i][e], k), __fmul_rn(a.momentum, m[i][e])) : m[i][e];
+                    u[i][e] = __fmul_rn(u[i][e], inv);
+                }
+                if (!transposed) {
+                    if (p.left && r < rows) put_x4(s, matrix + static_cast<uint64_t>(r) * ldx + p.col, u[i]);
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) s_t[threadIdx.x / 16 + 16 * i][threadIdx.x % 16 * 4 + e] = u[i][e];
+                }
             }
-        }
-        if (s.transposed) {
-            __syncthreads();
-            const uint32_t r = t.tr * kPrepTile + lc;  // X's column
-#pragma unroll 4
-            for (uint32_t i = 0; i < kPrepTile; i += kThreads / kPrepTile) {
-                const uint32_t xc = t.tc * kPrepTile + lr + i;  // X's row
-                if (r >= s.rows || xc >= s.cols) continue;
-                put_x(s, matrix, static_cast<uint64_t>(xc) * s.ldx + r, s_t[lc][lr + i]);
+            if (transposed) {
+                __syncthreads();
+                // four source rows (X's columns) of one source column (X's row)
+                const uint32_t r0 = (p.row - threadIdx.x / 16) + threadIdx.x % 16 * 4;
+                const uint32_t c0 = p.col - threadIdx.x % 16 * 4;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const uint32_t c = threadIdx.x / 16 + 16 * i;
+                    if (r0 >= rows || c0 + c >= cols) continue;
+                    float v[4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) v[e] = s_t[threadIdx.x % 16 * 4 + e][c];
+                    put_x4(s, matrix + static_cast<uint64_t>(c0 + c) * ldx + r0, v);
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
     }
 }
@@ -500,6 +589,7 @@ struct Target {
     float* ema;
     uint64_t base, pitch;
     float lr_wd, lr_s;  // Muon: lr times the weight decay, and times the shape factor
+    bool vec;           // in place for vectors of four
 };
 
 // A 32 x 32 block of the result, from floats in shared memory (`fs`, rows of 32,
@@ -551,17 +641,102 @@ __device__ __forceinline__ void put_block(const ApplyArgs& step, const Target& s
     }
 }
 
+// The same for a whole block in place for vectors (Target::vec): four lines of 32
+// elements at a time, four elements to a lane. A line is a row of X, or a column
+// where X is the transpose.
+template <int kDst>
+__device__ __forceinline__ void put_block4(const ApplyArgs& step, const Target& s, bool ema, const float* fs,
+                                           bool by_rows, uint32_t lane, uint64_t to) {
+    constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
+    constexpr bool kHalf = kDst == kDstBf16 || kDst == kDstParamMixed;  // writes bf16
+    const uint32_t l = lane >> 3, k = 4 * (lane & 7);
+    to += l * s.pitch + k;
+    const uint64_t inc = 4 * s.pitch;
+    float4 w[8];
+    if constexpr (kMuon) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const float4*>(s.master + to + i * inc);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint32_t line = 4 * i + l;
+        float o[4];
+        if (by_rows) {
+            // the four lie in one 16-byte group, turned by line / 8 = i / 2
+            const float4 q = *reinterpret_cast<const float4*>(fs + line * 32 + ((k >> 2 ^ (line & 7u)) << 2));
+            const float t[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) o[e] = t[(e + i / 2) & 3];
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) o[e] = fs[block_at(k + e, line)];
+        }
+        if constexpr (kMuon) {
+            float* v = &w[i].x;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                if (s.lr_wd != 0.0f) v[e] = __fsub_rn(v[e], __fmul_rn(s.lr_wd, v[e]));
+                v[e] = __fsub_rn(v[e], __fmul_rn(s.lr_s, o[e]));
+                o[e] = v[e];
+            }
+            *reinterpret_cast<float4*>(s.master + to + i * inc) = w[i];
+        }
+        if constexpr (kHalf)
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(s.dst) + to + i * inc) =
+                make_uint2(pack_bf16x2_rn(o[0], o[1]), pack_bf16x2_rn(o[2], o[3]));
+        else if constexpr (!kMuon)
+            *reinterpret_cast<float4*>(static_cast<float*>(s.dst) + to + i * inc) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    if (kMuon && ema) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            float4* p = reinterpret_cast<float4*>(s.ema + to + i * inc);
+            float4 e = *p;
+            e.x = __fadd_rn(__fmul_rn(step.ema_decay, e.x), __fmul_rn(step.ema_omd, w[i].x));
+            e.y = __fadd_rn(__fmul_rn(step.ema_decay, e.y), __fmul_rn(step.ema_omd, w[i].y));
+            e.z = __fadd_rn(__fmul_rn(step.ema_decay, e.z), __fmul_rn(step.ema_omd, w[i].z));
+            e.w = __fadd_rn(__fmul_rn(step.ema_decay, e.w), __fmul_rn(step.ema_omd, w[i].w));
+            *p = e;
+        }
+    }
+}
+
 // The block of X at (y, x), which is the caller's matrix or its transpose.
 template <int kDst>
 __device__ __forceinline__ void put_transposed_or_not(const ApplyArgs& step, const Target& s, bool ema,
                                                       const float* fs, bool transposed, uint32_t lane, uint32_t y,
                                                       uint32_t x, uint32_t m, uint32_t n) {
+    if (s.vec && y + 32 <= m && x + 32 <= n) {
+        put_block4<kDst>(step, s, ema, fs, !transposed, lane,
+                         s.base + static_cast<uint64_t>(transposed ? x : y) * s.pitch + (transposed ? y : x));
+        return;
+    }
     const uint32_t mine = (transposed ? y : x) + lane, first = transposed ? x : y;
     if (mine >= (transposed ? m : n)) return;
     const uint32_t end = transposed ? n : m;
     const uint32_t count = first >= end ? 0 : end - first < 32 ? end - first : 32;
     put_block<kDst>(step, s, ema, fs, !transposed, lane, s.base + static_cast<uint64_t>(first) * s.pitch + mine,
                     s.pitch, count);
+}
+
+// Where a matrix of a stack goes.
+template <int kDst>
+__device__ __forceinline__ Target target_of(const NsStack& s, uint32_t index, const ApplyArgs& step, bool ema) {
+    constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
+    constexpr bool kHalf = kDst == kDstBf16 || kDst == kDstParamMixed;
+    Target t;
+    t.dst = kMuon ? s.param : s.dst;
+    t.master = s.master;
+    t.ema = s.mom + step.ema_delta;
+    t.base = kMuon ? static_cast<uint64_t>(index) * s.rows * s.cols : static_cast<uint64_t>(index) * s.dst_mat;
+    t.pitch = kMuon ? s.cols : s.dst_row;
+    t.lr_wd = __fmul_rn(step.lr, s.wd);
+    t.lr_s = __fmul_rn(step.lr, s.factor);
+    // four elements from a multiple of four on lie on a vector's boundary
+    t.vec = ((t.base | t.pitch) & 3u) == 0 && (reinterpret_cast<uintptr_t>(t.dst) & (kHalf ? 7u : 15u)) == 0 &&
+            (!kMuon || ((reinterpret_cast<uintptr_t>(t.master) |
+                         (ema ? reinterpret_cast<uintptr_t>(t.ema) : 0)) & 15u) == 0);
+    return t;
 }
 
 template <int kDst>
@@ -953,17 +1128,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const bool last = t.kind() == kNsLast;
             const uint32_t out_bar = smem_u32(&out_full[q & 1][group]);
             Target target{};
-            if (last) {
-                const NsStack& s = a.stacks[t.stack];
-                target.dst = kMuon ? s.param : s.dst;
-                target.master = s.master;
-                target.ema = s.mom + step.ema_delta;
-                target.base = kMuon ? static_cast<uint64_t>(t.index) * s.rows * s.cols
-                                    : static_cast<uint64_t>(t.index) * s.dst_mat;
-                target.pitch = kMuon ? s.cols : s.dst_row;
-                target.lr_wd = __fmul_rn(step.lr, s.wd);
-                target.lr_s = __fmul_rn(step.lr, s.factor);
-            }
+            if (last) target = target_of<kDst>(a.stacks[t.stack], t.index, step, a.ema != 0);
             const float ca = a.coef[t.step()][0], cb = a.coef[t.step()][1], cc = a.coef[t.step()][2];
             const bool two = u.three && (t.kind() == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
             // v = fv accumulator + fx addend (+ ca on the diagonal)
@@ -1442,14 +1607,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
             const uint32_t m = w.z, n = w.w, kb = (m + 63) / 64, chunks = (n + 63) / 64, blocks = (chunks + 1) / 2;
             const float sx = s.sx;
             const bool transposed = s.transposed != 0;
-            Target target{};
-            target.dst = kMuon ? s.param : s.dst;
-            target.master = s.master;
-            target.ema = s.mom + step.ema_delta;
-            target.base = kMuon ? static_cast<uint64_t>(w.y) * s.rows * s.cols : static_cast<uint64_t>(w.y) * s.dst_mat;
-            target.pitch = kMuon ? s.cols : s.dst_row;
-            target.lr_wd = __fmul_rn(step.lr, s.wd);
-            target.lr_s = __fmul_rn(step.lr, s.factor);
+            const Target target = target_of<kDst>(s, w.y, step, a.ema != 0);
             for (uint32_t it = 0; it < steps && ok; ++it) {
                 const float ca = a.coef[it][0], cb = a.coef[it][1], cc = a.coef[it][2];
                 const bool last = it + 1 == steps;

@@ -116,12 +116,14 @@ struct NsStack {
     uint32_t tensor;      // index of its tensor in the list (its gradient's place)
 };
 
-// Preparation tile: 64 x 64 elements of one matrix.
+// Preparation tile: `parts` squares of 64 x 64 elements of one matrix, along
+// its longer side.
 constexpr int kPrepTile = 64;
 struct PrepTile {
     uint32_t stack;
     uint32_t index;   // matrix of the stack
-    uint32_t tr, tc;  // tile row and column
+    uint16_t tr, tc;  // first square's row and column
+    uint32_t parts;
 };
 
 // One output tile of one product of one matrix.

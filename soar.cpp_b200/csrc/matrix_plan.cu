@@ -164,6 +164,13 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         return at;
     };
     uint64_t matrices = 0;
+    // A tile is one square where there are few (every SM gets some), four where there are many
+    // (a sum and a ticket for 16384 elements instead of 4096).
+    uint64_t squares = 0;
+    for (int i = 0; i < n_specs; ++i)
+        squares += specs[i].count * ((specs[i].rows + kPrepTile - 1) / kPrepTile) *
+                   ((specs[i].cols + kPrepTile - 1) / kPrepTile);
+    const uint32_t prep_parts = squares >= 16ull * static_cast<uint64_t>(plan->sms) ? 4 : 1;
     for (int i = 0; i < n_specs; ++i) {
         const MatrixSpec& q = specs[i];
         if (!q.rows || !q.cols || !q.count) continue;
@@ -196,12 +203,15 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.factor = q.factor;
         s.tensor = q.tensor;
         const uint32_t tr = (s.rows + kPrepTile - 1) / kPrepTile, tc = (s.cols + kPrepTile - 1) / kPrepTile;
-        s.tiles = tr * tc;
+        const bool down = s.rows > s.cols;
+        const uint32_t along = down ? tr : tc, across = down ? tc : tr;
+        s.tiles = across * ((along + prep_parts - 1) / prep_parts);
         s.first_tile = static_cast<uint32_t>(prep.size());
         for (uint32_t c = 0; c < s.count; ++c)
-            for (uint32_t y = 0; y < tr; ++y)
-                for (uint32_t x = 0; x < tc; ++x)
-                    prep.push_back({static_cast<uint32_t>(stacks.size()), c, y, x});
+            for (uint32_t y = 0; y < across; ++y)
+                for (uint32_t x = 0; x < along; x += prep_parts)
+                    prep.push_back({static_cast<uint32_t>(stacks.size()), c, static_cast<uint16_t>(down ? x : y),
+                                    static_cast<uint16_t>(down ? y : x), std::min(prep_parts, along - x)});
         Place p{};
         const size_t xb = static_cast<size_t>(s.count) * s.m * s.ldx * 2;
         const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
