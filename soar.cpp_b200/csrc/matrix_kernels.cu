@@ -215,10 +215,10 @@ __device__ __forceinline__ void put_x4(const NsStack& s, uint64_t at, const floa
         lo[e] = v[e] - __half2float(hi[e]);
     }
     *reinterpret_cast<uint2*>(s.x[0] + at) = *reinterpret_cast<const uint2*>(hi);
-    if (s.panel) {
+    if (!s.three) {
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(s.xl[0]) + at) =
-            e5m2x2(lo[0] * kPanelLoScale, lo[1] * kPanelLoScale) |
-            e5m2x2(lo[2] * kPanelLoScale, lo[3] * kPanelLoScale) << 16;
+            e5m2x2(lo[0] * kLoScale, lo[1] * kLoScale) |
+            e5m2x2(lo[2] * kLoScale, lo[3] * kLoScale) << 16;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) hi[e] = __float2half_rn(lo[e]);
@@ -546,11 +546,16 @@ __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(static_cast<uint16_t>(v)) : "memory");
 }
 
-// v += f times the thread's row of a chunk.
-__device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, float f, float (&v)[64]) {
+// Byte offset of sixteen columns (group j of 4) of a row of a slot of 8-bit lo:
+// rows of 64 bytes, 64-byte swizzle.
+__device__ __forceinline__ uint32_t lo8_at(uint32_t row, uint32_t j) {
+    return row * 64u + ((j ^ (row >> 1 & 3u)) << 4);
+}
+// v += f times the thread's row of a slot: 32 fp16.
+__device__ __forceinline__ void add_half(uint32_t slot, uint32_t row, float f, float* v) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint4 q = lds128(slot + slot_at(row, j));
+    for (int j = 0; j < 4; ++j) {
+        const uint4 q = lds128(slot + lo8_at(row, j));
         const __half2* h = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -560,15 +565,35 @@ __device__ __forceinline__ void slot_add(uint32_t slot, uint32_t row, float f, f
         }
     }
 }
-
-// Byte offset of sixteen columns (group j of 4) of a row of a slot of 8-bit lo:
-// rows of 64 bytes, 64-byte swizzle.
-__device__ __forceinline__ uint32_t lo8_at(uint32_t row, uint32_t j) {
-    return row * 64u + ((j ^ (row >> 1 & 3u)) << 4);
+// v += f times sixteen lo (group j of the thread's row).
+__device__ __forceinline__ void add_lo8(uint32_t slot, uint32_t row, uint32_t j, float f, float* v) {
+    const uint4 p = lds128(slot + lo8_at(row, j));
+    const uint32_t word[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        // (an e5m2 number is the upper byte of an fp16 one)
+        const uint32_t lo01 = __byte_perm(word[e], 0, 0x1404), lo23 = __byte_perm(word[e], 0, 0x3424);
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo01));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lo23));
+        v[4 * e] = __fmaf_rn(f, x.x, v[4 * e]);
+        v[4 * e + 1] = __fmaf_rn(f, x.y, v[4 * e + 1]);
+        v[4 * e + 2] = __fmaf_rn(f, y.x, v[4 * e + 2]);
+        v[4 * e + 3] = __fmaf_rn(f, y.y, v[4 * e + 3]);
+    }
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four values as packed fp16, and what is left of them in 8 bits.
+__device__ __forceinline__ uint32_t split4(const float* v, uint32_t& h0, uint32_t& h1) {
+    h0 = pack2(v[0], v[1]);
+    h1 = pack2(v[2], v[3]);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+    return e5m2x2((v[0] - x.x) * kLoScale, (v[1] - x.y) * kLoScale) |
+           e5m2x2((v[2] - y.x) * kLoScale, (v[3] - y.y) * kLoScale) << 16;
 }
 
 // Two values as packed fp16 (hi), and what is left of them (lo).
@@ -749,7 +774,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[kNsStages], empty_bar[kNsStages];
     __shared__ __align__(8) uint64_t acc_full[2], acc_empty[2], task_full[kRing], task_empty[kRing];
-    __shared__ __align__(8) uint64_t in_full[kNsGroups], in_empty[kNsGroups], out_empty[kNsGroups];
+    __shared__ __align__(8) uint64_t in_full[2 * kNsGroups], in_empty[2 * kNsGroups];
+    __shared__ __align__(8) uint64_t out_empty[kNsGroups];
     __shared__ __align__(8) uint64_t out_full[2][kNsGroups];  // of even and of odd tiles
     __shared__ __align__(8) uint64_t drain_bar;
     __shared__ __align__(16) NsTask s_task[kRing];
@@ -765,7 +791,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     const uint32_t rank = blockIdx.x & 1u;  // 0 leads the pair: hands out tasks, issues products
     const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t in_slots = smem + kNsStages * kNsStageBytes;
-    const uint32_t out_slots = in_slots + kNsGroups * kNsSlotBytes;
+    const uint32_t out_slots = in_slots + 2 * kNsGroups * kLoBytes;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kNsStages; ++i) {
             mbar_init(smem_u32(&full_bar[i]), 1);
@@ -776,8 +802,10 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             mbar_init(smem_u32(&acc_empty[i]), 2 * kNsMathWarps);  // both CTAs' warps
         }
         for (int i = 0; i < kNsGroups; ++i) {
-            mbar_init(smem_u32(&in_full[i]), 1);
-            mbar_init(smem_u32(&in_empty[i]), kNsMathWarps / kNsGroups);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(smem_u32(&in_full[2 * i + b]), 1);
+                mbar_init(smem_u32(&in_empty[2 * i + b]), kNsMathWarps / kNsGroups);
+            }
             for (int odd = 0; odd < 2; ++odd) mbar_init(smem_u32(&out_full[odd][i]), kNsMathWarps / kNsGroups);
             mbar_init(smem_u32(&out_empty[i]), 1);
         }
@@ -808,7 +836,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     };
 
     // What the epilogue does with a tile: chunks of 64 columns, taken by the two groups of its
-    // warps by turns, `ins` slots to add to each and `outs` buffers made of each.
+    // warps by turns, `ins` slots to add to each (in order) and `outs` buffers made of each.
     struct Tile {
         uint32_t row0, col0, chunks, ins, outs;
         bool sym, three, lo, some, mirror;
@@ -823,8 +851,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         u.lo = !u.sym || u.three;                   // made of hi and lo
         u.some = u.row0 < t.m;                      // this CTA has rows in the tile
         u.mirror = u.sym && u.col0 >= t.row() + kNsTileM;  // right of the diagonal's block
-        // A (and its lo), or X's lo where the product takes hi alone
-        u.ins = t.kind() == kNsXXt ? 0 : u.sym ? (u.three ? 2 : 1) : (u.three ? 0 : 1);
+        // A in two halves (and its lo), or X's lo where the product takes hi alone
+        u.ins = t.kind() == kNsXXt ? 0 : u.sym ? (u.three ? 4 : 2) : (u.three ? 0 : 1);
         u.outs = u.three && u.mirror ? 2 : 1;
         return u;
     };
@@ -998,7 +1026,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     } else if (warp == 3) {
         // ---- brings what the epilogue adds ----
         fence_async_proxy();  // (X of the kernel before)
-        uint32_t chunk = 0, phases = ~0u;  // chunks so far; by group: its empty slot's phase to wait for
+        uint32_t chunk = 0, turns = 0, phases = ~0u;  // chunks so far; by group, its next slot; by slot, its phase
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
             bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
@@ -1008,28 +1036,33 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             __syncwarp();
             if (lane == 0) release_task(slot);
             const Tile u = tile_of(t);
+            if (!u.some) continue;
             const CUtensorMap* src = a.maps + static_cast<uint64_t>(t.stack) * kMapsPerStack +
-                                     (u.sym ? static_cast<int>(kMapA) : kMapLo + (t.step() & 1 ? kMapX1 : kMapX0));
-            for (uint32_t i = 0; u.some && ok && i < u.chunks * u.ins; ++i) {
-                const uint32_t c = u.ins == 2 ? i >> 1 : i, g = (chunk + c) % kNsGroups;
-                ok = warp_wait(smem_u32(&in_empty[g]), phases >> g & 1u, &s_err);
-                if (!ok) break;
-                phases ^= 1u << g;
-                if (elect_one()) {
-                    const uint32_t bar = smem_u32(&in_full[g]);
-                    mbar_expect_tx(bar, kNsSlotBytes);
-                    tma_load(in_slots + g * kNsSlotBytes, src + (u.ins == 2 && (i & 1) ? kMapLo : 0), bar,
-                             u.col0 + c * 64, u.row0, t.index);
+                                     (u.sym ? kMapA + kMap32 : kMapLo + (t.step() & 1 ? kMapX1 : kMapX0));
+            for (uint32_t c = 0; c < u.chunks && ok; ++c) {
+                const uint32_t g = (chunk + c) % kNsGroups;
+                for (uint32_t i = 0; i < u.ins && ok; ++i) {
+                    const uint32_t b = 2 * g + (turns >> g & 1u);
+                    turns ^= 1u << g;
+                    ok = warp_wait(smem_u32(&in_empty[b]), phases >> b & 1u, &s_err);
+                    if (!ok) break;
+                    phases ^= 1u << b;
+                    if (elect_one()) {
+                        const uint32_t bar = smem_u32(&in_full[b]);
+                        mbar_expect_tx(bar, kLoBytes);
+                        tma_load(in_slots + b * kLoBytes, src + (i >= 2 ? kMapLo : 0), bar, u.col0 + c * 64 + (i & 1) * 32,
+                                 u.row0, t.index);
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             if (!ok) break;
-            if (u.some) chunk += u.chunks;
+            chunk += u.chunks;
         }
         if (*reinterpret_cast<volatile int*>(&s_err))
             // copies in flight land before the CTA may end
-            for (uint32_t g = 0; g < kNsGroups; ++g)
-                bar_wait(smem_u32(&in_full[g]), phases >> g & 1u, &s_drain_err);
+            for (uint32_t b = 0; b < 2 * kNsGroups; ++b)
+                bar_wait(smem_u32(&in_full[b]), phases >> b & 1u, &s_drain_err);
         __syncwarp();
     } else if (warp < kMathWarp) {
         // ---- two warps, by turns, store what a tile makes: one waits for its tile's stores to
@@ -1113,10 +1146,9 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         // ---- arithmetic: two groups of four warps; a warp has 32 rows of its group's chunks ----
         const uint32_t quad = warp & 3, group = (warp - kMathWarp) >> 2;
         const uint32_t trow = quad * 32 + lane;  // this thread's row (TMEM lane) of the CTA's 128
-        const uint32_t in_slot = in_slots + group * kNsSlotBytes, at = out_slots + group * 2 * kNsSlotBytes;
-        const uint32_t in_bar = smem_u32(&in_full[group]), in_free = smem_u32(&in_empty[group]);
+        const uint32_t at = out_slots + group * 2 * kNsSlotBytes;
         const uint32_t out_free = smem_u32(&out_empty[group]);
-        uint32_t chunk = 0, in_phase = 0, out_phase = 1;
+        uint32_t chunk = 0, turn = 0, in_phases = 0, out_phase = 1;  // turn: the group's next in slot
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
             if (!warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
@@ -1164,13 +1196,27 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (!u.some) continue;
 #pragma unroll
                 for (int j = 0; j < 64; ++j) v[j] *= fv;
-                for (uint32_t i = 0; i < u.ins && ok; ++i) {
-                    ok = warp_wait(in_bar, in_phase, &s_err);
-                    in_phase ^= 1;
-                    slot_add(in_slot, trow, fx, v);
+                auto take = [&](auto&& add) {
+                    const uint32_t b = 2 * group + turn;
+                    ok = ok && warp_wait(smem_u32(&in_full[b]), in_phases >> turn & 1u, &s_err);
+                    in_phases ^= 1u << turn;
+                    turn ^= 1;
+                    add(in_slots + b * kLoBytes);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(in_free);
+                    if (lane == 0) mbar_arrive(smem_u32(&in_empty[b]));
+                };
+                if (u.ins == 1) {
+                    take([&](uint32_t slot) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) add_lo8(slot, trow, j, fx / kLoScale, v + 16 * j);
+                    });
+                } else if (u.ins) {
+                    for (uint32_t i = 0; i < u.ins; i += 2) {
+                        take([&](uint32_t slot) { add_half(slot, trow, fx, v); });
+                        take([&](uint32_t slot) { add_half(slot, trow, fx, v + 32); });
+                    }
                 }
+                if (!ok) break;
                 if (t.kind() == kNsAA) {
                     const uint32_t diag = u.row0 + trow - col;  // (no match: no column)
 #pragma unroll
@@ -1193,6 +1239,22 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         put_transposed_or_not<kDst>(step, target, a.ema != 0, fs + float_at(quad * 32, k * 32),
                                                     t.transposed(), lane, y, x, t.m, t.n);
                     }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(out_bar);
+                    continue;
+                }
+                if (!u.sym && !u.three) {
+                    // hi, and lo in 8 bits
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t h[8], l[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) l[e] = split4(v + 16 * j + 4 * e, h[2 * e], h[2 * e + 1]);
+                        sts128(at + slot_at(trow, 2 * j), make_uint4(h[0], h[1], h[2], h[3]));
+                        sts128(at + slot_at(trow, 2 * j + 1), make_uint4(h[4], h[5], h[6], h[7]));
+                        sts128(at + kNsSlotBytes + lo8_at(trow, j), make_uint4(l[0], l[1], l[2], l[3]));
+                    }
+                    fence_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(out_bar);
                     continue;
@@ -1406,8 +1468,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                         if (!ok) break;
                         lo_phase ^= 1u << l;
                         if (elect_one()) {
-                            mbar_expect_tx(smem_u32(&lo_full[l]), kPanelLoBytes);
-                            tma_load(lo_slots + l * kPanelLoBytes, x + kMapLo, smem_u32(&lo_full[l]), (2 * j + g) * 64,
+                            mbar_expect_tx(smem_u32(&lo_full[l]), kLoBytes);
+                            tma_load(lo_slots + l * kLoBytes, x + kMapLo, smem_u32(&lo_full[l]), (2 * j + g) * 64,
                                      rank * kNsRows, index);
                         }
                         __syncwarp();
@@ -1561,7 +1623,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                         } else {
                             if (some) {
                                 tma_store(x, a_slots + h * kNsSlotBytes, c * 64, rank * kNsRows, w.y);
-                                tma_store(x + kMapLo, lo_slots + h * kPanelLoBytes, c * 64, rank * kNsRows, w.y);
+                                tma_store(x + kMapLo, lo_slots + h * kLoBytes, c * 64, rank * kNsRows, w.y);
                             }
                             bulk_commit();
                             // a slot is free once its store has read it: the one before's has when
@@ -1685,25 +1747,9 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     ok = warp_wait(smem_u32(&lo_full[h]), lo_phase >> h & 1, &s_err);
                     if (!ok) break;
                     lo_phase ^= 1u << h;
-                    const uint32_t lo = lo_slots + h * kPanelLoBytes;
+                    const uint32_t lo = lo_slots + h * kLoBytes;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint4 p = lds128(lo + lo8_at(trow, part * 2 + k));
-                        const uint32_t word[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            // (an e5m2 number is the upper byte of an fp16 one)
-                            const uint32_t lo01 = __byte_perm(word[e], 0, 0x1404), lo23 = __byte_perm(word[e], 0, 0x3424);
-                            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&lo01));
-                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&lo23));
-                            const float f = ca / kPanelLoScale;
-                            float* o = v + 16 * k + 4 * e;
-                            o[0] = __fmaf_rn(f, x.x, o[0]);
-                            o[1] = __fmaf_rn(f, x.y, o[1]);
-                            o[2] = __fmaf_rn(f, y.x, o[2]);
-                            o[3] = __fmaf_rn(f, y.y, o[3]);
-                        }
-                    }
+                    for (int k = 0; k < 2; ++k) add_lo8(lo, trow, part * 2 + k, ca / kLoScale, v + 16 * k);
                     if (last) {
                         // through shared memory as floats, the warp's own 32 rows, so that the result
                         // is written along the rows of the caller's matrix (in the group's two slots,
@@ -1730,17 +1776,10 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     uint32_t lo_word[8];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        uint32_t hw[4], lw[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int i = 8 * k + 2 * e;
-                            hw[e] = pack2(v[i], v[i + 1]);
-                            const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&hw[e]));
-                            lw[e] = e5m2x2((v[i] - x.x) * kPanelLoScale, (v[i + 1] - x.y) * kPanelLoScale);
-                        }
+                        uint32_t hw[4];
+                        lo_word[2 * k] = split4(v + 8 * k, hw[0], hw[1]);
+                        lo_word[2 * k + 1] = split4(v + 8 * k + 4, hw[2], hw[3]);
                         sts128(a_slots + h * kNsSlotBytes + slot_at(trow, part * 4 + k), make_uint4(hw[0], hw[1], hw[2], hw[3]));
-                        lo_word[2 * k] = lw[0] | lw[1] << 16;
-                        lo_word[2 * k + 1] = lw[2] | lw[3] << 16;
                     }
 #pragma unroll
                     for (int k = 0; k < 2; ++k)

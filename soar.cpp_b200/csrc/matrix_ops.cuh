@@ -13,7 +13,7 @@
 // lose lo. A rounding of X's small singular directions would otherwise grow by
 // a factor of a (3.4) per iteration: with X in hi alone, a matrix of a few
 // strong directions over noise comes out 0.6 % to 7 % off (bf16 operands: 5 %
-// to 60 %), with hi + lo 0.03 % to 0.2 %. That is below the rounding of a bf16
+// to 60 %), with hi + lo 0.04 % to 0.25 %. That is below the rounding of a bf16
 // result (0.17 % rms). For fp32 results every product is taken as hi hi + hi lo
 // + lo hi of both operands (22 bits).
 //
@@ -53,21 +53,24 @@ constexpr int kNsThreads = (6 + kNsMathWarps) * 32;
 constexpr uint32_t kNsBoxBytes = 64 * 64 * 2;  // one TMA box: 64 rows of 64 fp16
 constexpr uint32_t kNsStageBytes = 4 * kNsBoxBytes;
 constexpr uint32_t kNsSlotBytes = 2 * kNsBoxBytes;  // epilogue: 128 rows of 64 fp16
-constexpr int kNsGroups = 2;  // each with a slot of what it adds, and two of what it makes
+constexpr uint32_t kLoBytes = 128 * 64;  // a slot of 128 rows of 64 bytes: of lo, or of 32 columns of A
+constexpr int kNsGroups = 2;  // each with two such slots of what it adds, and two slots of what it makes
 constexpr size_t kNsSmemBytes =
-    static_cast<size_t>(kNsStages) * kNsStageBytes + 3 * kNsGroups * kNsSlotBytes + 1024;
+    static_cast<size_t>(kNsStages) * kNsStageBytes + kNsGroups * (2 * kLoBytes + 2 * kNsSlotBytes) + 1024;
+
+// Where products take hi alone, X's lo is held in 8 bits (e5m2, times 2^8: 3 more
+// bits of X). That leaves the errors stated above (16 bits: 0.03 % to 0.16 %), and
+// lo is a quarter of what is read and written beside the products' operands.
+constexpr float kLoScale = 256.0f;
 
 // Matrices whose shorter side is at most this, and whose result takes one
 // product, are worked on whole by one pair of CTAs (k_panel): A and B stay in
-// shared memory, X streams through it once per iteration. X's lo is then held
-// in 8 bits (e5m2, times 2^8: 3 bits more of X, errors of 0.05 % to 0.25 %).
+// shared memory, X streams through it once per iteration.
 constexpr uint32_t kPanelSide = 256;
-constexpr float kPanelLoScale = 256.0f;
 constexpr int kPanelThreads = 640;  // copies in, products, hand-out, copies out, sixteen warps of arithmetic
-constexpr uint32_t kPanelLoBytes = 128 * 64;       // 128 rows of 64 lo
 constexpr uint32_t kPanelBlockBytes = 4 * 64 * 64 * 2;  // a CTA's 64 columns of X, 256 rows
 constexpr size_t kPanelSmemBytes =
-    8 * 2 * kNsBoxBytes + 2 * kPanelBlockBytes + 4 * kPanelLoBytes + 1024;
+    8 * 2 * kNsBoxBytes + 2 * kPanelBlockBytes + 4 * kLoBytes + 1024;
 
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
@@ -76,18 +79,19 @@ constexpr size_t kPanelSmemBytes =
 enum NsMap {
     kMapX0 = 0,        // {K128, K64, N128, N64} of the first X buffer, then of the second
     kMapX1 = 4,
-    kMapA = 8,         // {K128, K64}
-    kMapB = 10,
-    kMapLo = 12,
-    kMapsPerStack = 24
+    kMapA = 8,         // {K128, K64, 128 rows of 32 columns}
+    kMapB = 11,        // {K128, K64}
+    kMapLo = 13,
+    kMapsPerStack = 26
 };
+constexpr int kMap32 = 2;  // from A's K128 map to its last
 constexpr int kMap64 = 1;  // from a K128 (N128) map to its K64 (N64) one
 constexpr int kMapN = 2;   // from X's K maps to its N maps
 
 // One stack of equal matrices.
 struct NsStack {
     __half* x[2];   // X hi, double-buffered across iterations: [count][m][ldx]
-    __half* xl[2];  // X lo
+    __half* xl[2];  // X lo (three products; else 8-bit numbers, of the same pitch in elements)
     __half* a;      // [count][m][lda]
     __half* al;     // (three products only)
     __half* b;
@@ -99,7 +103,7 @@ struct NsStack {
     uint32_t first;       // index of its first matrix in the plan
     uint32_t transposed;  // rows > cols: X is the transpose
     uint32_t three;       // products in three parts
-    uint32_t panel;       // worked on by k_panel; xl then holds 8-bit numbers, of the same pitch
+    uint32_t panel;       // worked on by k_panel
     uint32_t tiles;       // preparation tiles per matrix
     uint32_t first_tile;
     float sx;             // power of two X is held by

@@ -35,15 +35,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
 }
 
-// A stack of `count` row-major fp16 matrices, in boxes of `height` rows of 64 columns.
+// A stack of `count` row-major fp16 matrices, in boxes of `height` rows of 64 (or 32) columns.
 bool encode_rows(PFN_cuTensorMapEncodeTiled_v12000 f, CUtensorMap* map, void* base, uint32_t rows,
-                 uint32_t cols, uint32_t ld, uint32_t count, uint32_t height) {
+                 uint32_t cols, uint32_t ld, uint32_t count, uint32_t height, uint32_t width = 64) {
     const cuuint64_t dims[3] = {cols, rows, count};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld) * 2,
                                    static_cast<cuuint64_t>(ld) * rows * 2};
-    const cuuint32_t box[3] = {64, height, 1}, es[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {width, height, 1}, es[3] = {1, 1, 1};
     return f(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, es,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE,
+             width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // X's lo in 8 bits, in boxes of 128 rows of 64 columns (a row of `ld` bytes).
@@ -217,7 +218,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
         for (int k = 0; k < 2; ++k) {
             p.x[k] = take(xb);
-            p.xl[k] = take(s.panel ? xb / 2 : xb);
+            p.xl[k] = take(three ? xb : xb / 2);
         }
         if (!s.panel) {
             p.a = take(ab);
@@ -288,7 +289,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     for (uint32_t si = 0; si < stacks.size(); ++si) {
         const NsStack& s = stacks[si];
         if (s.panel) continue;
-        const uint64_t each = 2ull * s.m * (4ull * s.ldx + (three ? 4ull : 2ull) * s.lda);
+        const uint64_t each = s.m * ((three ? 8ull : 6ull) * s.ldx + (three ? 8ull : 4ull) * s.lda);
         const uint64_t tiles = product_tiles(s, kNsXXt, kNsTileN).size();
         for (uint32_t i = 0; i < s.count;) {
             // as many as the wave still takes: until it has both the bytes and the tiles
@@ -369,6 +370,10 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
             for (int k = 0; k < 2; ++k) {
                 __half* x = lo ? s.xl[k] : s.x[k];
                 CUtensorMap* qx = q + (k ? kMapX1 : kMapX0);
+                if (lo && !three) {
+                    ok = ok && encode_lo8(encoder, qx, x, s.m, s.n, s.ldx, s.count);
+                    continue;
+                }
                 ok = ok && encode_rows(encoder, qx, x, s.m, s.n, s.ldx, s.count, 128) &&
                      encode_rows(encoder, qx + kMap64, x, s.m, s.n, s.ldx, s.count, 64) &&
                      encode_groups(encoder, qx + kMapN, x, s.m, s.ldx, s.count, 2) &&
@@ -376,7 +381,8 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                 __half* ab = k ? (lo ? s.bl : s.b) : (lo ? s.al : s.a);
                 CUtensorMap* qa = q + (k ? kMapB : kMapA);
                 ok = ok && encode_rows(encoder, qa, ab, s.m, s.m, s.lda, s.count, 128) &&
-                     encode_rows(encoder, qa + kMap64, ab, s.m, s.m, s.lda, s.count, 64);
+                     encode_rows(encoder, qa + kMap64, ab, s.m, s.m, s.lda, s.count, 64) &&
+                     (k || encode_rows(encoder, qa + kMap32, ab, s.m, s.m, s.lda, s.count, 128, 32));
             }
         }
     }
