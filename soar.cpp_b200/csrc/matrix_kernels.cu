@@ -860,7 +860,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     if (warp == 0) {
         // ---- loads operand tiles ----
         fence_async_proxy();  // (X of the kernel before)
-        uint32_t phases = ~0u;  // by stage: its empty barrier's phase to wait for
+        uint32_t st = 0, phase = 1;  // the next stage; its empty barrier's phase to wait for
+        uint32_t issued = 0;
         const uint32_t lead_full = uniform(map_to(smem_u32(&full_bar[0]), 0));
         for (uint32_t q = 0;; ++q) {
             const uint32_t slot = q % kRing;
@@ -892,18 +893,13 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint32_t depth = kind == kNsXXt ? tn : tm;
             // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
             const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
-            // three products: the small ones first, lo hi, hi lo, hi hi
-            uint32_t p = three ? 0 : 2, k0 = 0;
-            const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
-            const CUtensorMap* mapb = maps + mb;
-            // (a tile starts at the first stage: addresses in the loop are constants)
-            while (ok && p < 3) {
-#pragma unroll
-                for (uint32_t st = 0; st < kNsStages; ++st) {
-                    if (p == 3) break;
-                    ok = warp_wait(smem_u32(&empty_bar[st]), phases >> st & 1u, &s_err);
+            for (uint32_t p = three ? 0 : 2; p < 3 && ok; ++p) {
+                // three products: the small ones first, lo hi, hi lo, hi hi
+                const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
+                const CUtensorMap* mapb = maps + mb + (p == 1 ? kMapLo : 0);
+                for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK) {
+                    ok = warp_wait(smem_u32(&empty_bar[st]), phase, &s_err);
                     if (!ok) break;
-                    phases ^= 1u << st;
                     if (elect_one()) {
                         const uint32_t bar = lead_full + st * 8;
                         const uint32_t sa = smem + st * kNsStageBytes, sb = sa + 2 * kNsBoxBytes;
@@ -914,26 +910,23 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         else
                             tma_load_pair(sb, mapb, bar, k0, col, index);
                     }
-                    k0 += kNsTileK;
-                    if (k0 >= depth) {
-                        k0 = 0;
-                        ++p;
-                        mapa = maps + ma;
-                        mapb = maps + mb + (p == 1 ? kMapLo : 0);
+                    ++issued;
+                    if (++st == kNsStages) {
+                        st = 0;
+                        phase ^= 1;
                     }
                 }
             }
             if (!ok) break;
         }
         if (*reinterpret_cast<volatile int*>(&s_err) && rank == 0 && lane == 0) {
-            // copies in flight land before the CTA may end (a stage's next phase to wait for on
-            // its empty barrier is also the one its last copies complete on its full barrier)
-            for (uint32_t st = 0; st < kNsStages; ++st)
-                bar_wait(smem_u32(&full_bar[st]), phases >> st & 1u, &s_drain_err);
+            // copies in flight land before the CTA may end
+            for (uint32_t j = issued > kNsStages ? issued - kNsStages : 0; j < issued; ++j)
+                bar_wait(smem_u32(&full_bar[j % kNsStages]), (j / kNsStages) & 1, &s_drain_err);
         }
     } else if (warp == 1) {
         // ---- the leader's second warp issues the pair's products ----
-        uint32_t phases = 0;  // by stage: its full barrier's phase to wait for
+        uint32_t st = 0, phase = 0;  // the next stage; its full barrier's phase to wait for
         for (uint32_t q = 0; rank == 0; ++q) {
             const uint32_t slot = q % kRing, buf = q & 1;
             bool ok = warp_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err);
@@ -958,27 +951,25 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             if (q >= 2) ok = warp_wait(smem_u32(&acc_empty[buf]), (q / 2 + 1) & 1, &s_err);
             if (!ok) break;
             tc_fence_after();
-            for (uint32_t j = 0; j < steps && ok;) {
+            for (uint32_t j = 0; j < steps; ++j) {
+                ok = warp_wait(smem_u32(&full_bar[st]), phase, &s_err);
+                if (!ok) break;
+                tc_fence_after();
+                const bool second = j >= from && j < to;
+                const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
+                const bool fresh = j == 0 || (second && j == from);
+                if (elect_one()) {
+                    const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
+                    mma_f16(dd, da, db, idesc, !fresh);
 #pragma unroll
-                for (uint32_t st = 0; st < kNsStages; ++st) {
-                    if (j == steps) break;
-                    ok = warp_wait(smem_u32(&full_bar[st]), phases >> st & 1u, &s_err);
-                    if (!ok) break;
-                    phases ^= 1u << st;
-                    tc_fence_after();
-                    const bool second = j >= from && j < to;
-                    const uint32_t dd = d + (second ? kNsTileN / 2 : 0);
-                    const bool fresh = j == 0 || (second && j == from);
-                    if (elect_one()) {
-                        const uint64_t da = da0 + st * (kNsStageBytes >> 4), db = db0 + st * (kNsStageBytes >> 4);
-                        mma_f16(dd, da, db, idesc, !fresh);
-#pragma unroll
-                        for (uint32_t k = 1; k < kNsTileK / 16; ++k)
-                            mma_f16(dd, da + k * 2, db + k * db_k, idesc, true);
-                        mma_commit(smem_u32(&empty_bar[st]));
-                        if (j + 1 == steps) mma_commit(smem_u32(&acc_full[buf]));
-                    }
-                    ++j;
+                    for (uint32_t k = 1; k < kNsTileK / 16; ++k)
+                        mma_f16(dd, da + k * 2, db + k * db_k, idesc, true);
+                    mma_commit(smem_u32(&empty_bar[st]));
+                    if (j + 1 == steps) mma_commit(smem_u32(&acc_full[buf]));
+                }
+                if (++st == kNsStages) {
+                    st = 0;
+                    phase ^= 1;
                 }
             }
             if (!ok) break;
