@@ -893,11 +893,15 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const uint32_t depth = kind == kNsXXt ? tn : tm;
             // both CTAs' bytes count on the leader's barrier (boxes past the edge come as zeros)
             const uint32_t bytes = 4 * kNsBoxBytes + (narrow ? 2 : 4) * kNsBoxBytes;
+            // The block on A's or B's diagonal, the largest, comes last: each addition rounds a
+            // sum towards zero by up to 2^-23 of it, and few follow then.
+            uint32_t first_k = kind == kNsXXt ? 0 : (place & 0xFFFFu) * kNsTileM + kNsTileM;
+            if (first_k >= depth) first_k = 0;
             for (uint32_t p = three ? 0 : 2; p < 3 && ok; ++p) {
                 // three products: the small ones first, lo hi, hi lo, hi hi
                 const CUtensorMap* mapa = maps + ma + (p == 0 ? kMapLo : 0);
                 const CUtensorMap* mapb = maps + mb + (p == 1 ? kMapLo : 0);
-                for (uint32_t k0 = 0; k0 < depth; k0 += kNsTileK) {
+                for (uint32_t j = 0, k0 = first_k; j < depth; j += kNsTileK) {
                     ok = warp_wait(smem_u32(&empty_bar[st]), phase, &s_err);
                     if (!ok) break;
                     if (elect_one()) {
@@ -911,6 +915,8 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                             tma_load_pair(sb, mapb, bar, k0, col, index);
                     }
                     ++issued;
+                    k0 += kNsTileK;
+                    if (k0 >= depth) k0 = 0;
                     if (++st == kNsStages) {
                         st = 0;
                         phase ^= 1;
