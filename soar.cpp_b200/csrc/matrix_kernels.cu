@@ -328,10 +328,11 @@ __device__ __forceinline__ void cluster_sync() {
 // shared memory and TMEM that the pair's products read and write (through the
 // async proxy, fenced for that), not global memory: a release at cluster scope
 // would first wait for all of the thread's global accesses, about a microsecond.
+// Without it nothing orders plain reads of shared memory before the arrival.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The same where it does order global memory.
+// The same where it does order global memory, or plain reads of shared memory.
 __device__ __forceinline__ void mbar_arrive_release(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -383,6 +384,12 @@ __device__ __forceinline__ bool warp_wait_acquire(uint32_t bar, uint32_t parity,
     Patience p;
     while (!__all_sync(0xFFFFFFFFu, mbar_try_acquire(bar, parity)))
         if (!__all_sync(0xFFFFFFFFu, p.more(s_err))) return false;
+    return true;
+}
+__device__ __forceinline__ bool bar_wait_acquire(uint32_t bar, uint32_t parity, int* s_err) {
+    Patience p;
+    while (!mbar_try_acquire(bar, parity))
+        if (!p.more(s_err)) return false;
     return true;
 }
 // Sixteen bytes into the other CTA's shared memory, counted on a barrier there.
@@ -811,8 +818,9 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
         }
         for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&task_full[i]), 1);
-            // five readers and the arithmetic here, four and the arithmetic in the other CTA
-            mbar_init(smem_u32(&task_empty[i]), 9 + 2 * kNsMathWarps);
+            // the leader: five readers, the arithmetic and the other CTA's word that it is done too;
+            // the other CTA: four readers and the arithmetic
+            mbar_init(smem_u32(&task_empty[i]), (rank == 0 ? 6 : 4) + kNsMathWarps);
             if (rank == 1) mbar_expect_tx(smem_u32(&task_full[i]), sizeof(NsTask));
         }
         mbar_init(smem_u32(&drain_bar), 1);
@@ -831,9 +839,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     // A reader of the tasks is done with slot q (one lane).
-    auto release_task = [&](uint32_t slot) {
-        mbar_arrive_pair(map_to(smem_u32(&task_empty[slot]), 0));
-    };
+    auto release_task = [&](uint32_t slot) { mbar_arrive(smem_u32(&task_empty[slot])); };
 
     // What the epilogue does with a tile: chunks of 64 columns, taken by the two groups of its
     // warps by turns, `ins` slots to add to each (in order) and `outs` buffers made of each.
@@ -1007,7 +1013,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                         fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
                     }
                 }
-                if (q >= kRing && !bar_wait(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
+                if (q >= kRing && !bar_wait_acquire(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
                     break;
                 const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
 #pragma unroll
@@ -1017,6 +1023,16 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 s_task[slot] = t;
                 mbar_arrive(smem_u32(&task_full[slot]));
                 if (t.stack == kEnd) break;
+            }
+        } else if (rank == 1 && lane == 0) {
+            // the other CTA's reads of a slot come before the leader's next write into it: its readers
+            // count here, and one thread without global accesses of its own passes that on
+            for (uint32_t q = 0;; ++q) {
+                const uint32_t slot = q % kRing;
+                if (!bar_wait(smem_u32(&task_full[slot]), (q / kRing) & 1, &s_err)) break;
+                if (s_task[slot].stack == kEnd) break;
+                if (!bar_wait(smem_u32(&task_empty[slot]), (q / kRing) & 1, &s_err)) break;
+                mbar_arrive_release(map_to(smem_u32(&task_empty[slot]), 0));
             }
         }
         __syncwarp();
@@ -1363,7 +1379,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&mat_full[i]), 1);
             // copies in, products, copies out, arithmetic here; all but the products there
-            mbar_init(smem_u32(&mat_empty[i]), 5 + 2 * kMathWarps);
+            mbar_init(smem_u32(&mat_empty[i]), (rank == 0 ? 4 : 2) + kMathWarps);
             mbar_init(smem_u32(&x_full[i]), 1);
             mbar_init(smem_u32(&x_empty[i]), 1);
             mbar_init(smem_u32(&d_full[i]), 1);
@@ -1401,7 +1417,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     const uint32_t steps = static_cast<uint32_t>(a.steps);
-    auto release_mat = [&](uint32_t slot) { mbar_arrive_pair(map_to(smem_u32(&mat_empty[slot]), 0)); };
+    auto release_mat = [&](uint32_t slot) { mbar_arrive(smem_u32(&mat_empty[slot])); };
     auto lead = [&](uint64_t* bar) { return map_to(smem_u32(bar), 0); };
     // Copies of this CTA's that landed or not when something failed are waited for by this barrier's
     // owner below; nothing else may touch shared memory after that.
@@ -1584,11 +1600,20 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     const NsStack& s = a.stacks[p.x];
                     w = make_uint4(p.x, p.y, s.m, s.n);
                 }
-                if (q >= 2 && !bar_wait(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
+                if (q >= 2 && !bar_wait_acquire(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
                 st_async_v4(map_to(smem_u32(&s_mat[slot]), 1), w, map_to(smem_u32(&mat_full[slot]), 1));
                 s_mat[slot] = w;
                 mbar_arrive(smem_u32(&mat_full[slot]));
                 if (w.x == kEnd) break;
+            }
+        } else if (rank == 1 && lane == 0) {
+            // (as in k_ns: this CTA's reads of a slot come before the leader's next write into it)
+            for (uint32_t q = 0;; ++q) {
+                const uint32_t slot = q & 1;
+                if (!bar_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err)) break;
+                if (s_mat[slot].x == kEnd) break;
+                if (!bar_wait(smem_u32(&mat_empty[slot]), q >> 1 & 1, &s_err)) break;
+                mbar_arrive_release(map_to(smem_u32(&mat_empty[slot]), 0));
             }
         }
         __syncwarp();

@@ -221,6 +221,33 @@ def test_two_plans_on_two_streams(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("src", [torch.float32, torch.bfloat16])
+def test_many_runs_of_ragged_lists(cuda, src):
+    """Runs back to back, by turns, of lists of many matrices of a few tiles each:
+    every pair of CTAs goes through hundreds of tiles of changing shape and chunk
+    counts, some without rows for its second CTA, and through several matrices
+    of at most 256 rows. No wait gives up, and every run leaves the same bits."""
+    shapes = [(24, 128, 131), (24, 130, 192), (24, 250, 257), (24, 320, 320), (24, 300, 400), (24, 512, 250),
+              (24, 400, 400), (24, 640, 300), (16, 480, 480), (16, 385, 510)]
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    lists = [[torch.randn(s, generator=gen, device="cuda").to(src) for s in shapes] for _ in range(2)]
+    dsts = [[torch.empty_like(x) for x in xs] for xs in lists]
+    plans = [sb.Orthogonalizer(xs, ys) for xs, ys in zip(lists, dsts)]
+    first = []
+    for plan, ys in zip(plans, dsts):
+        plan.run()
+        first.append([y.clone() for y in ys])
+    for _ in range(10):
+        for _ in range(30):
+            for plan in plans:
+                plan.run()
+        torch.cuda.synchronize()
+        for plan, ys, want in zip(plans, dsts, first):
+            assert plan.error() == 0
+            assert all(torch.equal(y, w) for y, w in zip(ys, want))
+
+
+@gpu
 def test_empty(cuda):
     plan = sb.Orthogonalizer([], [])
     plan.run()
