@@ -67,6 +67,7 @@ constexpr float kLoScale = 256.0f;
 // product, are worked on whole by one pair of CTAs (k_panel): A and B stay in
 // shared memory, X streams through it once per iteration.
 constexpr uint32_t kPanelSide = 256;
+constexpr uint32_t kPanelAnyColumns = 1152;  // up to this longer side always, beyond it in long lists
 constexpr int kPanelThreads = 640;  // copies in, products, hand-out, copies out, sixteen warps of arithmetic
 constexpr uint32_t kPanelBlockBytes = 4 * 64 * 64 * 2;  // a CTA's 64 columns of X, 256 rows
 constexpr size_t kPanelSmemBytes =

@@ -171,6 +171,16 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     for (int i = 0; i < n_specs; ++i)
         squares += specs[i].count * ((specs[i].rows + kPrepTile - 1) / kPrepTile) *
                    ((specs[i].cols + kPrepTile - 1) / kPrepTile);
+    // k_panel or k_ns for a matrix of at most 256 rows (of X). k_panel gives it to one pair of CTAs
+    // for 30 us + 0.075 us a column, k_ns deals its tiles to all pairs but goes through 15 products
+    // one after the other. One 256 x 1024 matrix takes 120 us in either, 256 x 512 79 in k_panel and
+    // 112 in k_ns, 256 x 4096 376 and 172; 37 of 256 x 4096 (half the pairs) 528 and 502, 74 of them
+    // 702 and 877. So long matrices go to k_panel where the list has enough columns for all pairs.
+    uint64_t panel_columns = 0;
+    for (int i = 0; i < n_specs; ++i)
+        if (!three && specs[i].rows && specs[i].cols && std::min(specs[i].rows, specs[i].cols) <= kPanelSide)
+            panel_columns += specs[i].count * std::max(specs[i].rows, specs[i].cols);
+    const uint64_t panel_most = std::max<uint64_t>(kPanelAnyColumns, 2 * panel_columns / std::max(1, plan->sms / 2));
     const uint32_t prep_parts = squares >= 16ull * static_cast<uint64_t>(plan->sms) ? 4 : 1;
     for (int i = 0; i < n_specs; ++i) {
         const MatrixSpec& q = specs[i];
@@ -183,7 +193,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.three = three;
         s.m = std::min(s.rows, s.cols);
         s.n = std::max(s.rows, s.cols);
-        s.panel = !three && s.m <= kPanelSide;
+        s.panel = !three && s.m <= kPanelSide && s.n <= panel_most;
         s.ldx = static_cast<uint32_t>(up(s.n, 64));
         s.lda = static_cast<uint32_t>(up(s.m, 8));
         s.first = static_cast<uint32_t>(matrices);

@@ -136,6 +136,20 @@ def test_list_of_stacks_padded(cuda, dst):
 
 
 @gpu
+@pytest.mark.parametrize("shapes", [[(1, 130, 1152)], [(1, 130, 1153)], [(2, 4100, 100)], [(1, 1, 20000)],
+                                    [(2, 256, 1300), (80, 90, 1400)], [(3, 240, 5001), (1, 33, 64), (1, 300, 310)]],
+                         ids=lambda s: "+".join("x".join(map(str, v)) for v in s))
+def test_long_matrices_of_few_rows(cuda, shapes):
+    """At most 256 rows: alone, where the longest columns are dealt to all SMs,
+    and in lists long enough for a pair of CTAs per matrix."""
+    gs = [matrices(s, 60 + i) for i, s in enumerate(shapes)]
+    got, _ = _run(gs, torch.bfloat16)
+    for g, d in zip(gs, got):
+        want = ns64(g.cuda())
+        assert rel(d, want) <= tolerance(g.cuda(), want, torch.bfloat16)
+
+
+@gpu
 def test_values(cuda):
     """Zeros give zeros; one inf or NaN makes its matrix NaN and no other; very
     small, very large and one-element matrices come out as the definition says."""
