@@ -241,6 +241,142 @@ private:
     void* h_{nullptr};
 };
 
+// ---- matrices (no reference counterpart) -----------------------------------
+
+// Orthogonalises a list of stacks of matrices by Newton-Schulz products
+// (soar_ortho_create). Buffers are bound when it is made; run() is
+// asynchronous on its stream.
+class Orthogonalizer {
+public:
+    static soar_ortho_opts default_options() {
+        soar_ortho_opts o;
+        soar_ortho_default_opts(&o);
+        return o;
+    }
+    explicit Orthogonalizer(const std::vector<soar_matrix_desc>& stacks,
+                            const soar_ortho_opts& options = default_options()) {
+        detail::check(soar_ortho_create(stacks.data(), static_cast<int>(stacks.size()), &options, &h_),
+                      "ortho_create");
+    }
+    Orthogonalizer(Orthogonalizer&& o) noexcept : h_(std::exchange(o.h_, nullptr)) {}
+    Orthogonalizer& operator=(Orthogonalizer&& o) noexcept {
+        if (this != &o) {
+            if (h_) soar_ortho_destroy(h_);
+            h_ = std::exchange(o.h_, nullptr);
+        }
+        return *this;
+    }
+    Orthogonalizer(const Orthogonalizer&) = delete;
+    Orthogonalizer& operator=(const Orthogonalizer&) = delete;
+    ~Orthogonalizer() {
+        if (h_) soar_ortho_destroy(h_);
+    }
+    void run(void* stream = nullptr) { detail::check(soar_ortho_run(h_, stream), "ortho_run"); }
+    // Nonzero if a device-side wait of some run timed out (synchronises).
+    [[nodiscard]] int error() const {
+        int e = 0;
+        detail::check(soar_ortho_error(h_, &e), "ortho_error");
+        return e;
+    }
+    [[nodiscard]] void* handle() const noexcept { return h_; }
+
+private:
+    void* h_{nullptr};
+};
+
+struct MuonOptions {
+    float lr{2e-2f};
+    float momentum{0.95f};
+    float weight_decay{0.0f};
+    bool nesterov{true};
+    int scale{SOAR_MUON_SCALE_ASPECT};
+    int steps{5};  // Newton-Schulz iterations
+};
+
+// Muon on the same device step, over weight matrices: shapes[i] is parameter
+// i's stack of rows x cols matrices. Same methods as SGD's.
+class Muon {
+public:
+    template <class P>
+    explicit Muon(const std::vector<P>& params, const std::vector<soar_matrix_shape>& shapes,
+                  MuonOptions options = {}, AdamWExtOptions ext = {}) {
+        if (params.size() != shapes.size()) throw std::runtime_error("muon_create: one shape per parameter");
+        std::vector<soar_tensor_desc> d;
+        d.reserve(params.size());
+        for (const auto& p : params) {
+            soar_tensor_desc t{};
+            if (p) {
+                t.param = p->cuda_data();
+                auto g = p->grad();
+                t.grad = g ? g->cuda_data() : nullptr;
+                t.numel = static_cast<uint64_t>(p->numel());
+            }
+            t.weight_decay = options.weight_decay;
+            d.push_back(t);
+        }
+        soar_muon_opts c;
+        soar_muon_default_opts(&c);
+        c.lr = options.lr;
+        c.momentum = options.momentum;
+        c.weight_decay = options.weight_decay;
+        c.nesterov = options.nesterov ? 1 : 0;
+        c.scale = options.scale;
+        c.steps = options.steps;
+        c.layout = ext.layout;
+        c.max_grad_norm = ext.max_grad_norm;
+        c.use_loss_scaler = ext.use_loss_scaler ? 1 : 0;
+        c.init_scale = ext.init_scale;
+        c.growth_factor = ext.growth_factor;
+        c.backoff_factor = ext.backoff_factor;
+        c.growth_interval = ext.growth_interval;
+        c.device = ext.device;
+        detail::check(soar_muon_create(d.data(), shapes.data(), static_cast<int>(d.size()), &c, &h_),
+                      "muon_create");
+    }
+    Muon(Muon&& o) noexcept : h_(std::exchange(o.h_, nullptr)) {}
+    Muon& operator=(Muon&& o) noexcept {
+        if (this != &o) {
+            if (h_) soar_optim_destroy(h_);
+            h_ = std::exchange(o.h_, nullptr);
+        }
+        return *this;
+    }
+    Muon(const Muon&) = delete;
+    Muon& operator=(const Muon&) = delete;
+    ~Muon() {
+        if (h_) soar_optim_destroy(h_);
+    }
+
+    void step(void* stream = nullptr) { detail::check(soar_optim_step(h_, stream), "step"); }
+    void zero_grad(void* stream = nullptr) {
+        detail::check(soar_optim_zero_grad(h_, stream), "zero_grad");
+    }
+    float clip_grad_norm(float max_norm, void* stream = nullptr) {
+        float n = 0.0f;
+        detail::check(soar_optim_clip_grad_norm(h_, max_norm, &n, stream), "clip_grad_norm");
+        return n;
+    }
+    void clip_grad_norm_async(float max_norm, void* stream = nullptr) {
+        detail::check(soar_optim_clip_grad_norm_async(h_, max_norm, stream),
+                      "clip_grad_norm_async");
+    }
+    void set_lr(float lr) noexcept { soar_optim_set_lr(h_, lr); }
+    [[nodiscard]] float get_lr() const noexcept {
+        float lr = 0.0f;
+        soar_optim_get_lr(h_, &lr);
+        return lr;
+    }
+    [[nodiscard]] soar_step_info info(void* stream = nullptr) const {
+        soar_step_info i{};
+        detail::check(soar_optim_get_info(h_, &i, stream), "get_info");
+        return i;
+    }
+    [[nodiscard]] void* handle() const noexcept { return h_; }
+
+private:
+    void* h_{nullptr};
+};
+
 // CosineAnnealingLR(AdamW&, total_steps, eta_min = 1e-6f, warmup_steps = 0)
 // (adamw.hpp:45-57). Bound to the optimizer's handle, so it follows the
 // optimizer across moves (the reference binds a reference to the object).
