@@ -160,10 +160,13 @@ SOAR_API int soar_sgd_create(const soar_tensor_desc* tensors, int n_tensors,
    result), which drives every singular value that is not tiny to about 1. A
    matrix of zeros gives zeros; one with an inf or NaN gives NaN throughout.
    The products run with fp16 operands (11 bits, scaled by powers of two) and
-   fp32 sums, X being carried in 22 bits: 0.03 % to 0.2 % off in norm. Where
-   the result is fp32 (fp32 destinations, SOAR_LAYOUT_FP32) every product is
-   taken in three parts, about as exact as fp32 products. Sides are at most
-   1048576. The same inputs give the same bits. */
+   fp32 sums, X being carried in 14 bits: 0.04 % to 0.25 % off in norm. Where
+   the result is fp32 (fp32 destinations, SOAR_LAYOUT_FP32) X and the products'
+   operands have 22 bits and every product is taken in three parts, about as
+   exact as fp32 products (sides up to about 2048; the sums' rounding grows with
+   the side). The coefficients have to keep X's singular values below 8 and
+   |a + b s^2 + c s^4| at them below 60 (fp16's range), as the default ones do.
+   Sides are at most 1048576. The same inputs give the same bits. */
 #define SOAR_NS_MAX_STEPS 16
 
 enum soar_dtype {
@@ -193,9 +196,9 @@ typedef struct soar_ortho_opts {
 
 SOAR_API void soar_ortho_default_opts(soar_ortho_opts* out);
 /* Plans the orthogonalisation of a list of stacks (a stack without elements is
-   left alone) and allocates its workspace: 8 bytes per element and 4 per
-   element of the m x m products (8 with fp32 destinations). Buffers are bound
-   as the optimizer's are. */
+   left alone) and allocates its workspace: 6 bytes per element and 4 per
+   element of the m x m products, 8 and 8 with fp32 destinations (rows padded to
+   multiples of 64 and 8 elements). Buffers are bound as the optimizer's are. */
 SOAR_API int soar_ortho_create(const soar_matrix_desc* mats, int n_mats,
                                const soar_ortho_opts* opts, void** out_handle);
 /* Enqueues one orthogonalisation of every matrix on `stream`; never

@@ -14,6 +14,7 @@
 #include <cstring>
 #include <new>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include <cuda_runtime.h>
@@ -433,6 +434,7 @@ bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::stri
         *why = "eps must be >= 0";
         return false;
     }
+    std::unordered_set<const void*> taken;
     for (int i = 0; i < n; ++i) {
         const soar_matrix_shape& s = p.shapes[i];
         if (!soarb::matrix_shape_ok(s.count, s.rows, s.cols, why)) {
@@ -441,6 +443,10 @@ bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::stri
         }
         if (s.count * s.rows * s.cols != t[i].numel) {
             *why = "tensor " + std::to_string(i) + ": count x rows x cols is not numel";
+            return false;
+        }
+        if (t[i].numel && t[i].param && !taken.insert(t[i].param).second) {
+            *why = "tensor " + std::to_string(i) + ": another tensor has the same parameters";
             return false;
         }
     }

@@ -2,6 +2,7 @@
 #include <cstring>
 #include <exception>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include <cuda_runtime.h>
@@ -39,6 +40,12 @@ struct Ortho {
     soarb::MatrixPlan* plan = nullptr;
 };
 
+// Whether the strides stay below 2^44 elements in all (so that no offset wraps).
+bool within(uint64_t count, uint64_t rows, uint64_t row, uint64_t mat) {
+    constexpr uint64_t kMost = 1ull << 43;
+    return (rows <= 1 || row <= kMost / (rows - 1)) && (count <= 1 || mat <= kMost / (count - 1));
+}
+
 // Whether `count` matrices of `rows` rows of `cols` elements do not overlap.
 bool apart(uint64_t count, uint64_t rows, uint64_t cols, uint64_t row, uint64_t mat) {
     if (rows > 1 && row < cols) return false;
@@ -60,6 +67,7 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
     const uint64_t sb = opts->src_type == SOAR_DTYPE_BF16 ? 2 : 4;
     const uint64_t db = opts->dst_type == SOAR_DTYPE_BF16 ? 2 : 4;
     std::vector<soarb::MatrixSpec> specs;
+    std::unordered_set<const void*> taken;
     for (int i = 0; i < n; ++i) {
         const soar_matrix_desc& d = mats[i];
         const std::string at = "stack " + std::to_string(i) + ": ";
@@ -71,12 +79,15 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
             return fail(at + "pointer not aligned to its element size");
         for (uint64_t s : {d.src_row, d.src_mat, d.dst_row, d.dst_mat})
             if (s > (1ull << 40)) return fail(at + "a stride of more than 2^40 elements");
+        if (!within(d.count, d.rows, d.src_row, d.src_mat) || !within(d.count, d.rows, d.dst_row, d.dst_mat))
+            return fail(at + "strides over more than 2^44 elements");
         if (d.rows > 1 && d.src_row < d.cols) return fail(at + "source rows overlap");
         if (!apart(d.count, d.rows, d.cols, d.dst_row, d.dst_mat))
             return fail(at + "destination rows or matrices overlap");
         if (d.src == d.dst &&
             (sb != db || (d.rows > 1 && d.src_row != d.dst_row) || (d.count > 1 && d.src_mat != d.dst_mat)))
             return fail(at + "in place needs the same type and strides");
+        if (!taken.insert(d.dst).second) return fail(at + "another stack has the same destination");
         soarb::MatrixSpec q;
         q.src = d.src;
         q.dst = d.dst;

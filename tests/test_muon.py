@@ -45,6 +45,11 @@ def test_refusals(shape, numel, over, word):
     assert rc == -1 and word in why, why
 
 
+def test_refuses_the_same_parameters_twice():
+    rc, why = _create([(1, 4, 8), (2, 4, 4)], [32, 32])
+    assert rc == -1 and "same parameters" in why, why
+
+
 def test_null_arguments_and_defaults():
     lib = sb.lib()
     out = ctypes.c_void_p()
@@ -195,6 +200,35 @@ def test_steps_match_definition(cuda, layout, scale, nesterov, wd, clip, scaler)
         if scaler:
             assert info.loss_scale == model.scale and info.growth_tracker == model.tracker
     _check(opt, model, params, mixed, steps)
+
+
+@gpu
+@pytest.mark.parametrize("layout", ["fp32", "bf16_mixed"])
+def test_parameters_at_odd_offsets(cuda, layout):
+    """Parameters and gradients that start one to three elements into a buffer:
+    the elements around them stay, and the step is the same."""
+    dt = torch.bfloat16 if layout == "bf16_mixed" else torch.float32
+    shapes = [(64, 64), (64, 128), (300, 96), (260, 520), (2, 32, 64)]
+
+    def place(x, off):
+        buf = torch.full((x.numel() + 8,), 7.0, dtype=dt, device="cuda")
+        buf[off:off + x.numel()] = x.to(dt).cuda().flatten()
+        return buf, buf[off:off + x.numel()].view(x.shape)
+
+    ps = [place(matrices(s, i, "noise", 0.02), 1 + i % 3) for i, s in enumerate(shapes)]
+    gs = [place(matrices(s, 50 + i), 1 + i % 3) for i, s in enumerate(shapes)]
+    params = [v for _, v in ps]
+    opts = sb.MuonOptions(lr=2e-3, scale="rms", weight_decay=0.1)
+    opt = sb.Muon(params, opts, grads=[v for _, v in gs], layout=layout)
+    model = Model64(params, [0.1] * len(shapes), opts)
+    for _ in range(2):
+        model.step([v for _, v in gs], layout == "fp32")
+        opt.step()
+    assert opt.info().error == 0
+    _check(opt, model, params, layout == "bf16_mixed", 2)
+    for i, (buf, v) in enumerate(ps + gs):
+        off = 1 + i % len(shapes) % 3
+        assert bool((buf[:off] == 7).all()) and bool((buf[off + v.numel():] == 7).all())
 
 
 @gpu

@@ -59,6 +59,16 @@ def test_refusals(desc, over, word):
     assert rc == -1 and word in why, why
 
 
+def test_refuses_destinations_taken_and_strides_that_wrap():
+    rc, why = _create([_desc(), _desc(src=1 << 20)])
+    assert rc == -1 and "same destination" in why, why
+    # (count - 1) x stride is past 64 bits
+    rc, why = _create([_desc(count=1 << 26, dst_mat=1 << 40)])
+    assert rc == -1 and "2^44" in why, why
+    rc, why = _create([_desc(count=1 << 26, src_mat=1 << 40)])
+    assert rc == -1 and "2^44" in why, why
+
+
 def test_null_arguments():
     lib = sb.lib()
     assert lib.soar_ortho_create(None, 1, None, None) == -1
@@ -216,6 +226,24 @@ def test_in_place_repeat_stream_graph(cuda):
     torch.cuda.synchronize()
     (other,), _ = _run([matrices((3, 130, 260), 10)], torch.float32)
     assert torch.equal(dst, other) and not torch.equal(dst, first)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 130, 260), (5, 100, 64), (1, 600, 520)], ids=str)
+def test_in_place_runs_back_to_back(cuda, shape):
+    """Each run in place takes the last one's result: as two runs between buffers."""
+    for dt in (torch.float32, torch.bfloat16):
+        x, y = matrices(shape, 11).to(dt).cuda(), torch.empty(shape, dtype=dt, device="cuda")
+        there, back = sb.Orthogonalizer([x], [y]), sb.Orthogonalizer([y], [x])
+        z = x.clone()
+        in_place = sb.Orthogonalizer([z], [z])
+        for _ in range(4):
+            in_place.run()
+            in_place.run()
+            there.run()
+            back.run()
+        torch.cuda.synchronize()
+        assert torch.equal(z, x)
 
 
 @gpu
