@@ -97,7 +97,7 @@ __device__ __forceinline__ float clipped(float raw, const StepCoeffs& k) {
 }
 
 template <int kSrc>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     __shared__ double s_red[32];
     __shared__ StepDecision s_d;
@@ -119,49 +119,69 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
         for (uint32_t q = blockIdx.x; q < a.n_prep; q += gridDim.x) {
             const PrepTile t = a.prep[q];
             const NsStack& s = a.stacks[t.stack];
-            const uint32_t rows = s.rows;
-            float* mom = s.mom;
             double acc = 0.0;
-            for (uint32_t part = 0; part < t.parts; ++part) {
-                const PrepPart p = prep_part<kSrc>(a, s, t, part);
-                float u[4][4], m[4][4];
+            // (the square of a float is exact in 64 bits; what is not in the matrix is 0)
+            auto square = [&](float x) { acc = fma(static_cast<double>(x), static_cast<double>(x), acc); };
+            if constexpr (kMuon) {
+                // A parameter's matrix is one run of elements, cut evenly whatever its columns: a tile
+                // takes vectors of four from the run's first boundary of four on, tile 0 what is
+                // before it, the last tile what is left over.
+                const uint64_t numel = static_cast<uint64_t>(s.rows) * s.cols, base = t.index * numel;
+                const uint32_t tile = q - s.first_tile - t.index * s.tiles;
+                const uint64_t chunk = ((numel + s.tiles - 1) / s.tiles + 3) & ~3ull;
+                const void* g = a.grads[s.tensor];
+                float* mom = s.mom + base;
+                const uint64_t lead = (16 - (reinterpret_cast<uintptr_t>(mom) & 15)) / 4 & 3;
+                constexpr uint32_t kElem = kIsBf16<kSrc> ? 2 : 4;
+                const bool vec = (reinterpret_cast<uintptr_t>(g) + (base + lead) * kElem) % (4 * kElem) == 0;
+                const uint64_t from = tile * chunk + lead, end = from + chunk < numel ? from + chunk : numel;
+                auto take = [&](float raw, float& m) {
+                    const float d = clipped(raw, k);
+                    m = __fadd_rn(__fmul_rn(a.momentum, m), d);
+                    square(a.nesterov ? __fadd_rn(d, __fmul_rn(a.momentum, m)) : m);
+                };
+                auto alone = [&](uint64_t i) {
+                    float one[4], m = mom[i];
+                    read4<kIsBf16<kSrc>>(g, base + i, false, 1, one);
+                    take(one[0], m);
+                    mom[i] = m;
+                };
+                if (tile == 0 && threadIdx.x < lead && threadIdx.x < numel) alone(threadIdx.x);
+                for (uint64_t i0 = from + 4 * threadIdx.x; i0 < end; i0 += 16 * kThreads) {
+                    float u[4][4], m[4][4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const bool in = p.left && p.row + 16 * i < rows;
-                    const uint64_t at = p.at + 16 * i * p.pitch;
-                    read4<kIsBf16<kSrc>>(p.src, at, p.vec && in, in ? p.left : 0, u[i]);
-                    if constexpr (kMuon) {
-                        if (p.vec && in) {
-                            *reinterpret_cast<float4*>(m[i]) = *reinterpret_cast<const float4*>(mom + at);
+                    for (uint32_t v = 0; v < 4; ++v) {
+                        const uint64_t i = i0 + v * 4 * kThreads;
+                        if (!vec || i + 4 > end) continue;
+                        read4<kIsBf16<kSrc>>(g, base + i, true, 4, u[v]);
+                        *reinterpret_cast<float4*>(m[v]) = *reinterpret_cast<const float4*>(mom + i);
+                    }
+#pragma unroll
+                    for (uint32_t v = 0; v < 4; ++v) {
+                        const uint64_t i = i0 + v * 4 * kThreads;
+                        if (vec && i + 4 <= end) {
+#pragma unroll
+                            for (uint32_t e = 0; e < 4; ++e) take(u[v][e], m[v][e]);
+                            *reinterpret_cast<float4*>(mom + i) = *reinterpret_cast<const float4*>(m[v]);
                         } else {
-#pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e) m[i][e] = in && e < p.left ? mom[at + e] : 0.0f;
+                            for (uint64_t e = i; e < end && e < i + 4; ++e) alone(e);
                         }
                     }
                 }
+            } else {
+                const uint32_t rows = s.rows;
+                for (uint32_t part = 0; part < t.parts; ++part) {
+                    const PrepPart p = prep_part<kSrc>(a, s, t, part);
+                    float u[4][4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    if constexpr (kMuon) {
+                    for (uint32_t i = 0; i < 4; ++i) {
                         const bool in = p.left && p.row + 16 * i < rows;
-                        const uint64_t at = p.at + 16 * i * p.pitch;
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            const float d = clipped(u[i][e], k);
-                            m[i][e] = __fadd_rn(__fmul_rn(a.momentum, m[i][e]), d);
-                            u[i][e] = a.nesterov ? __fadd_rn(d, __fmul_rn(a.momentum, m[i][e])) : m[i][e];
-                        }
-                        if (p.vec && in) {
-                            *reinterpret_cast<float4*>(mom + at) = *reinterpret_cast<const float4*>(m[i]);
-                        } else {
-#pragma unroll
-                            for (uint32_t e = 0; e < 4; ++e)
-                                if (in && e < p.left) mom[at + e] = m[i][e];
-                        }
+                        read4<kIsBf16<kSrc>>(p.src, p.at + 16 * i * p.pitch, p.vec && in, in ? p.left : 0, u[i]);
                     }
-                    // (the square of a float is exact in 64 bits; what is not in the matrix is 0)
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e)
-                        acc = fma(static_cast<double>(u[i][e]), static_cast<double>(u[i][e]), acc);
+                    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) square(u[i][e]);
                 }
             }
             const double sum = block_sum(acc, s_red);
