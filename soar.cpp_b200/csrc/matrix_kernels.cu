@@ -260,8 +260,10 @@ k_matrix_split(MatrixArgs a) {
         k.inv = st.inv;
         k.coef = st.coef;
     }
+    // In a Muon step the last tiles first: k_matrix_norm has left their momentum in the L2 cache,
+    // and the products begin with what comes last here (46M parameters: 1614 -> 1606 us).
     for (uint32_t q = blockIdx.x; q < a.n_prep; q += gridDim.x) {
-        const PrepTile t = a.prep[q];
+        const PrepTile t = a.prep[kMuon ? a.n_prep - 1 - q : q];
         const NsStack& s = a.stacks[t.stack];
         const float inv = a.inv[s.first + t.index];
         const uint32_t rows = s.rows, cols = s.cols, ldx = s.ldx;
