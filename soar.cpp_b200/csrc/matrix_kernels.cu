@@ -91,6 +91,12 @@ __device__ __forceinline__ PrepPart prep_part(const MatrixArgs& a, const NsStack
     return p;
 }
 
+// (Four 16-byte loads a thread leave the memory idle while the four are worked on; the next
+// four asked for ahead: 46M-parameter Muon step 1612 -> 1580 us, 200M 5950 -> 5880.)
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // Unscaled and clipped.
 __device__ __forceinline__ float clipped(float raw, const StepCoeffs& k) {
     return __fmul_rn(__fmul_rn(raw, k.inv), k.coef);
@@ -149,6 +155,16 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
                 if (tile == 0 && threadIdx.x < lead && threadIdx.x < numel) alone(threadIdx.x);
                 for (uint64_t i0 = from + 4 * threadIdx.x; i0 < end; i0 += 16 * kThreads) {
                     float u[4][4], m[4][4];
+                    if ((threadIdx.x & 7) == 0) {
+                        // the next ones' lines on their way to the L2 cache
+#pragma unroll
+                        for (uint32_t v = 4; v < 8; ++v) {
+                            const uint64_t i = i0 + v * 4 * kThreads;
+                            if (i >= end) continue;
+                            prefetch_l2(static_cast<const char*>(g) + (base + i) * kElem);
+                            prefetch_l2(mom + i);
+                        }
+                    }
 #pragma unroll
                     for (uint32_t v = 0; v < 4; ++v) {
                         const uint64_t i = i0 + v * 4 * kThreads;
@@ -272,6 +288,19 @@ k_matrix_split(MatrixArgs a) {
         for (uint32_t part = 0; part < t.parts; ++part) {
             const PrepPart p = prep_part<kSrc>(a, s, t, part);
             float u[4][4], m[4][4];
+            if (part + 1 < t.parts && (threadIdx.x & 7) == 0) {
+                // the next part's lines on their way to the L2 cache
+                const uint64_t ahead = p.at + (transposed ? kPrepTile * p.pitch : kPrepTile);
+                const uint32_t row = p.row + (transposed ? kPrepTile : 0), col = p.col + (transposed ? 0 : kPrepTile);
+                constexpr uint32_t kElem = kIsBf16<kSrc> ? 2 : 4;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    if (row + 16 * i >= rows || col >= cols) continue;
+                    if (!kMuon || a.nesterov)
+                        prefetch_l2(static_cast<const char*>(p.src) + (ahead + 16 * i * p.pitch) * kElem);
+                    if constexpr (kMuon) prefetch_l2(s.mom + ahead + 16 * i * p.pitch);
+                }
+            }
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i) {
                 const bool in = p.left && p.row + 16 * i < rows;
