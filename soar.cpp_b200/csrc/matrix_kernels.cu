@@ -1,24 +1,35 @@
 // Kernels of the matrix operators (matrix_ops.cuh): orthogonalisation by
 // Newton-Schulz products, and the Muon step around it.
 //
-//   k_matrix_norm   one pass over the matrices for their Frobenius norms; in a
-//                   Muon step the same pass unscales and clips the gradient,
-//                   updates the momentum and takes the step's decision.
-//   k_matrix_split  X = G / (|G| + eps) as fp16 hi + lo, transposed where the
-//                   matrix has more rows than columns.
-//   k_ns            every product of every matrix in one persistent kernel.
-//                   CTAs take tiles from one list in order; the list holds the
-//                   products in an order in which every tile's inputs come
-//                   before it, and a tile waits (bounded) until the tiles of
-//                   its matrix that it reads are counted as done. So a CTA
-//                   that waits, waits only for tiles that running CTAs hold,
-//                   whatever else runs on the GPU.
-//                   One warp loads operand tiles by TMA, one thread issues
-//                   tcgen05.mma into one of two TMEM accumulators, sixteen warps
-//                   turn finished accumulators into the next operand: A, B =
-//                   aI + bA + cAA, X = BX, or the result (for Muon: the
+//   k_matrix_norm   one pass over the matrices for their Frobenius norms (64-bit
+//                   sums, in a fixed order); in a Muon step the same pass
+//                   unscales and clips the gradient, updates the momentum and
+//                   takes the step's decision. Bound by memory: 200M mixed
+//                   parameters, 10 bytes each, 338 us (5.9 TB/s).
+//   k_matrix_split  X = G / (|G| + eps) as fp16 hi and lo, transposed where the
+//                   matrix has more rows than columns. Bound by memory: the
+//                   same parameters, 9 bytes each, 372 us (4.8 TB/s).
+//   k_ns            every product of every matrix in one persistent kernel, a
+//                   pair of CTAs to an SM pair. Pairs take tiles from one list
+//                   in order; the list holds the products in an order in which
+//                   every tile's inputs come before it, and a tile waits
+//                   (bounded) until the tiles of its matrix that it reads are
+//                   counted as done. So a pair that waits, waits only for
+//                   tiles that running pairs hold, whatever else runs on the
+//                   GPU. One warp loads operand tiles by TMA, one issues
+//                   tcgen05.mma into one of two TMEM accumulators, one hands
+//                   out tiles, one brings what the epilogue adds, two store,
+//                   and eight turn finished accumulators into the next operand:
+//                   A, B = aI + bA + cAA, X = BX, or the result (for Muon: the
 //                   weights' update). A and B are symmetric: only tiles on or
 //                   above the diagonal are computed, and each is stored twice.
+//                   Large matrices are bound by the products (4096 x 4096 and
+//                   2048 x 8192: 1.52 ms, 1.27 PFLOP/s with A and B
+//                   counted by half, 0.77 of the library's rate for one
+//                   large product), small ones by the epilogue (a 256 x 256 tile of
+//                   depth 320 is multiplied in 1.4 us and passed on in about
+//                   4) and by the wait from one product to the next, about 9 us.
+//   k_panel         matrices of at most 256 rows (of X), whole, by a pair each.
 #include <algorithm>
 
 #include "matrix_ops.cuh"
@@ -1394,7 +1405,9 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
 // memory for A A. So a matrix waits for nobody, and its 15 products cost two
 // exchanges with the L2 cache per iteration. (In k_ns, tiles of such matrices
 // spent most of their time waiting for one another: 64 matrices of 256 x 1024
-// took 276 us there.)
+// took 276 us there, 141 here.) With 256 rows a block takes 2.1 us an iteration,
+// 1.5 of them its two products at the measured rate of large ones; with 64 rows
+// 1.7, the products being as wide.
 //
 // Shared memory per CTA: four slots of 128 rows x 64 fp16 for A, or for the hi
 // parts of two blocks; four for B; two blocks of X (64 columns of all rows); four
