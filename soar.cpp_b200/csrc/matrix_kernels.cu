@@ -837,7 +837,7 @@ template <int kDst>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNsThreads, 1)
 k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
-    constexpr int kRing = 4;  // tasks handed out ahead
+    constexpr int kRing = 2;  // tasks handed out: one at work, one next
     constexpr int kMathWarp = 6;            // the first of them
     constexpr uint32_t kEnd = 0xFFFFFFFFu;  // stack of a task that ends the list
     extern __shared__ unsigned char smem_raw[];
@@ -1056,27 +1056,23 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     } else if (warp == 2) {
         // ---- the leader hands out tasks, to both CTAs, once their inputs are there ----
         if (rank == 0 && lane == 0) {
-            // a task is read one task ahead, and its number taken two ahead
-            NsTask ahead{};
-            uint32_t claim = atomicAdd(a.next, 1u);
-            auto read_ahead = [&]() {
-                if (claim < a.n_tasks) ahead = a.tasks[claim];
-                else ahead.stack = kEnd;
-                claim = atomicAdd(a.next, 1u);
-            };
-            read_ahead();
+            // A tile is taken only when the arithmetic begins with the last but one: a pair that
+            // holds more leaves others without, and the next product waits for it (2048 x 2048 in
+            // fp32 with two more taken ahead: 890 instead of 610 us).
             for (uint32_t q = 0;; ++q) {
                 const uint32_t slot = q % kRing;
-                const NsTask t = ahead;
+                if (q >= kRing && !bar_wait_acquire(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
+                    break;
+                const uint32_t claim = atomicAdd(a.next, 1u);
+                NsTask t{};
+                if (claim < a.n_tasks) t = a.tasks[claim];
+                else t.stack = kEnd;
                 if (t.stack != kEnd) {
-                    read_ahead();
                     if (t.need) {
                         if (!wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
                         fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
                     }
                 }
-                if (q >= kRing && !bar_wait_acquire(smem_u32(&task_empty[slot]), (q / kRing + 1) & 1, &s_err))
-                    break;
                 const uint32_t there = map_to(smem_u32(&s_task[slot]), 1);
 #pragma unroll
                 for (int i = 0; i < 3; ++i)
@@ -1417,15 +1413,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPanelThreads, 1)
 k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
     constexpr bool kMuon = kDst == kDstParamF32 || kDst == kDstParamMixed;
     constexpr int kMathWarp = 4, kMathWarps = 16;
+    constexpr int kRing = 1;  // matrices handed out ahead (46M parameters in ragged matrices: with two, 1357 us, with one 1315)
     constexpr uint32_t kEnd = 0xFFFFFFFFu;
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) uint64_t mat_full[2], mat_empty[2], mat_done;
+    __shared__ __align__(8) uint64_t mat_full[kRing], mat_empty[kRing], mat_done;
     __shared__ __align__(8) uint64_t g0_full[4], g0_empty[4];       // X's slots of the first A
     __shared__ __align__(8) uint64_t x_full[2], x_empty[2], x_done;  // blocks of X; X of an iteration written
     __shared__ __align__(8) uint64_t lo_full[4], lo_empty[4];
     __shared__ __align__(8) uint64_t hi_full[4], hi_out[4], hi_empty[4];  // for products, for stores; free
     __shared__ __align__(8) uint64_t d_full[2], d_empty[2], a_full, aa_full, a_ready, b_ready, drain_bar;
-    __shared__ __align__(16) uint4 s_mat[2];  // stack, matrix of the stack, m, n
+    __shared__ __align__(16) uint4 s_mat[kRing];  // stack, matrix of the stack, m, n
     __shared__ uint32_t s_tmem;
     __shared__ int s_err, s_drain_err;
 
@@ -1440,15 +1437,18 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
     const uint32_t a_slots = smem, b_slots = smem + 4 * kNsSlotBytes;
     const uint32_t x_blocks = b_slots + 4 * kNsSlotBytes, lo_slots = x_blocks + 2 * kPanelBlockBytes;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < kRing; ++i) {
             mbar_init(smem_u32(&mat_full[i]), 1);
-            // copies in, products, copies out, arithmetic here; all but the products there
+            // copies in, products, copies out, arithmetic and the other CTA's word here; copies and
+            // arithmetic there
             mbar_init(smem_u32(&mat_empty[i]), (rank == 0 ? 4 : 2) + kMathWarps);
+            if (rank == 1) mbar_expect_tx(smem_u32(&mat_full[i]), sizeof(uint4));
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&x_full[i]), 1);
             mbar_init(smem_u32(&x_empty[i]), 1);
             mbar_init(smem_u32(&d_full[i]), 1);
             mbar_init(smem_u32(&d_empty[i]), 2 * kMathWarps);
-            if (rank == 1) mbar_expect_tx(smem_u32(&mat_full[i]), sizeof(uint4));
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(smem_u32(&g0_full[i]), 1);
@@ -1493,8 +1493,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         const uint32_t lead_g0 = uniform(lead(&g0_full[0])), lead_x = uniform(lead(&x_full[0]));
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
-            const uint32_t slot = q & 1;
-            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            const uint32_t slot = q % kRing;
+            ok = warp_wait(smem_u32(&mat_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const uint32_t stack = uniform(s_mat[slot].x), index = uniform(s_mat[slot].y);
             const uint32_t m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
@@ -1578,8 +1578,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
             for (uint32_t k = 1; k < 4; ++k) mma_f16(d, da + k * 2, db + k * db_k, idesc, true);
         };
         for (uint32_t q = 0; rank == 0 && ok; ++q) {
-            const uint32_t slot = q & 1;
-            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            const uint32_t slot = q % kRing;
+            ok = warp_wait(smem_u32(&mat_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const uint32_t stack = uniform(s_mat[slot].x), m = uniform(s_mat[slot].z), n = uniform(s_mat[slot].w);
             __syncwarp();
@@ -1657,14 +1657,15 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         // ---- the leader hands out matrices, to both CTAs ----
         if (rank == 0 && lane == 0) {
             for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q & 1, claim = atomicAdd(a.next + 1, 1u);
+                const uint32_t slot = q % kRing;
+                if (q >= kRing && !bar_wait_acquire(smem_u32(&mat_empty[slot]), (q / kRing + 1) & 1, &s_err)) break;
+                const uint32_t claim = atomicAdd(a.next + 1, 1u);
                 uint4 w = make_uint4(kEnd, 0, 0, 0);
                 if (claim < a.n_panels) {
                     const uint2 p = a.panels[claim];
                     const NsStack& s = a.stacks[p.x];
                     w = make_uint4(p.x, p.y, s.m, s.n);
                 }
-                if (q >= 2 && !bar_wait_acquire(smem_u32(&mat_empty[slot]), (q >> 1 ^ 1) & 1, &s_err)) break;
                 st_async_v4(map_to(smem_u32(&s_mat[slot]), 1), w, map_to(smem_u32(&mat_full[slot]), 1));
                 s_mat[slot] = w;
                 mbar_arrive(smem_u32(&mat_full[slot]));
@@ -1673,10 +1674,10 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         } else if (rank == 1 && lane == 0) {
             // (as in k_ns: this CTA's reads of a slot come before the leader's next write into it)
             for (uint32_t q = 0;; ++q) {
-                const uint32_t slot = q & 1;
-                if (!bar_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err)) break;
+                const uint32_t slot = q % kRing;
+                if (!bar_wait(smem_u32(&mat_full[slot]), (q / kRing) & 1, &s_err)) break;
                 if (s_mat[slot].x == kEnd) break;
-                if (!bar_wait(smem_u32(&mat_empty[slot]), q >> 1 & 1, &s_err)) break;
+                if (!bar_wait(smem_u32(&mat_empty[slot]), (q / kRing) & 1, &s_err)) break;
                 mbar_arrive_release(map_to(smem_u32(&mat_empty[slot]), 0));
             }
         }
@@ -1686,8 +1687,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         uint32_t out_phase = 0;
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
-            const uint32_t slot = q & 1;
-            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            const uint32_t slot = q % kRing;
+            ok = warp_wait(smem_u32(&mat_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const uint4 w = s_mat[slot];
             __syncwarp();
@@ -1744,8 +1745,8 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         uint32_t a_phase = 0, d_phase = 0, lo_phase = 0, hi_phase = 0, hi_used = 0;
         bool ok = true;
         for (uint32_t q = 0; ok; ++q) {
-            const uint32_t slot = q & 1;
-            ok = warp_wait(smem_u32(&mat_full[slot]), q >> 1 & 1, &s_err);
+            const uint32_t slot = q % kRing;
+            ok = warp_wait(smem_u32(&mat_full[slot]), (q / kRing) & 1, &s_err);
             if (!ok) break;
             const uint4 w = s_mat[slot];
             __syncwarp();

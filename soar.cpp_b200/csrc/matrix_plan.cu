@@ -244,12 +244,16 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
 
     // The tasks, in an order in which every tile's inputs come before it: lists
     // ("waves") of matrices go through their products side by side, one list
-    // after another. A list is long enough that a product of it occupies every
-    // pair of CTAs three times (or the tiles of its next product wait for the
-    // last of this one: at 1, 2, 3, 4 and 6 times, 200M parameters in layers
-    // 1024 wide took 6.40, 6.00, 5.69, 5.82 and 5.85 ms a step), and else as short
-    // as half of the L2 cache, which then holds its operands.
-    constexpr uint64_t kWaveBytes = 64ull << 20;
+    // after another, all about as long. A product's last tiles are waited for by
+    // the first ones of its matrix's next product, for some 10 us, which the other
+    // matrices of the list have to fill: with 64 MB in a list 46M parameters in
+    // matrices of many shapes took 1573 us a step, with 128 MB and more 1414, and a
+    // short last list cost 80. Nor does the L2 cache ask for short ones (200M
+    // parameters in layers 1024 wide: 5.94 ms with 64 MB, 5.87 with 256 MB). A
+    // list of few tiles is drawn out until a product of it occupies every pair of
+    // CTAs three times (that model with lists by tiles alone: 6.40, 6.00, 5.69 ms
+    // at one, two and three times).
+    constexpr uint64_t kWaveBytes = 256ull << 20;
     const uint64_t wave_tiles = 3 * static_cast<uint64_t>(plan->sms) / 2;
     std::vector<NsTask> tasks;
     struct Run {
@@ -297,23 +301,30 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         wave.clear();
         wave_bytes = 0;
     };
+    auto bytes_of = [&](const NsStack& s) {
+        return s.m * ((three ? 8ull : 6ull) * s.ldx + (three ? 8ull : 4ull) * s.lda);
+    };
+    uint64_t all_bytes = 0;
+    for (const NsStack& s : stacks)
+        if (!s.panel) all_bytes += s.count * bytes_of(s);
+    const uint64_t wave_most = all_bytes / std::max<uint64_t>(1, all_bytes / kWaveBytes) + 1;
     uint64_t tiles_in_wave = 0;
     for (uint32_t si = 0; si < stacks.size(); ++si) {
         const NsStack& s = stacks[si];
         if (s.panel) continue;
-        const uint64_t each = s.m * ((three ? 8ull : 6ull) * s.ldx + (three ? 8ull : 4ull) * s.lda);
+        const uint64_t each = bytes_of(s);
         const uint64_t tiles = product_tiles(s, kNsXXt, kNsTileN).size();
         for (uint32_t i = 0; i < s.count;) {
             // as many as the wave still takes: until it has both the bytes and the tiles
             uint64_t k = 1;
-            if (wave_bytes < kWaveBytes) k = std::max(k, (kWaveBytes - wave_bytes) / each);
+            if (wave_bytes < wave_most) k = std::max(k, (wave_most - wave_bytes) / each);
             if (tiles_in_wave < wave_tiles) k = std::max(k, (wave_tiles - tiles_in_wave) / tiles);
             k = std::min<uint64_t>(k, s.count - i);
             wave.push_back({si, i, i + static_cast<uint32_t>(k)});
             wave_bytes += each * k;
             tiles_in_wave += tiles * k;
             i += static_cast<uint32_t>(k);
-            if (wave_bytes >= kWaveBytes && tiles_in_wave >= wave_tiles) {
+            if (wave_bytes >= wave_most && tiles_in_wave >= wave_tiles) {
                 flush();
                 tiles_in_wave = 0;
             }
