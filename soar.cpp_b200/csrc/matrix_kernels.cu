@@ -24,8 +24,8 @@
 //                   weights' update). A and B are symmetric: only tiles on or
 //                   above the diagonal are computed, and each is stored twice.
 //                   Large matrices are bound by the products (4096 x 4096 and
-//                   2048 x 8192: 1.52 ms, 1.27 PFLOP/s with A and B
-//                   counted by half, 0.77 of the library's rate for one
+//                   2048 x 8192: 1.49 ms, 1.30 PFLOP/s with A and B
+//                   counted by half, 0.79 of the library's rate for one
 //                   large product), small ones by the epilogue (a 256 x 256 tile of
 //                   depth 320 is multiplied in 1.4 us and passed on in about
 //                   4) and by the wait from one product to the next, about 9 us.
