@@ -174,8 +174,8 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     // k_panel or k_ns for a matrix of at most 256 rows (of X). k_panel gives it to one pair of CTAs
     // for 30 us + 0.075 us a column, k_ns deals its tiles to all pairs but goes through 15 products
     // one after the other. One 256 x 1024 matrix takes 120 us in either, 256 x 512 79 in k_panel and
-    // 112 in k_ns, 256 x 4096 376 and 172; 37 of 256 x 4096 (half the pairs) 528 and 502, 74 of them
-    // 702 and 877. So long matrices go to k_panel where the list has enough columns for all pairs.
+    // 109 in k_ns, 256 x 4096 376 and 171; 37 of 256 x 4096 (half the pairs) 546 and 516, 74 of them
+    // 731 and 906. So long matrices go to k_panel where the list has enough columns for all pairs.
     uint64_t panel_columns = 0;
     for (int i = 0; i < n_specs; ++i)
         if (!three && specs[i].rows && specs[i].cols && std::min(specs[i].rows, specs[i].cols) <= kPanelSide)
