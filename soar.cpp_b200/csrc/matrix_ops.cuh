@@ -13,8 +13,8 @@
 // products of small entries lose lo. A rounding of X's small singular directions would otherwise grow by
 // a factor of a (3.4) per iteration: with X in hi alone, a matrix of a few
 // strong directions over noise comes out 0.6 % to 7 % off (bf16 operands: 5 %
-// to 60 %), with hi + lo 0.04 % to 0.25 %. That is below the rounding of a bf16
-// result (0.17 % rms). For fp32 results lo is an fp16 number too, of A and B as
+// to 60 %), with hi + lo 0.04 % to 0.25 %, about what the rounding of a bf16
+// result costs (0.17 % rms). For fp32 results lo is an fp16 number too, of A and B as
 // well, and every product is taken as hi hi + hi lo + lo hi (22 bits). The tensor
 // cores round a sum towards zero at each addition, so there the large terms come
 // last and half of them have an accumulator of their own (2048 x 2048: 4.6e-6 off
