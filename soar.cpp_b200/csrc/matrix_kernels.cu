@@ -113,9 +113,50 @@ __device__ __forceinline__ float clipped(float raw, const StepCoeffs& k) {
     return __fmul_rn(__fmul_rn(raw, k.inv), k.coef);
 }
 
+// 2^k, for -126 <= k <= 127.
+__device__ __forceinline__ float pow2(int k) { return __uint_as_float(static_cast<uint32_t>(127 + k) << 23); }
+
+// From a matrix's norm: what its X is held by before each step (powers of two), and what
+// its elements are multiplied by at the start (by x, then by y: numbers at the end of fp32's
+// range need more than one factor). `bound` is one of X's singular values, which
+// a step multiplies by at most |a| + |b| bound^2 + |c| bound^4: they are held at 1/2 to 1 times
+// sx, or, from a bound of 1/2 on, times sx itself.
+__device__ __noinline__ float2 hold_lifted(const MatrixArgs& a, float sx, double norm, NsHold* hold) {
+    constexpr int kMostLift = 100;
+    const double full = norm + a.eps;
+    // (NaN for zeros with an eps of 0 and of an inf or NaN: not lifted)
+    float bound = static_cast<float>(norm / full);
+    auto scale_of = [&]() {
+        if (!(bound < 0.5f)) return sx;
+        return sx * pow2(min(kMostLift, 126 - static_cast<int>(__float_as_uint(bound) >> 23)));
+    };
+    float scale = scale_of();
+    float2 inv = make_float2(0.0f, 1.0f);  // (zeros with an eps of 0 stay zeros)
+    if (full != 0.0) {
+        const double q = static_cast<double>(scale) / full;
+        if (q >= 0x1p64) inv = make_float2(static_cast<float>(q * 0x1p-64), 0x1p64f);
+        else inv.x = static_cast<float>(q);
+    }
+    for (int i = 0; i < a.steps; ++i) {
+        const float* c = a.coef[i];
+        const float s2 = bound * bound, one_over = __fdiv_rn(1.0f, scale);
+        bound *= fabsf(c[0]) + s2 * (fabsf(c[1]) + s2 * fabsf(c[2]));
+        scale = scale_of();
+        hold[i] = NsHold{one_over, scale * one_over};
+    }
+    return inv;
+}
+__device__ __forceinline__ float2 hold_x(const MatrixArgs& a, const NsStack& s, double norm, NsHold* hold) {
+    const double q = static_cast<double>(s.sx) / (norm + a.eps);
+    // (a bound of 1/2 or more stays one)
+    if (!(norm >= a.eps && q < 0x1p64 && a.grows)) return hold_lifted(a, s.sx, norm, hold);
+    for (int i = 0; i < a.steps; ++i) hold[i] = NsHold{s.one_over_sx, 1.0f};
+    return make_float2(static_cast<float>(q), 1.0f);
+}
+
 template <int kSrc>
 __global__ void __launch_bounds__(kThreads, 4)
-k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
+k_matrix_norm(const __grid_constant__ MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     __shared__ double s_red[32];
     __shared__ StepDecision s_d;
     __shared__ int s_last;
@@ -227,7 +268,7 @@ k_matrix_norm(MatrixArgs a, Ctl* ctl, ApplyArgs step) {
                 for (uint32_t i = threadIdx.x; i < s.tiles; i += kThreads) v += __ldcg(p + i);
                 const double total = block_sum(v, s_red);
                 if (threadIdx.x == 0) {
-                    a.inv[matrix] = static_cast<float>(static_cast<double>(s.sx) / (sqrt(total) + a.eps));
+                    a.inv[matrix] = hold_x(a, s, sqrt(total), a.hold + static_cast<uint64_t>(matrix) * a.steps);
                     a.tickets[matrix] = 0u;
                 }
             }
@@ -292,7 +333,7 @@ k_matrix_split(MatrixArgs a) {
     for (uint32_t q = blockIdx.x; q < a.n_prep; q += gridDim.x) {
         const PrepTile t = a.prep[kMuon ? a.n_prep - 1 - q : q];
         const NsStack& s = a.stacks[t.stack];
-        const float inv = a.inv[s.first + t.index];
+        const float2 inv = a.inv[s.first + t.index];
         const uint32_t rows = s.rows, cols = s.cols, ldx = s.ldx;
         const bool transposed = s.transposed != 0;
         const uint64_t matrix = static_cast<uint64_t>(t.index) * s.m * ldx;
@@ -334,7 +375,8 @@ k_matrix_split(MatrixArgs a) {
                 for (uint32_t e = 0; e < 4; ++e) {
                     if constexpr (kMuon)
                         u[i][e] = a.nesterov ? __fadd_rn(clipped(u[i][e], k), __fmul_rn(a.momentum, m[i][e])) : m[i][e];
-                    u[i][e] = __fmul_rn(u[i][e], inv);
+                    u[i][e] = __fmul_rn(u[i][e], inv.x);
+                    if (inv.y != 1.0f) u[i][e] = __fmul_rn(u[i][e], inv.y);
                 }
                 if (!transposed) {
                     if (p.left && r < rows) put_x4(s, matrix + static_cast<uint64_t>(r) * ldx + p.col, u[i]);
@@ -1068,6 +1110,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (claim < a.n_tasks) t = a.tasks[claim];
                 else t.stack = kEnd;
                 if (t.stack != kEnd) {
+                    t.hold = a.hold[static_cast<uint64_t>(t.matrix) * a.steps + t.step()];
                     if (t.need) {
                         if (!wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
                         fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
@@ -1235,9 +1278,11 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
             const float ca = a.coef[t.step()][0], cb = a.coef[t.step()][1], cc = a.coef[t.step()][2];
             const bool two = u.three && (t.kind() == kNsXXt ? t.n : t.m) > kNsTileK;  // two accumulators
             // v = fv accumulator + fx addend (+ ca on the diagonal)
-            const float fx = u.sym ? cb : ca;
-            const float fv = t.kind() == kNsXXt ? kNsScaleA / (t.sx * t.sx)
-                                                : t.kind() == kNsAA ? cc / kNsScaleA : 1.0f / kNsScaleA;
+            const float regrade = last ? 1.0f : t.hold.regrade;
+            const float fx = u.sym ? cb : ca * regrade;
+            const float fv = t.kind() == kNsXXt  ? kNsScaleA * t.hold.inv * t.hold.inv
+                             : t.kind() == kNsAA ? cc / kNsScaleA
+                                                 : regrade / kNsScaleA;
             if (!warp_wait(smem_u32(&acc_full[buf]), (q / 2) & 1, &s_err)) break;
             tc_fence_after();
             bool ok = true, held = true;
@@ -1299,7 +1344,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (last) {
                     // through shared memory as floats, the warp's own 32 rows, so that the result is
                     // written along the rows of the caller's matrix
-                    const float f = 1.0f / t.sx;
+                    const float f = t.hold.inv;
                     float* fs = reinterpret_cast<float*>(smem_raw + (at - smem_u32(smem_raw)));
 #pragma unroll
                     for (int j = 0; j < 64; ++j) fs[float_at(trow, j)] = v[j] * f;
@@ -1754,12 +1799,15 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
             if (w.x == kEnd) break;
             const NsStack& s = a.stacks[w.x];
             const uint32_t m = w.z, n = w.w, kb = (m + 63) / 64, chunks = (n + 63) / 64, blocks = (chunks + 1) / 2;
-            const float sx = s.sx;
+            const NsHold* hold = a.hold + static_cast<uint64_t>(s.first + w.y) * steps;
             const bool transposed = s.transposed != 0;
             const Target target = target_of<kDst>(s, w.y, step, a.ema != 0);
             for (uint32_t it = 0; it < steps && ok; ++it) {
-                const float ca = a.coef[it][0], cb = a.coef[it][1], cc = a.coef[it][2];
                 const bool last = it + 1 == steps;
+                const NsHold held = hold[it];
+                // (B and the addend carry the next iteration's scale)
+                const float regrade = last ? 1.0f : held.regrade;
+                const float ca = a.coef[it][0] * regrade, cb = a.coef[it][1] * regrade, cc = a.coef[it][2] * regrade;
                 // A, from its accumulator to shared memory (the slots' last blocks have left them)
                 ok = warp_wait(smem_u32(&a_full), a_phase, &s_err);
                 for (uint32_t h = 0; h < 4 && ok; ++h)
@@ -1770,7 +1818,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                     float v[32];
                     __syncwarp();
                     tmem_ld32(lanes + 256 + c * 64 + part * 32, v);
-                    const float f = kNsScaleA / (sx * sx);
+                    const float f = kNsScaleA * held.inv * held.inv;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t h[4];
@@ -1841,7 +1889,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
                         // through shared memory as floats, the warp's own 32 rows, so that the result
                         // is written along the rows of the caller's matrix (in the group's two slots,
                         // which nothing else uses by now)
-                        const float f = 1.0f / sx;
+                        const float f = held.inv;
                         float* fs = reinterpret_cast<float*>(
                             smem_raw + (a_slots - smem_u32(smem_raw) + group * 2 * kNsSlotBytes));
                         __syncwarp();

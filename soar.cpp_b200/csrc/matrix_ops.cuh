@@ -24,7 +24,11 @@
 // (within 2^6 .. 2^12), which gives its elements an rms of about 1 at the start
 // and of at most sqrt(m) at the end; A and B are held times 2^10, where their
 // eigenvalues (at most about 1.5, and 4) stay below 2^12 and entries down to
-// 2^-34 still count.
+// 2^-34 still count. Where eps is larger than |G|, X starts at |G| / (|G| + eps) and
+// grows by a factor of a an iteration: it is then held by a larger power of two, before
+// every iteration the one that a bound on its singular values allows
+// (NsHold), so that its parts keep their bits (with sx alone, fp32 results for
+// |G| = 1e-12 and eps = 1e-7 came out 0.35 % off, below 1e-16 as zeros).
 #pragma once
 
 #include <cstdint>
@@ -92,6 +96,12 @@ constexpr int kMap32 = 2;  // from A's K128 map to its last
 constexpr int kMap64 = 1;  // from a K128 (N128) map to its K64 (N64) one
 constexpr int kMapN = 2;   // from X's K maps to its N maps
 
+// One over the power of two that a matrix's X is held by before an iteration, and what it is
+// held by after that over what it was held by before.
+struct __align__(8) NsHold {
+    float inv, regrade;
+};
+
 // One stack of equal matrices.
 struct NsStack {
     __half* x[2];   // X hi, double-buffered across iterations: [count][m][ldx]
@@ -110,7 +120,7 @@ struct NsStack {
     uint32_t panel;       // worked on by k_panel
     uint32_t tiles;       // preparation tiles per matrix
     uint32_t first_tile;
-    float sx;             // power of two X is held by
+    float sx, one_over_sx;  // power of two X is held by at least (NsHold)
     // input and output of a plain orthogonalisation; row and matrix strides in elements
     const void* src;
     void* dst;
@@ -143,10 +153,10 @@ struct __align__(16) NsTask {
     uint32_t shape;   // columns | kind << 16 | three products << 20 | transposed << 21 | step << 24
     // of the stack, so that a tile needs one read
     uint32_t m, n;
-    float sx;
     uint32_t matrix;  // matrix of the plan
     uint32_t need;    // CTAs' tiles of this matrix that must be done before
-    uint32_t pad[3];
+    NsHold hold;      // the matrix's before the step, read as the task is handed out
+    uint32_t pad[2];
 
     __host__ __device__ uint32_t row() const { return (place & 0xFFFFu) * kNsTileM; }
     __host__ __device__ uint32_t col() const { return (place >> 16) * 32u; }
@@ -178,13 +188,15 @@ struct MatrixArgs {
     uint32_t n_matrices;
     double* partials;      // one per preparation tile
     uint32_t* tickets;     // per matrix: preparation tiles summed (0 between launches)
-    float* inv;            // per matrix: sx / (norm + eps)
+    float2* inv;           // per matrix: what X is held by at first / (norm + eps), in two factors
+    NsHold* hold;          // per matrix, per step
     uint32_t* done;        // per matrix: product tiles done, counted by each CTA with rows in one
     uint32_t* next;        // tasks handed out, and k_panel's matrices
     int steps;
     MatrixStep* step;
     int* err;              // nonzero: a wait ran out
     float coef[kNsMaxSteps][3];
+    int grows;             // every |a| is at least 1: a step does not shrink a bound on X's singular values
     double eps;
     const void* const* grads;  // Muon: gradient per tensor
     float momentum;

@@ -201,6 +201,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         const int lg = static_cast<int>(
             std::floor(0.5 * std::log2(static_cast<double>(s.m) * static_cast<double>(s.n))));
         s.sx = std::ldexp(1.0f, std::min(12, std::max(6, lg)));
+        s.one_over_sx = 1.0f / s.sx;
         s.src = q.src;
         s.dst = q.dst;
         s.src_row = q.src_row;
@@ -287,7 +288,6 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                                       s.three << 20 | s.transposed << 21 | static_cast<uint32_t>(step) << 24;
                             k.m = s.m;
                             k.n = s.n;
-                            k.sx = s.sx;
                             k.matrix = s.first + i;
                             k.need = counted[w];
                             tasks.push_back(k);
@@ -355,7 +355,8 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     const size_t o_panels = take(panels.size() * sizeof(uint2));
     const size_t tables_end = off;
     const size_t o_partials = take(prep.size() * sizeof(double));
-    const size_t o_inv = take(matrices * sizeof(float));
+    const size_t o_inv = take(matrices * sizeof(float2));
+    const size_t o_hold = take(matrices * opts.steps * sizeof(NsHold));
     const size_t zero_from = off;
     const size_t o_tickets = take(matrices * sizeof(uint32_t));
     const size_t o_done = take(matrices * sizeof(uint32_t));
@@ -440,13 +441,17 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     a.steps = opts.steps;
     a.n_matrices = static_cast<uint32_t>(matrices);
     a.partials = reinterpret_cast<double*>(at(o_partials));
-    a.inv = reinterpret_cast<float*>(at(o_inv));
+    a.inv = reinterpret_cast<float2*>(at(o_inv));
+    a.hold = reinterpret_cast<NsHold*>(at(o_hold));
     a.tickets = reinterpret_cast<uint32_t*>(at(o_tickets));
     a.done = reinterpret_cast<uint32_t*>(at(o_done));
     a.next = reinterpret_cast<uint32_t*>(at(o_words));
     a.step = reinterpret_cast<MatrixStep*>(at(o_words + 64));
     a.err = opts.err ? opts.err : reinterpret_cast<int*>(at(o_words + 128));
     std::memcpy(a.coef, opts.coef, sizeof a.coef);
+    a.grows = 1;
+    for (int i = 0; i < opts.steps; ++i)
+        if (!(std::fabs(opts.coef[i][0]) >= 1.0f)) a.grows = 0;
     a.eps = opts.eps;
     return plan.release();
 }
