@@ -208,7 +208,8 @@ SOAR_API int soar_ortho_create(const soar_matrix_desc* mats, int n_mats,
    graphs included. */
 SOAR_API int soar_ortho_run(void* handle, void* stream);
 /* Nonzero in *out_error if a device-side wait of some run timed out: that
-   run's results must not be used (synchronises the device). */
+   run's results must not be used (synchronises the device). The word stays for
+   the handle's life; later runs are whole again, unless they time out too. */
 SOAR_API int soar_ortho_error(void* handle, int* out_error);
 SOAR_API int soar_ortho_destroy(void* handle);
 

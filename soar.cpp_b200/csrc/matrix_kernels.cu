@@ -167,6 +167,7 @@ k_matrix_norm(const __grid_constant__ MatrixArgs a, Ctl* ctl, ApplyArgs step) {
     for (uint32_t i = blockIdx.x * kThreads + threadIdx.x; i < a.n_matrices; i += gridDim.x * kThreads)
         a.done[i] = 0u;
     if (blockIdx.x == 0 && threadIdx.x < 2) a.next[threadIdx.x] = 0u;
+    if (blockIdx.x == 0 && threadIdx.x == 2) *a.gave_up = 0u;
     StepCoeffs k{1.0f, 1.0f, 0.0f, 1.0f, 1};
     if constexpr (kMuon) {
         if (threadIdx.x == 0) s_d = decide_step(step, ctl);
@@ -604,13 +605,13 @@ __device__ __forceinline__ void red_release_add1(uint32_t* p) {
     asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p) : "memory");
 }
 
-// Bounded wait until *p >= need; gives up when the kernel's error word is set.
+// Bounded wait until *p >= need; gives up when another CTA of this run has.
 __device__ __forceinline__ bool wait_done(const uint32_t* p, uint32_t need, int* s_err,
-                                          const int* err) {
+                                          const uint32_t* gave_up) {
     Patience wait;
     while (ld_acquire(p) < need) {
         if (!wait.more(s_err)) return false;
-        if ((wait.tries & 1023u) == 0 && *reinterpret_cast<const volatile int*>(err)) {
+        if ((wait.tries & 1023u) == 0 && *reinterpret_cast<const volatile uint32_t*>(gave_up)) {
             atomicOr(s_err, 1);
             return false;
         }
@@ -1112,7 +1113,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
                 if (t.stack != kEnd) {
                     t.hold = a.hold[static_cast<uint64_t>(t.matrix) * a.steps + t.step()];
                     if (t.need) {
-                        if (!wait_done(a.done + t.matrix, t.need, &s_err, a.err)) break;
+                        if (!wait_done(a.done + t.matrix, t.need, &s_err, a.gave_up)) break;
                         fence_async_proxy();  // (other SMs' stores, by TMA, before loads by TMA)
                     }
                 }
@@ -1425,6 +1426,7 @@ k_ns(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs ste
     __syncthreads();
     if (threadIdx.x == 0 && (s_err | s_drain_err)) {
         atomicOr(a.err, 1);
+        atomicOr(a.gave_up, 1u);
         // the other CTA's copies may still be landing here, or counting on barriers here
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 2000000ull) {}
@@ -1938,6 +1940,7 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
     __syncthreads();
     if (threadIdx.x == 0 && (s_err | s_drain_err)) {
         atomicOr(a.err, 1);
+        atomicOr(a.gave_up, 1u);
         // the other CTA's copies may still be landing here, or counting on barriers here
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 2000000ull) {}

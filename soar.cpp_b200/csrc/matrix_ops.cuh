@@ -194,7 +194,8 @@ struct MatrixArgs {
     uint32_t* next;        // tasks handed out, and k_panel's matrices
     int steps;
     MatrixStep* step;
-    int* err;              // nonzero: a wait ran out
+    int* err;              // nonzero: a wait ran out in some run (stays)
+    uint32_t* gave_up;     // nonzero: a wait ran out in this run (0 at its start): others need not wait
     float coef[kNsMaxSteps][3];
     int grows;             // every |a| is at least 1: a step does not shrink a bound on X's singular values
     double eps;

@@ -446,6 +446,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     a.tickets = reinterpret_cast<uint32_t*>(at(o_tickets));
     a.done = reinterpret_cast<uint32_t*>(at(o_done));
     a.next = reinterpret_cast<uint32_t*>(at(o_words));
+    a.gave_up = a.next + 2;
     a.step = reinterpret_cast<MatrixStep*>(at(o_words + 64));
     a.err = opts.err ? opts.err : reinterpret_cast<int*>(at(o_words + 128));
     std::memcpy(a.coef, opts.coef, sizeof a.coef);
