@@ -176,7 +176,8 @@ enum soar_dtype {
 };
 
 /* A stack of `count` rows x cols matrices. Elements of a row are adjacent;
-   strides are in elements: `*_row` between rows, `*_mat` between matrices. */
+   strides are in elements: `*_row` between rows, `*_mat` between matrices.
+   Destinations of a list may interleave, but not share elements. */
 typedef struct soar_matrix_desc {
     const void* src;    /* device; read only */
     void* dst;          /* device; may be src itself (same type and strides) */
@@ -256,7 +257,8 @@ typedef struct soar_muon_opts {
 } soar_muon_opts;
 
 SOAR_API void soar_muon_default_opts(soar_muon_opts* out);
-/* shapes[i]: tensor i's shape; its product must be tensors[i].numel. */
+/* shapes[i]: tensor i's shape; its product must be tensors[i].numel. Parameters
+   must not share elements. */
 SOAR_API int soar_muon_create(const soar_tensor_desc* tensors, const soar_matrix_shape* shapes,
                               int n_tensors, const soar_muon_opts* opts, void** out_handle);
 

@@ -33,6 +33,7 @@
 
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -218,6 +219,15 @@ cudaError_t launch_matrix_ops(const MatrixArgs& args, int source, int dest, Ctl*
 // ---- host: plans (matrix_plan.cu) ----
 // Whether a stack's shape can be planned (a stack without elements can).
 bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* why);
+// A stack that is written: `count` matrices of `rows` rows of `width` bytes, which do not
+// overlap one another; strides in bytes.
+struct MatrixSpan {
+    uint64_t base;
+    uint64_t count, rows, width, row, mat;
+    int index;  // of the caller's list
+};
+// Whether no two of them share a byte; else the indices of two that do.
+bool matrix_spans_apart(std::vector<MatrixSpan> spans, int* one, int* other);
 // The quintic's usual coefficients, for every step.
 void matrix_default_coef(float (*coef)[3]);
 struct MatrixSpec {

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <queue>
 #include <vector>
 
 #include <cudaTypedefs.h>
@@ -112,6 +113,59 @@ bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* 
     if (count > 0x7FFFFFFFull) {
         *why = "more than 2^31 - 1 matrices";
         return false;
+    }
+    return true;
+}
+
+namespace {
+// A span's rows one after another, by their addresses.
+struct SpanRows {
+    const MatrixSpan* s;
+    bool by_matrix;  // all of a matrix's rows come before the next matrix's
+    uint64_t matrix = 0, row = 0;
+    uint64_t begin() const { return s->base + matrix * s->mat + row * s->row; }
+    bool next() {
+        uint64_t& inner = by_matrix ? row : matrix;
+        uint64_t& outer = by_matrix ? matrix : row;
+        if (++inner < (by_matrix ? s->rows : s->count)) return true;
+        inner = 0;
+        return ++outer < (by_matrix ? s->count : s->rows);
+    }
+};
+uint64_t span_end(const MatrixSpan& s) { return s.base + (s.count - 1) * s.mat + (s.rows - 1) * s.row + s.width; }
+}  // namespace
+
+bool matrix_spans_apart(std::vector<MatrixSpan> spans, int* one, int* other) {
+    for (MatrixSpan& s : spans) {
+        if (s.rows > 1 && s.row == s.width) s.width *= s.rows, s.rows = 1;
+        if (s.rows == 1 && s.count > 1 && s.mat == s.width) s.width *= s.count, s.count = 1;
+    }
+    std::sort(spans.begin(), spans.end(), [](const MatrixSpan& x, const MatrixSpan& y) { return x.base < y.base; });
+    // those that reach into one another, row by row
+    for (size_t i = 0, j; i < spans.size(); i = j) {
+        uint64_t end = span_end(spans[i]);
+        for (j = i + 1; j < spans.size() && spans[j].base < end; ++j) end = std::max(end, span_end(spans[j]));
+        if (j == i + 1) continue;
+        auto later = [](const SpanRows& x, const SpanRows& y) { return x.begin() > y.begin(); };
+        std::priority_queue<SpanRows, std::vector<SpanRows>, decltype(later)> rows(later);
+        for (size_t k = i; k < j; ++k) {
+            const MatrixSpan& s = spans[k];
+            rows.push({&s, s.count == 1 || s.mat >= (s.rows - 1) * s.row + s.width});
+        }
+        uint64_t taken = 0;
+        int by = -1;
+        while (!rows.empty()) {
+            SpanRows r = rows.top();
+            rows.pop();
+            if (r.begin() < taken) {
+                *one = std::min(by, r.s->index);
+                *other = std::max(by, r.s->index);
+                return false;
+            }
+            taken = r.begin() + r.s->width;
+            by = r.s->index;
+            if (r.next()) rows.push(r);
+        }
     }
     return true;
 }

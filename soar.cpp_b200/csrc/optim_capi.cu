@@ -435,6 +435,7 @@ bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::stri
         return false;
     }
     std::unordered_set<const void*> taken;
+    std::vector<soarb::MatrixSpan> spans;
     for (int i = 0; i < n; ++i) {
         const soar_matrix_shape& s = p.shapes[i];
         if (!soarb::matrix_shape_ok(s.count, s.rows, s.cols, why)) {
@@ -449,6 +450,14 @@ bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::stri
             *why = "tensor " + std::to_string(i) + ": another tensor has the same parameters";
             return false;
         }
+        const uint64_t eb = o.layout == SOAR_LAYOUT_BF16_MIXED ? 2 : 4;
+        if (t[i].numel && t[i].param && t[i].grad)  // (the others stay as they are)
+            spans.push_back({reinterpret_cast<uintptr_t>(t[i].param), 1, 1, t[i].numel * eb, 0, 0, i});
+    }
+    int one = 0, other = 0;
+    if (!soarb::matrix_spans_apart(std::move(spans), &one, &other)) {
+        *why = "tensors " + std::to_string(one) + " and " + std::to_string(other) + ": their parameters overlap";
+        return false;
     }
     return true;
 }

@@ -68,6 +68,7 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
     const uint64_t db = opts->dst_type == SOAR_DTYPE_BF16 ? 2 : 4;
     std::vector<soarb::MatrixSpec> specs;
     std::unordered_set<const void*> taken;
+    std::vector<soarb::MatrixSpan> spans;
     for (int i = 0; i < n; ++i) {
         const soar_matrix_desc& d = mats[i];
         const std::string at = "stack " + std::to_string(i) + ": ";
@@ -99,7 +100,13 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
         q.dst_row = d.dst_row;
         q.dst_mat = d.dst_mat;
         specs.push_back(q);
+        spans.push_back({reinterpret_cast<uintptr_t>(d.dst), d.count, d.rows, d.cols * db, d.dst_row * db,
+                         d.dst_mat * db, i});
     }
+    int one = 0, other = 0;
+    if (!soarb::matrix_spans_apart(std::move(spans), &one, &other))
+        return fail("stacks " + std::to_string(one) + " and " + std::to_string(other) +
+                    ": their destinations overlap");
     DeviceGuard g(opts->device);
     if (!g.ok) return fail("cannot select device " + std::to_string(opts->device));
     soarb::MatrixPlanOpts mo;
