@@ -165,8 +165,9 @@ SOAR_API int soar_sgd_create(const soar_tensor_desc* tensors, int n_tensors,
    operands have 22 bits and every product is taken in three parts, about as
    exact as fp32 products (sides up to about 2048; the sums' rounding grows with
    the side). Norms far below eps keep that too: X, which is tiny then, is held
-   by a power of two of its own before every step. The coefficients have to keep X's singular values below 8 and
-   |a + b s^2 + c s^4| at them below 60 (fp16's range), as the default ones do.
+   by a power of two of its own before every step. Coefficients that do not
+   keep X's singular values below 7.99 and |a + b s^2 + c s^4| at them up to 60
+   (fp16's range), from singular values of up to 1, are refused.
    Sides are at most 1048576. The same inputs give the same bits. */
 #define SOAR_NS_MAX_STEPS 16
 

@@ -219,6 +219,9 @@ cudaError_t launch_matrix_ops(const MatrixArgs& args, int source, int dest, Ctl*
 // ---- host: plans (matrix_plan.cu) ----
 // Whether a stack's shape can be planned (a stack without elements can).
 bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* why);
+// Whether fp16 holds what these coefficients make of singular values of up to 1: X's below 7.99
+// (A is held times 2^10), and B's eigenvalues up to 60 (likewise).
+bool matrix_coef_ok(const float (*coef)[3], int steps, std::string* why);
 // A stack that is written: `count` matrices of `rows` rows of `width` bytes, which do not
 // overlap one another; strides in bytes.
 struct MatrixSpan {

@@ -117,6 +117,32 @@ bool matrix_shape_ok(uint64_t count, uint64_t rows, uint64_t cols, std::string* 
     return true;
 }
 
+bool matrix_coef_ok(const float (*coef)[3], int steps, std::string* why) {
+    // X's singular values lie in [0, most], and |s p(s)| takes that to [0, its largest value there]
+    constexpr int kPoints = 4096;
+    double most = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        double next = 0.0, b = 0.0;
+        bool finite = true;
+        for (int i = 0; i <= kPoints; ++i) {
+            const double s = most * i / kPoints, q = s * s;
+            const double p = std::fabs(coef[k][0] + q * (coef[k][1] + q * static_cast<double>(coef[k][2])));
+            finite = finite && std::isfinite(p);
+            b = std::max(b, p);
+            next = std::max(next, s * p);
+        }
+        if (!finite || b > 60.0 || next >= 7.99) {
+            *why = "coefficients of step " + std::to_string(k) + ": " +
+                   (!finite   ? "not finite"
+                    : b > 60.0 ? "|a + b s^2 + c s^4| above 60 at a singular value of X"
+                               : "a singular value of X would reach 7.99");
+            return false;
+        }
+        most = next;
+    }
+    return true;
+}
+
 namespace {
 // A span's rows one after another, by their addresses.
 struct SpanRows {

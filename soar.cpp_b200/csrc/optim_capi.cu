@@ -434,6 +434,7 @@ bool muon_valid(const soar_tensor_desc* t, int n, const MuonParams& p, std::stri
         *why = "eps must be >= 0";
         return false;
     }
+    if (!soarb::matrix_coef_ok(o.coef, o.steps, why)) return false;
     std::unordered_set<const void*> taken;
     std::vector<soarb::MatrixSpan> spans;
     for (int i = 0; i < n; ++i) {

@@ -64,6 +64,8 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
     if (opts->steps < 1 || opts->steps > SOAR_NS_MAX_STEPS)
         return fail("steps must be 1 .. " + std::to_string(SOAR_NS_MAX_STEPS));
     if (!(opts->eps >= 0.0f)) return fail("eps must be >= 0");
+    std::string bad;
+    if (!soarb::matrix_coef_ok(opts->coef, opts->steps, &bad)) return fail(bad);
     const uint64_t sb = opts->src_type == SOAR_DTYPE_BF16 ? 2 : 4;
     const uint64_t db = opts->dst_type == SOAR_DTYPE_BF16 ? 2 : 4;
     std::vector<soarb::MatrixSpec> specs;
