@@ -244,7 +244,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         off = up(off + bytes, 1024);
         return at;
     };
-    uint64_t matrices = 0;
+    uint64_t matrices = 0, prep_tiles = 0;
     // A tile is one square where there are few (every SM gets some), four where there are many
     // (a sum and a ticket for 16384 elements instead of 4096).
     uint64_t squares = 0;
@@ -294,16 +294,11 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.wd = q.wd;
         s.factor = q.factor;
         s.tensor = q.tensor;
-        const uint32_t tr = (s.rows + kPrepTile - 1) / kPrepTile, tc = (s.cols + kPrepTile - 1) / kPrepTile;
-        const bool down = s.rows > s.cols;
-        const uint32_t along = down ? tr : tc, across = down ? tc : tr;
+        // (tiles lie along the longer side)
+        const uint32_t along = (s.n + kPrepTile - 1) / kPrepTile, across = (s.m + kPrepTile - 1) / kPrepTile;
         s.tiles = across * ((along + prep_parts - 1) / prep_parts);
-        s.first_tile = static_cast<uint32_t>(prep.size());
-        for (uint32_t c = 0; c < s.count; ++c)
-            for (uint32_t y = 0; y < across; ++y)
-                for (uint32_t x = 0; x < along; x += prep_parts)
-                    prep.push_back({static_cast<uint32_t>(stacks.size()), c, static_cast<uint16_t>(down ? x : y),
-                                    static_cast<uint16_t>(down ? y : x), std::min(prep_parts, along - x)});
+        s.first_tile = static_cast<uint32_t>(prep_tiles);
+        prep_tiles += static_cast<uint64_t>(s.count) * s.tiles;
         Place p{};
         const size_t xb = static_cast<size_t>(s.count) * s.m * s.ldx * 2;
         const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
@@ -321,6 +316,30 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         }
         stacks.push_back(s);
         places.push_back(p);
+    }
+    // refused before the host's tables are made, which grow with the list as the workspace does
+    size_t free_bytes = 0, all_memory = 0;
+    if ((e = cudaMemGetInfo(&free_bytes, &all_memory)) != cudaSuccess) {
+        *why = std::string("device memory: ") + cudaGetErrorString(e);
+        return nullptr;
+    }
+    if (off > all_memory) {
+        *why = "matrix workspace (" + std::to_string(off) + " bytes): more than the device's memory";
+        return nullptr;
+    }
+    if (prep_tiles > 0xFFFF0000ull || matrices > 0xFFFF0000ull) {
+        *why = "too many matrices in one list";
+        return nullptr;
+    }
+    for (uint32_t si = 0; si < stacks.size(); ++si) {
+        const NsStack& s = stacks[si];
+        const bool down = s.rows > s.cols;
+        const uint32_t along = (s.n + kPrepTile - 1) / kPrepTile, across = (s.m + kPrepTile - 1) / kPrepTile;
+        for (uint32_t c = 0; c < s.count; ++c)
+            for (uint32_t y = 0; y < across; ++y)
+                for (uint32_t x = 0; x < along; x += prep_parts)
+                    prep.push_back({si, c, static_cast<uint16_t>(down ? x : y), static_cast<uint16_t>(down ? y : x),
+                                    std::min(prep_parts, along - x)});
     }
 
     // The tasks, in an order in which every tile's inputs come before it: lists
@@ -421,7 +440,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         for (uint32_t si : by)
             for (uint32_t i = 0; i < stacks[si].count; ++i) panels.push_back(make_uint2(si, i));
     }
-    if (tasks.size() > 0xFFFF0000ull || prep.size() > 0xFFFF0000ull || matrices > 0xFFFF0000ull) {
+    if (tasks.size() > 0xFFFF0000ull) {
         *why = "too many matrices in one list";
         return nullptr;
     }

@@ -500,7 +500,11 @@ bool plan_matrices(Optim& o, const MuonParams& p, std::string* why) {
     mo.source = o.mixed ? soarb::kSrcGradBf16 : soarb::kSrcGradF32;
     mo.dest = o.mixed ? soarb::kDstParamMixed : soarb::kDstParamF32;
     mo.err = &o.ctl->error;
-    o.matrices = soarb::matrix_plan_create(specs.data(), static_cast<int>(specs.size()), mo, why);
+    try {  // (the caller has device memory to free)
+        o.matrices = soarb::matrix_plan_create(specs.data(), static_cast<int>(specs.size()), mo, why);
+    } catch (const std::exception& ex) {
+        *why = ex.what();
+    }
     return o.matrices != nullptr;
 }
 

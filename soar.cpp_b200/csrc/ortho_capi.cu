@@ -1,6 +1,7 @@
 // C-ABI of the plain orthogonalisation (include/soar_optim.h, soar_ortho_*).
 #include <cstring>
 #include <exception>
+#include <memory>
 #include <string>
 #include <unordered_set>
 #include <vector>
@@ -118,14 +119,11 @@ int create(const soar_matrix_desc* mats, int n, const soar_ortho_opts* opts, voi
     mo.source = opts->src_type == SOAR_DTYPE_BF16 ? soarb::kSrcBf16 : soarb::kSrcF32;
     mo.dest = opts->dst_type == SOAR_DTYPE_BF16 ? soarb::kDstBf16 : soarb::kDstF32;
     std::string why;
-    auto* o = new Ortho();
+    auto o = std::make_unique<Ortho>();
     o->device = opts->device;
     o->plan = soarb::matrix_plan_create(specs.data(), static_cast<int>(specs.size()), mo, &why);
-    if (!o->plan) {
-        delete o;
-        return fail(why);
-    }
-    *out = o;
+    if (!o->plan) return fail(why);
+    *out = o.release();
     return SOAR_OK;
 }
 
