@@ -43,6 +43,8 @@ namespace {
 
 template <int kSrc>
 constexpr bool kIsMuon = kSrc == kSrcGradF32 || kSrc == kSrcGradBf16;
+template <int kDst>  // (results in fp32 take three, all in k_ns)
+constexpr bool kOneProduct = kDst == kDstBf16 || kDst == kDstParamMixed;
 template <int kSrc>
 constexpr bool kIsBf16 = kSrc == kSrcBf16 || kSrc == kSrcGradBf16;
 
@@ -1968,9 +1970,10 @@ cudaError_t launch_ns(const MatrixArgs& a, const ApplyArgs& step, int sms, cudaS
     if (a.n_tasks)
         e = launch_pdl(k_ns<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_tasks, pairs))),
                        dim3(kNsThreads), kNsSmemBytes, stream, a, step);
-    if (e == cudaSuccess && a.n_panels)
-        e = launch_pdl(k_panel<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_panels, pairs))),
-                       dim3(kPanelThreads), kPanelSmemBytes, stream, a, step);
+    if constexpr (kOneProduct<kDst>)
+        if (e == cudaSuccess && a.n_panels)
+            e = launch_pdl(k_panel<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_panels, pairs))),
+                           dim3(kPanelThreads), kPanelSmemBytes, stream, a, step);
     return e;
 }
 
@@ -1982,9 +1985,7 @@ cudaError_t prepare_matrix_kernels() {
         {reinterpret_cast<const void*>(k_ns<kDstBf16>), kNsSmemBytes},
         {reinterpret_cast<const void*>(k_ns<kDstParamF32>), kNsSmemBytes},
         {reinterpret_cast<const void*>(k_ns<kDstParamMixed>), kNsSmemBytes},
-        {reinterpret_cast<const void*>(k_panel<kDstF32>), kPanelSmemBytes},
         {reinterpret_cast<const void*>(k_panel<kDstBf16>), kPanelSmemBytes},
-        {reinterpret_cast<const void*>(k_panel<kDstParamF32>), kPanelSmemBytes},
         {reinterpret_cast<const void*>(k_panel<kDstParamMixed>), kPanelSmemBytes}};
     for (const auto& f : fns) {
         const cudaError_t e = cudaFuncSetAttribute(f.first, cudaFuncAttributeMaxDynamicSharedMemorySize,
