@@ -597,7 +597,8 @@ class Muon(AdamW):
     orthogonalisation, decoupled weight decay, with the layouts, fused clip and
     loss scaler of AdamW. Every parameter is a contiguous [rows, cols] weight or
     [count, rows, cols] stack of weights that are updated one by one; other
-    parameters (biases, norms, embeddings) belong in an AdamW beside it. The
+    parameters (biases, norms, embeddings) belong in an AdamW beside it. Gradients
+    have their parameter's type and are contiguous, in its shape or flat. The
     momentum buffer is state kind STATE_M; there is no STATE_V."""
 
     def __init__(self, params, options: MuonOptions | None = None, *, layout: str = "fp32",
@@ -622,12 +623,44 @@ class Muon(AdamW):
                 raise ValueError(f"parameter {i}: not contiguous")
             shapes[i].count = p.shape[0] if p.dim() == 3 else 1
             shapes[i].rows, shapes[i].cols = p.shape[-2], p.shape[-1]
+        grads = list(grads) if grads is not None else [p.grad for p in flat]
+        self._check_tensors(flat, grads, layout, device)
 
         def create(descs, n, opts, out):
             return lib().soar_muon_create(descs, shapes, n, opts, out)
 
         self._create(params, grads, options.weight_decay, o, layout, max_grad_norm, loss_scaler,
                      device, create, "soar_muon_create")
+
+    @staticmethod
+    def _check_tensors(params, grads, layout, device) -> None:
+        """The kernels read gradients as matrices of the parameters' type and order."""
+        import torch
+        types = {"fp32": torch.float32, "bf16_mixed": torch.bfloat16}
+        if layout not in types:
+            raise ValueError(f"layout must be one of {', '.join(types)}")
+        if len(grads) != len(params):
+            raise ValueError("one gradient (or None) per parameter")
+        for i, (p, g) in enumerate(zip(params, grads)):
+            for name, t in (("parameter", p), ("gradient", g)):
+                if t is not None and t.dtype != types[layout]:
+                    raise ValueError(f"{name} {i}: layout {layout} takes {types[layout]}, not {t.dtype}")
+            if g is not None and g.shape not in (p.shape, (p.numel(),)):  # (a slice of a flat buffer is one too)
+                raise ValueError(f"gradient {i}: {tuple(g.shape)} for a parameter {tuple(p.shape)}")
+            if g is not None and not g.is_contiguous():
+                raise ValueError(f"gradient {i}: not contiguous")
+        everything = [t for t in [*params, *grads] if t is not None]
+        for t in everything:
+            if t.device.type != "cuda":
+                raise ValueError("parameters and gradients must be CUDA tensors")
+        if len({t.device for t in everything} | ({torch.device("cuda", device)} if device is not None else set())) > 1:
+            raise ValueError("parameters and gradients on more than one device, or not on `device`")
+
+    def add_grads(self, grads) -> int:
+        if len(grads) == len(self.params):  # (else the base class tells)
+            layout = "fp32" if self.layout == LAYOUT_FP32 else "bf16_mixed"
+            self._check_tensors(self.params, list(grads), layout, self.device)
+        return super().add_grads(grads)
 
 
 @dataclass
@@ -677,6 +710,8 @@ class Orthogonalizer:
             raise ValueError("matrices on more than one device")
         if device is None:
             device = everything[0].device.index if everything else 0
+        elif everything and device != everything[0].device.index:
+            raise ValueError(f"matrices on {everything[0].device}, not on device {device}")
         o.device = self.device = device
         n = len(self.srcs)
         descs = (MatrixDesc * max(n, 1))()
