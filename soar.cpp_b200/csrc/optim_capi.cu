@@ -1487,7 +1487,11 @@ SOAR_API int soar_optim_add_grads(void* handle, void* const* grads, int* out_set
         e = cudaMemcpy(gs.sumsq_chunks, ns.data(), ns.size() * sizeof(soarb::Chunk),
                        cudaMemcpyHostToDevice);
     if (e == cudaSuccess && o.muon) e = upload_matrix_grads(ng, &gs.matrix_grads);
+    // (a copy from pageable memory may return before it has landed, and the next step may be on
+    // a stream that does not wait for this one)
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);
     if (e != cudaSuccess) {
+        cudaFree(gs.matrix_grads);
         cudaFree(gs.alloc);
         return fail(std::string("gradient-set tables: ") + cudaGetErrorString(e));
     }

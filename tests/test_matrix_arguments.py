@@ -53,3 +53,24 @@ def test_on_the_device(cuda):
     flat = torch.zeros(100, device="cuda")
     sb.Muon([w], grads=[flat[10:42]]).step()
     torch.cuda.synchronize()
+
+
+@gpu
+def test_added_gradients_on_another_stream(cuda):
+    """A set that was just added, used at once by a stream that waits for no other."""
+    from matrix_helpers import matrices
+    ws = [torch.zeros(64, 96, device="cuda") for _ in range(2)]
+    gs = [matrices((64, 96), i).cuda() for i in range(6)]
+    opts = sb.MuonOptions(momentum=0.0, nesterov=False)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i, g in enumerate(gs):
+        a, b = (w.zero_() for w in ws)
+        one = sb.Muon([a], opts, grads=[gs[0]])
+        two = sb.Muon([b], opts, grads=[g])
+        torch.cuda.synchronize()
+        one.use_grads(one.add_grads([g]))
+        one.step(stream)
+        two.step(stream)
+        stream.synchronize()
+        assert torch.equal(a, b), i
