@@ -30,6 +30,7 @@
 //                   depth 320 is multiplied in 1.4 us and passed on in about
 //                   4) and by the wait from one product to the next, about 9 us.
 //   k_panel         matrices of at most 256 rows (of X), whole, by a pair each.
+//   k_few           matrices of at most 8 rows (of X), whole, by a CTA each.
 #include <algorithm>
 
 #include "matrix_ops.cuh"
@@ -1954,6 +1955,165 @@ k_panel(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs 
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// ------------------------------------------------------ matrices of few rows ---
+// k_few: the whole iteration of a matrix with at most 8 rows (of X) by one CTA. Products of 11
+// bits are off by up to 1 % there: the roundings of A's and B's few elements do not average out
+// (2 x 3: 1.0 %, 4 x 4 0.6 %, 1 x 1 0.5 %). Every X of the iteration is a polynomial P of the
+// first A times the first X, and neither P nor A has more than 8 x 8 elements. So one pass
+// over the first X (22 bits, from the L2 cache) sums A, the steps are P <- B P and A <- B A B in
+// shared memory, and a second pass writes P X. All of it in 64 bits. A <- B A B multiplies
+// the roundings in small directions of A by up to a^2 a step: where they may have grown by more
+// than 2^27, A is summed again from P X (with the usual coefficients after the eighth step). The
+// call takes 28 us for 8 x 4096 and 94 us for 200 of those, 12 us for 8 x 8 (as tiles and pairs'
+// matrices, in products of 11 bits, 153, 833 and 30).
+constexpr int kFewMost = static_cast<int>(kFewRows);
+constexpr double kFewGrowth = 0x1p27;
+struct FewShared {
+    double p[kFewMost][kFewMost], a[kFewMost][kFewMost], b[kFewMost][kFewMost], t[kFewMost][kFewMost];
+    double part[kThreads / 32][kFewMost * (kFewMost + 1) / 2];
+};
+
+// One element of the result at `at`, or Muon's update of one weight.
+template <int kDst>
+__device__ __forceinline__ void put_one(const ApplyArgs& step, const Target& s, bool ema, uint64_t at, float o) {
+    if constexpr (kDst == kDstBf16) {
+        static_cast<uint16_t*>(s.dst)[at] = f32_to_bf16_rn(o);
+    } else {
+        static_assert(kDst == kDstParamMixed, "results that take one product");
+        float w = s.master[at];
+        if (s.lr_wd != 0.0f) w = __fsub_rn(w, __fmul_rn(s.lr_wd, w));
+        w = __fsub_rn(w, __fmul_rn(s.lr_s, o));
+        s.master[at] = w;
+        static_cast<uint16_t*>(s.dst)[at] = f32_to_bf16_rn(w);
+        if (ema) s.ema[at] = __fadd_rn(__fmul_rn(step.ema_decay, s.ema[at]), __fmul_rn(step.ema_omd, w));
+    }
+}
+
+// (kRows: m, or the next power of two; rows that X does not have are zeros)
+template <int kDst, int kRows>
+__device__ __forceinline__ void few_rows(const MatrixArgs& a, const ApplyArgs& step, const NsStack& s, uint32_t index,
+                                         FewShared& sh) {
+    constexpr int kPairs = kRows * (kRows + 1) / 2;
+    using Square = double[kFewMost][kFewMost];
+    const uint32_t m = s.m, n = s.n, ldx = s.ldx;
+    const uint64_t base = static_cast<uint64_t>(index) * m * ldx;
+    const __half *hi = s.x[0] + base, *lo = s.xl[0] + base;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool mine = threadIdx.x < kRows * kRows;  // an element of P, A and B
+    const int ti = threadIdx.x / kRows, tk = threadIdx.x % kRows;
+    auto read = [&](uint32_t j, double (&x)[kRows]) {
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+            const uint32_t at = k * ldx + j;
+            x[k] = k < m ? static_cast<double>(__half2float(hi[at]) + __half2float(lo[at])) : 0.0;
+        }
+    };
+    auto times_p = [&](const double (&x)[kRows], double (&y)[kRows]) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            y[i] = 0.0;
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) y[i] = fma(sh.p[i][k], x[k], y[i]);
+        }
+    };
+    // this thread's element of a product
+    auto element = [&](const Square& p, const Square& q) {
+        double v = 0.0;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) v = fma(p[ti][k], q[k][tk], v);
+        return v;
+    };
+    // A = f (P X)(P X)^T, or f X X^T, in a fixed order
+    auto sum_a = [&](bool first, double f) {
+        double sum[kPairs];
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) sum[e] = 0.0;
+#pragma unroll 1
+        for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+            double x[kRows];
+            read(j, x);
+            if (!first) {
+                double y[kRows];
+                times_p(x, y);
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) x[i] = y[i];
+            }
+#pragma unroll
+            for (int i = 0, e = 0; i < kRows; ++i)
+#pragma unroll
+                for (int k = 0; k <= i; ++k, ++e) sum[e] = fma(x[i], x[k], sum[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < kPairs; ++e) {
+            sum[e] = warp_sum(sum[e]);
+            if (lane == 0) sh.part[warp][e] = sum[e];
+        }
+        __syncthreads();
+        if (mine) {
+            const int i = ti > tk ? ti : tk, k = ti > tk ? tk : ti;
+            double v = 0.0;
+#pragma unroll
+            for (int w = 0; w < kThreads / 32; ++w) v += sh.part[w][i * (i + 1) / 2 + k];
+            sh.a[ti][tk] = f * v;
+        }
+    };
+    const double one_over = a.hold[(static_cast<uint64_t>(s.first) + index) * a.steps].inv;
+    if (mine) sh.p[ti][tk] = ti == tk ? one_over : 0.0;
+    sum_a(true, one_over * one_over);
+    __syncthreads();
+    double growth = 1.0;
+#pragma unroll 1
+    for (int it = 0; it < a.steps; ++it) {
+        const double ca = a.coef[it][0], cb = a.coef[it][1], cc = a.coef[it][2];
+        if (mine) sh.b[ti][tk] = cb * sh.a[ti][tk] + cc * element(sh.a, sh.a) + (ti == tk ? ca : 0.0);
+        __syncthreads();
+        const double p = mine ? element(sh.b, sh.p) : 0.0;
+        if (mine) sh.t[ti][tk] = element(sh.b, sh.a);
+        __syncthreads();
+        if (mine) sh.p[ti][tk] = p;
+        growth *= ca * ca > 1.0 ? ca * ca : 1.0;
+        if (growth <= kFewGrowth) {
+            if (mine) sh.a[ti][tk] = element(sh.t, sh.b);
+        } else if (it + 1 < a.steps) {
+            __syncthreads();
+            sum_a(false, 1.0);
+            growth = 1.0;
+        }
+        __syncthreads();
+    }
+    const Target target = target_of<kDst>(s, index, step, a.ema != 0);
+    const uint64_t across = s.transposed ? 1 : target.pitch, along = s.transposed ? target.pitch : 1;
+#pragma unroll 1
+    for (uint32_t j = threadIdx.x; j < n; j += kThreads) {
+        double x[kRows], y[kRows];
+        read(j, x);
+        times_p(x, y);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (i < m) put_one<kDst>(step, target, a.ema != 0, target.base + i * across + j * along, static_cast<float>(y[i]));
+    }
+    __syncthreads();  // (the next matrix writes P)
+}
+
+template <int kDst>
+__global__ void __launch_bounds__(kThreads, 2)
+k_few(const __grid_constant__ MatrixArgs a, const __grid_constant__ ApplyArgs step) {
+    __shared__ FewShared sh;
+    pdl_wait();
+    pdl_trigger();
+    if constexpr (kDst == kDstParamMixed) {
+        if (a.step->skip) return;
+    }
+    for (uint32_t q = blockIdx.x; q < a.n_few; q += gridDim.x) {
+        const uint2 f = a.few[q];
+        const NsStack& s = a.stacks[f.x];
+        if (s.m == 1) few_rows<kDst, 1>(a, step, s, f.y, sh);
+        else if (s.m == 2) few_rows<kDst, 2>(a, step, s, f.y, sh);
+        else if (s.m <= 4) few_rows<kDst, 4>(a, step, s, f.y, sh);
+        else few_rows<kDst, 8>(a, step, s, f.y, sh);
+    }
+}
+
 template <int kSrc>
 cudaError_t launch_prep(const MatrixArgs& a, Ctl* ctl, const ApplyArgs& step, int sms,
                         cudaStream_t stream) {
@@ -1970,10 +2130,14 @@ cudaError_t launch_ns(const MatrixArgs& a, const ApplyArgs& step, int sms, cudaS
     if (a.n_tasks)
         e = launch_pdl(k_ns<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_tasks, pairs))),
                        dim3(kNsThreads), kNsSmemBytes, stream, a, step);
-    if constexpr (kOneProduct<kDst>)
+    if constexpr (kOneProduct<kDst>) {
         if (e == cudaSuccess && a.n_panels)
             e = launch_pdl(k_panel<kDst>, dim3(2 * static_cast<unsigned>(std::min<uint64_t>(a.n_panels, pairs))),
                            dim3(kPanelThreads), kPanelSmemBytes, stream, a, step);
+        if (e == cudaSuccess && a.n_few)
+            e = launch_pdl(k_few<kDst>, dim3(static_cast<unsigned>(std::min<uint64_t>(a.n_few, 2ull * sms))),
+                           dim3(kThreads), 0, stream, a, step);
+    }
     return e;
 }
 

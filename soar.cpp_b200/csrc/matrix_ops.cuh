@@ -14,7 +14,8 @@
 // a factor of a (3.4) per iteration: with X in hi alone, a matrix of a few
 // strong directions over noise comes out 0.6 % to 7 % off (bf16 operands: 5 %
 // to 60 %), with hi + lo 0.04 % to 0.25 %, about what the rounding of a bf16
-// result costs (0.17 % rms). For fp32 results lo is an fp16 number too, of A and B as
+// result costs (0.17 % rms); with fewer than 64 rows, whose roundings average out
+// less, up to 0.4 %, and with at most 8 it would be up to 1 %: those are worked on in 64 bits. For fp32 results lo is an fp16 number too, of A and B as
 // well, and every product is taken as hi hi + hi lo + lo hi (22 bits). The tensor
 // cores round a sum towards zero at each addition, so there the large terms come
 // last and half of them have an accumulator of their own (2048 x 2048: 4.6e-6 off
@@ -81,6 +82,10 @@ constexpr uint32_t kPanelBlockBytes = 4 * 64 * 64 * 2;  // a CTA's 64 columns of
 constexpr size_t kPanelSmemBytes =
     8 * 2 * kNsBoxBytes + 2 * kPanelBlockBytes + 4 * kLoBytes + 1024;
 
+// Matrices with at most this many rows (of X) whose result takes one product go to k_few, in
+// 64 bits on the ordinary cores.
+constexpr uint32_t kFewRows = 8;
+
 // Tensor maps of a stack. Operand rows run along a product's depth ("K": boxes
 // of 64 columns of 128 or 64 rows) except X in B X, whose columns are taken
 // ("N": boxes of 64 rows of two or one groups of 64 columns). The lo parts'
@@ -117,8 +122,9 @@ struct NsStack {
     uint32_t count;
     uint32_t first;       // index of its first matrix in the plan
     uint32_t transposed;  // rows > cols: X is the transpose
-    uint32_t three;       // products in three parts
+    uint32_t three;       // X in 22 bits (and products in three parts)
     uint32_t panel;       // worked on by k_panel
+    uint32_t few;         // worked on by k_few
     uint32_t tiles;       // preparation tiles per matrix
     uint32_t first_tile;
     float sx, one_over_sx;  // power of two X is held by at least (NsHold)
@@ -184,6 +190,8 @@ struct MatrixArgs {
     uint32_t n_tasks;
     const uint2* panels;   // k_panel's matrices: stack, matrix of the stack
     uint32_t n_panels;
+    const uint2* few;      // k_few's
+    uint32_t n_few;
     const PrepTile* prep;
     uint32_t n_prep;
     uint32_t n_matrices;

@@ -258,7 +258,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     // 731 and 906. So long matrices go to k_panel where the list has enough columns for all pairs.
     uint64_t panel_columns = 0;
     for (int i = 0; i < n_specs; ++i)
-        if (!three && specs[i].rows && specs[i].cols && std::min(specs[i].rows, specs[i].cols) <= kPanelSide)
+        if (const uint64_t m = std::min(specs[i].rows, specs[i].cols); !three && m > kFewRows && m <= kPanelSide)
             panel_columns += specs[i].count * std::max(specs[i].rows, specs[i].cols);
     const uint64_t panel_most = std::max<uint64_t>(kPanelAnyColumns, 2 * panel_columns / std::max(1, plan->sms / 2));
     const uint32_t prep_parts = squares >= 16ull * static_cast<uint64_t>(plan->sms) ? 4 : 1;
@@ -270,10 +270,11 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         s.cols = static_cast<uint32_t>(q.cols);
         s.count = static_cast<uint32_t>(q.count);
         s.transposed = s.rows > s.cols;
-        s.three = three;
         s.m = std::min(s.rows, s.cols);
         s.n = std::max(s.rows, s.cols);
-        s.panel = !three && s.m <= kPanelSide && s.n <= panel_most;
+        s.few = !three && s.m <= kFewRows;
+        s.three = three || s.few;
+        s.panel = !s.three && s.m <= kPanelSide && s.n <= panel_most;
         s.ldx = static_cast<uint32_t>(up(s.n, 64));
         s.lda = static_cast<uint32_t>(up(s.m, 8));
         s.first = static_cast<uint32_t>(matrices);
@@ -302,11 +303,11 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         Place p{};
         const size_t xb = static_cast<size_t>(s.count) * s.m * s.ldx * 2;
         const size_t ab = static_cast<size_t>(s.count) * s.m * s.lda * 2;
-        for (int k = 0; k < 2; ++k) {
+        for (int k = 0; k < (s.few ? 1 : 2); ++k) {
             p.x[k] = take(xb);
-            p.xl[k] = take(three ? xb : xb / 2);
+            p.xl[k] = take(s.three ? xb : xb / 2);
         }
-        if (!s.panel) {
+        if (!s.panel && !s.few) {
             p.a = take(ab);
             p.b = take(ab);
         }
@@ -405,12 +406,12 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     };
     uint64_t all_bytes = 0;
     for (const NsStack& s : stacks)
-        if (!s.panel) all_bytes += s.count * bytes_of(s);
+        if (!s.panel && !s.few) all_bytes += s.count * bytes_of(s);
     const uint64_t wave_most = all_bytes / std::max<uint64_t>(1, all_bytes / kWaveBytes) + 1;
     uint64_t tiles_in_wave = 0;
     for (uint32_t si = 0; si < stacks.size(); ++si) {
         const NsStack& s = stacks[si];
-        if (s.panel) continue;
+        if (s.panel || s.few) continue;
         const uint64_t each = bytes_of(s);
         const uint64_t tiles = product_tiles(s, kNsXXt, kNsTileN).size();
         for (uint32_t i = 0; i < s.count;) {
@@ -430,15 +431,16 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
         }
     }
     flush();
-    // k_panel's matrices, the longest first
-    std::vector<uint2> panels;
+    // k_panel's and k_few's matrices, the longest first
+    std::vector<uint2> panels, few;
     {
         std::vector<uint32_t> by;
         for (uint32_t si = 0; si < stacks.size(); ++si)
-            if (stacks[si].panel) by.push_back(si);
+            if (stacks[si].panel || stacks[si].few) by.push_back(si);
         std::stable_sort(by.begin(), by.end(), [&](uint32_t x, uint32_t y) { return stacks[x].n > stacks[y].n; });
         for (uint32_t si : by)
-            for (uint32_t i = 0; i < stacks[si].count; ++i) panels.push_back(make_uint2(si, i));
+            for (uint32_t i = 0; i < stacks[si].count; ++i)
+                (stacks[si].few ? few : panels).push_back(make_uint2(si, i));
     }
     if (tasks.size() > 0xFFFF0000ull) {
         *why = "too many matrices in one list";
@@ -452,6 +454,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     const size_t o_tasks = take(tasks.size() * sizeof(NsTask));
     const size_t o_prep = take(prep.size() * sizeof(PrepTile));
     const size_t o_panels = take(panels.size() * sizeof(uint2));
+    const size_t o_few = take(few.size() * sizeof(uint2));
     const size_t tables_end = off;
     const size_t o_partials = take(prep.size() * sizeof(double));
     const size_t o_inv = take(matrices * sizeof(float2));
@@ -488,7 +491,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
                  encode_groups(encoder, qx + kMapN + kMap64, s.x[k], s.m, s.ldx, s.count, 1) &&
                  encode_lo8(encoder, qx + kMapLo, s.xl[k], s.m, s.n, s.ldx, s.count);
         }
-        for (int lo = 0; !s.panel && lo < 2; ++lo) {
+        for (int lo = 0; !s.panel && !s.few && lo < 2; ++lo) {
             CUtensorMap* q = m + (lo ? kMapLo : 0);
             for (int k = 0; k < 2; ++k) {
                 __half* x = lo ? s.xl[k] : s.x[k];
@@ -517,6 +520,7 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     put(o_tasks, tasks.data(), tasks.size() * sizeof(NsTask));
     put(o_prep, prep.data(), prep.size() * sizeof(PrepTile));
     put(o_panels, panels.data(), panels.size() * sizeof(uint2));
+    put(o_few, few.data(), few.size() * sizeof(uint2));
     if (ok) {
         e = cudaMemset(plan->slab, 0, operand_bytes);
         if (e == cudaSuccess) e = cudaMemcpy(at(operand_bytes), host.data(), host.size(), cudaMemcpyHostToDevice);
@@ -537,6 +541,8 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     a.n_prep = static_cast<uint32_t>(prep.size());
     a.panels = reinterpret_cast<const uint2*>(at(o_panels));
     a.n_panels = static_cast<uint32_t>(panels.size());
+    a.few = reinterpret_cast<const uint2*>(at(o_few));
+    a.n_few = static_cast<uint32_t>(few.size());
     a.steps = opts.steps;
     a.n_matrices = static_cast<uint32_t>(matrices);
     a.partials = reinterpret_cast<double*>(at(o_partials));
