@@ -161,7 +161,7 @@ SOAR_API int soar_sgd_create(const soar_tensor_desc* tensors, int n_tensors,
    matrix of zeros gives zeros; one with an inf or NaN gives NaN throughout.
    The products run with fp16 operands (11 bits, scaled by powers of two) and
    fp32 sums, X being carried in 14 bits: 0.04 % to 0.25 % off in norm, with a
-   shorter side of 9 to 63 up to 0.4 % (one of up to 8 goes in 64 bits). Where
+   shorter side of 9 to 63 up to 0.5 % (one of up to 8 goes in 64 bits). Where
    the result is fp32 (fp32 destinations, SOAR_LAYOUT_FP32) X and the products'
    operands have 22 bits and every product is taken in three parts, about as
    exact as fp32 products (sides up to about 2048; the sums' rounding grows with

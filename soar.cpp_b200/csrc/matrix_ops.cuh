@@ -15,7 +15,7 @@
 // strong directions over noise comes out 0.6 % to 7 % off (bf16 operands: 5 %
 // to 60 %), with hi + lo 0.04 % to 0.25 %, about what the rounding of a bf16
 // result costs (0.17 % rms); with fewer than 64 rows, whose roundings average out
-// less, up to 0.4 %, and with at most 8 it would be up to 1 %: those are worked on in 64 bits. For fp32 results lo is an fp16 number too, of A and B as
+// less, up to 0.5 %, and with at most 8 it would be up to 1 %: those are worked on in 64 bits. For fp32 results lo is an fp16 number too, of A and B as
 // well, and every product is taken as hi hi + hi lo + lo hi (22 bits). The tensor
 // cores round a sum towards zero at each addition, so there the large terms come
 // last and half of them have an accumulator of their own (2048 x 2048: 4.6e-6 off
