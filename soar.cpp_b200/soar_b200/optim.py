@@ -613,6 +613,8 @@ class Muon(AdamW):
         o.nesterov, o.scale = int(options.nesterov), MUON_SCALES[options.scale]
         o.steps, o.eps = options.steps, options.eps
         _fill_coef(o.coef, options.coefficients, options.steps)
+        # (taken apart here and again below: either may be an iterator, as model.parameters() is)
+        params = [ParamGroup(list(p.params), p.weight_decay, p.extra) if isinstance(p, ParamGroup) else p for p in params]
         flat = [q for p in params for q in (p.params if isinstance(p, ParamGroup) else [p])]
         shapes = (MatrixShape * max(len(flat), 1))()
         for i, p in enumerate(flat):

@@ -25,6 +25,19 @@ def test_muon_refuses(param, grad, layout, word):
         sb.Muon([param], grads=[grad], layout=layout)
 
 
+def test_muon_takes_iterators(monkeypatch):
+    """As model.parameters() is one: every parameter reaches the library."""
+    ps = [torch.nn.Parameter(torch.zeros(4, 8)) for _ in range(3)]
+    seen = []
+    monkeypatch.setattr(sb.Muon, "_check_tensors", staticmethod(lambda *a: None))
+    monkeypatch.setattr(sb.Muon, "_create", lambda self, params, grads, *a: seen.append((
+        [q for p in params for q in (p.params if isinstance(p, sb.ParamGroup) else [p])], list(grads))))
+    sb.Muon(iter(ps))
+    sb.Muon([sb.ParamGroup(iter(ps[:2]), 0.1), ps[2]], grads=iter([None] * 3))
+    for params, grads in seen:
+        assert all(a is b for a, b in zip(params, ps)) and len(params) == len(grads) == 3
+
+
 def test_muon_refuses_a_grad_attribute_of_another_order():
     p = torch.nn.Parameter(torch.zeros(4, 8))
     p.grad = torch.zeros(4, 8).as_strided((4, 8), (1, 4))
