@@ -179,7 +179,8 @@ enum soar_dtype {
 
 /* A stack of `count` rows x cols matrices. Elements of a row are adjacent;
    strides are in elements: `*_row` between rows, `*_mat` between matrices.
-   Destinations of a list may interleave, but not share elements. */
+   Destinations of a list may interleave, but not share elements. Every source is
+   read before a result is written, so they may lie in any of the sources. */
 typedef struct soar_matrix_desc {
     const void* src;    /* device; read only */
     void* dst;          /* device; may be src itself (same type and strides) */
@@ -237,7 +238,12 @@ enum soar_muon_scale {
    The handle works with every soar_optim_* call as an AdamW handle does (step,
    zero_grad, clip, lr, info, state: MASTER and M, gradient sets, checkpoint,
    EMA, grad_sumsq / apply, destroy). Not with soar_zero1_create: a shard of
-   the flat buffers does not hold whole matrices. Fill with
+   the flat buffers does not hold whole matrices. create() allocates the state
+   (the momentum; in the mixed layout the fp32 master weights) and the
+   orthogonalisation's workspace for the whole list: 6 bytes per element and 4 per
+   element of the m x m products, 8 and 8 in the fp32 layout (padded as
+   soar_ortho_create's). After an error (soar_step_info.error) the weights are partly
+   those of the step before: restore a checkpoint. Fill with
    soar_muon_default_opts() first. */
 typedef struct soar_muon_opts {
     float lr;               /* 2e-2 */

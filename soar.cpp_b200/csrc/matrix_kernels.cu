@@ -5,10 +5,10 @@
 //                   sums, in a fixed order); in a Muon step the same pass
 //                   unscales and clips the gradient, updates the momentum and
 //                   takes the step's decision. Bound by memory: 200M mixed
-//                   parameters, 10 bytes each, 338 us (5.9 TB/s).
+//                   parameters, 10 bytes each, 338 to 347 us (5.9 TB/s).
 //   k_matrix_split  X = G / (|G| + eps) as fp16 hi and lo, transposed where the
 //                   matrix has more rows than columns. Bound by memory: the
-//                   same parameters, 9 bytes each, 372 us (4.8 TB/s).
+//                   same parameters, 9 bytes each, 371 to 401 us (4.7 TB/s).
 //   k_ns            every product of every matrix in one persistent kernel, a
 //                   pair of CTAs to an SM pair. Pairs take tiles from one list
 //                   in order; the list holds the products in an order in which

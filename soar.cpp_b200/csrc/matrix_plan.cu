@@ -347,13 +347,13 @@ MatrixPlan* matrix_plan_create(const MatrixSpec* specs, int n_specs, const Matri
     // ("waves") of matrices go through their products side by side, one list
     // after another, all about as long. A product's last tiles are waited for by
     // the first ones of its matrix's next product, for some 10 us, which the other
-    // matrices of the list have to fill: with 64 MB in a list 46M parameters in
-    // matrices of many shapes took 1573 us a step, with 128 MB and more 1414, and a
-    // short last list cost 80. Nor does the L2 cache ask for short ones (200M
-    // parameters in layers 1024 wide: 5.94 ms with 64 MB, 5.87 with 256 MB). A
-    // list of few tiles is drawn out until a product of it occupies every pair of
-    // CTAs three times (that model with lists by tiles alone: 6.40, 6.00, 5.69 ms
-    // at one, two and three times).
+    // matrices of the list have to fill: with 32, 64 and 128 MB in a list 46M
+    // parameters in matrices of many shapes take 1682, 1369 and 1313 us a step, with
+    // more no less. Nor does the L2 cache ask for short ones. A list of few tiles is
+    // drawn out until a product of it occupies every pair of CTAs three times: 200M
+    // parameters in layers 1024 wide take 5.70, 5.67, 5.62 and 5.69 ms with 64, 128, 256
+    // and 512 MB, all of them in one list 5.70, and with a product that occupies the pairs
+    // once 6.15, 5.88, 5.75 and 5.67. (The 46M in lists of 64 MB lose 29 us by it.)
     constexpr uint64_t kWaveBytes = 256ull << 20;
     const uint64_t wave_tiles = 3 * static_cast<uint64_t>(plan->sms) / 2;
     std::vector<NsTask> tasks;
